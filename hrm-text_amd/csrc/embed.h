@@ -1,0 +1,311 @@
+// Scaled embedding lookup and the gradient of its table (models/lm_head.py:34-43).
+//
+//   y_i = round(s * T[id_i]),   dT_v = round(s * sum over i with id_i = v, in the order of i, of dy_i)
+//
+// The gradient needs the tokens grouped by id: a stable radix sort of (id, i), then one pass over
+// the sorted tokens that adds the rows of each run in fp32. Stable, so every sum has one order and
+// the result is bitwise deterministic; no atomics touch floating-point data.
+#pragma once
+#include "common.h"
+
+namespace prefixlm {
+namespace emb {
+
+// 8 consecutive elements of a row, 16-byte aligned
+template <class T>
+struct Row8;
+template <>
+struct Row8<bf16> {
+  u32x4 w;
+  __device__ __forceinline__ void load(const bf16* p) { w = *reinterpret_cast<const u32x4*>(p); }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[2 * e] = bf16lo(w[e]);
+      f[2 * e + 1] = bf16hi(w[e]);
+    }
+  }
+  __device__ static __forceinline__ void store(bf16* p, const float* f) {
+    *reinterpret_cast<bf16x8*>(p) = cvt8(f[0], f[1], f[2], f[3], f[4], f[5], f[6], f[7]);
+  }
+};
+template <>
+struct Row8<float> {
+  f32x4 w[2];
+  __device__ __forceinline__ void load(const float* p) {
+    w[0] = reinterpret_cast<const f32x4*>(p)[0];
+    w[1] = reinterpret_cast<const f32x4*>(p)[1];
+  }
+  __device__ __forceinline__ void get(float* f) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = w[e >> 2][e & 3];
+  }
+  __device__ static __forceinline__ void store(float* p, const float* f) {
+    reinterpret_cast<f32x4*>(p)[0] = f32x4{f[0], f[1], f[2], f[3]};
+    reinterpret_cast<f32x4*>(p)[1] = f32x4{f[4], f[5], f[6], f[7]};
+  }
+};
+
+struct FwdParams {
+  const void* table;
+  const void* ids;
+  void* y;
+  int64_t table_st, y_st, T, V;
+  int cols, wide_ids;
+  float scale;
+};
+__device__ __forceinline__ int64_t id_of(const void* ids, int wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(ids)[i] : (int64_t) static_cast<const int32_t*>(ids)[i];
+}
+
+// thread = 8 columns of one token's row. Ids outside the table give NaN rows.
+template <class TT, class TY>
+__global__ __launch_bounds__(256) void lookup_kernel(FwdParams P) {
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int c8 = P.cols >> 3;
+  const int64_t i = idx / c8;
+  if (i >= P.T) return;
+  const int c = (int)(idx - i * c8) * 8;
+  const int64_t id = id_of(P.ids, P.wide_ids, i);
+  float f[8];
+  if (id >= 0 && id < P.V) {
+    Row8<TT> r;
+    r.load(static_cast<const TT*>(P.table) + id * P.table_st + c);
+    r.get(f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = __builtin_nanf("");
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] *= P.scale;
+  Row8<TY>::store(static_cast<TY*>(P.y) + i * P.y_st + c, f);
+}
+
+// ---- the gradient ----------------------------------------------------------------------------
+constexpr int kBits = 9, kBins = 1 << kBits;   // a digit; two cover 2^18 ids
+constexpr int kSortThreads = 256, kSortWaves = kSortThreads / 64;
+constexpr int kMaxTiles = 128;
+constexpr int kRun = 64;                       // sorted tokens per wave of the sum
+
+struct SortParams {
+  const void* ids;          // first pass: the caller's ids; else null
+  const uint32_t* key_in;   // later passes
+  const uint32_t* pos_in;
+  uint32_t* key_out;
+  uint32_t* pos_out;
+  uint32_t* hist;           // [tiles, kBins]
+  void* zero;               // rows to clear beside the sort, and this launch's share of them
+  int64_t zero_begin, zero_end;   // in 16-byte units
+  int64_t T, V, padding;
+  int wide_ids, tile, tiles, shift;
+};
+
+// The id as a sort key; ids without a gradient (outside the table, or the padding id) come last
+__device__ __forceinline__ uint32_t key_at(const SortParams& P, int64_t i) {
+  if (!P.ids) return P.key_in[i];
+  const int64_t id = id_of(P.ids, P.wide_ids, i);
+  return id >= 0 && id < P.V && id != P.padding ? (uint32_t)id : (uint32_t)P.V;
+}
+
+// Workgroups past the sort's clear the gradient: the sort is a chain of short launches that leaves
+// the memory idle, and the clearing needs nothing from it.
+__device__ __forceinline__ bool clears(const SortParams& P) {
+  const int b = (int)blockIdx.x - P.tiles;
+  if (b < 0) return false;
+  const int64_t n = (int64_t)(gridDim.x - P.tiles) * kSortThreads;
+  const u32x4 z = {0u, 0u, 0u, 0u};
+  for (int64_t i = P.zero_begin + (int64_t)b * kSortThreads + threadIdx.x; i < P.zero_end; i += n)
+    __builtin_nontemporal_store(z, static_cast<u32x4*>(P.zero) + i);
+  return true;
+}
+
+// How many of each digit a tile holds
+__global__ __launch_bounds__(kSortThreads) void histogram_kernel(SortParams P) {
+  if (clears(P)) return;
+  __shared__ uint32_t n[kBins];
+  for (int d = threadIdx.x; d < kBins; d += kSortThreads) n[d] = 0;
+  __syncthreads();
+  const int64_t i0 = (int64_t)blockIdx.x * P.tile, i1 = i0 + P.tile < P.T ? i0 + P.tile : P.T;
+  for (int64_t i = i0 + threadIdx.x; i < i1; i += kSortThreads)
+    atomicAdd(&n[(key_at(P, i) >> P.shift) & (kBins - 1)], 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < kBins; d += kSortThreads) P.hist[(int64_t)blockIdx.x * kBins + d] = n[d];
+}
+
+// Moves a tile's tokens to their places by one digit, keeping their order: the place is the number
+// of tokens with a lower digit, plus those of the same digit in earlier tiles, in earlier waves'
+// parts of this tile, and before it in its wave's part.
+__global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortParams P) {
+  if (clears(P)) return;
+  static_assert(kBins == 2 * kSortThreads, "a thread has two digits");
+  __shared__ uint32_t place[kSortWaves][kBins];
+  __shared__ uint32_t wave_sum[kSortWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t i0 = (int64_t)blockIdx.x * P.tile, i1 = i0 + P.tile < P.T ? i0 + P.tile : P.T;
+  const int part = P.tile / kSortWaves;                     // a multiple of 64
+  const int64_t w0 = i0 + (int64_t)wave * part, w1 = w0 + part < i1 ? w0 + part : i1;
+  for (int d = tid; d < kSortWaves * kBins; d += kSortThreads) (&place[0][0])[d] = 0;
+  __syncthreads();
+  for (int64_t i = w0 + lane; i < w1; i += 64) atomicAdd(&place[wave][(key_at(P, i) >> P.shift) & (kBins - 1)], 1u);
+  // digits 2 tid and 2 tid + 1: all tiles' tokens, and those of earlier tiles
+  uint32_t all[2] = {0, 0}, before[2] = {0, 0};
+  for (int b = 0; b < P.tiles; ++b) {
+    const u32x2 h = reinterpret_cast<const u32x2*>(P.hist + (int64_t)b * kBins)[tid];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      all[e] += h[e];
+      if (b < (int)blockIdx.x) before[e] += h[e];
+    }
+  }
+  uint32_t sum = all[0] + all[1];
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const uint32_t y = __shfl_up(sum, m);
+    if (lane >= m) sum += y;
+  }
+  if (lane == 63) wave_sum[wave] = sum;
+  __syncthreads();   // the waves' counts too
+  uint32_t low = sum - all[0] - all[1];
+  for (int g = 0; g < wave; ++g) low += wave_sum[g];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    uint32_t at = low + before[e];
+    if (e) at += all[0];
+#pragma unroll
+    for (int g = 0; g < kSortWaves; ++g) {
+      const uint32_t n = place[g][2 * tid + e];
+      place[g][2 * tid + e] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  // each wave takes 64 tokens at a time; lanes with one digit share its place
+  for (int64_t i = w0; i < w1; i += 64) {
+    const bool in = i + lane < w1;
+    const uint32_t key = in ? key_at(P, i + lane) : 0;
+    const uint32_t digit = (key >> P.shift) & (kBins - 1);
+    unsigned long long same = __builtin_amdgcn_ballot_w64(in);
+#pragma unroll
+    for (int b = 0; b < kBits; ++b) {
+      const unsigned long long ones = __builtin_amdgcn_ballot_w64((digit >> b) & 1);
+      same &= (digit >> b) & 1 ? ones : ~ones;
+    }
+    if (in) {
+      const int rank = __builtin_popcountll(same & ((1ull << lane) - 1));
+      const uint32_t at = place[wave][digit] + (uint32_t)rank;
+      P.key_out[at] = key;
+      P.pos_out[at] = P.ids ? (uint32_t)(i + lane) : P.pos_in[i + lane];
+    }
+    __builtin_amdgcn_wave_barrier();
+    // the last lane of each digit moves its place on
+    if (in && (same >> lane) == 1ull) place[wave][digit] += (uint32_t)__builtin_popcountll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+struct SumParams {
+  const uint32_t* key;
+  const uint32_t* pos;
+  const void* dy;
+  void* grad;
+  float* part;              // [chunks, 2, cols]: the runs that a chunk's first and last token belong to
+  int64_t dy_st, T, V;
+  int cols, chunks;
+  float scale;
+};
+
+// Wave = (chunk of kRun sorted tokens, 512 columns). Runs that lie inside the chunk are written; a
+// run that goes on in a neighbour leaves its sum in `part` (slot 0: the run the chunk begins with,
+// if it began earlier; slot 1: the run that goes on behind it, if it began here).
+template <class TY, class TG>
+__global__ __launch_bounds__(256) void sum_kernel(SumParams P) {
+  const int cblk = (P.cols + 511) / 512, lane = threadIdx.x & 63;
+  const int64_t w = __builtin_amdgcn_readfirstlane((int)((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const int chunk = (int)(w / cblk);
+  if (chunk >= P.chunks) return;
+  const int c = (int)(w - (int64_t)chunk * cblk) * 512 + lane * 8;
+  const bool on = c < P.cols;
+  const int64_t t0 = (int64_t)chunk * kRun;
+  const int n = (int)(P.T - t0 < kRun ? P.T - t0 : kRun);
+  const uint32_t key = lane < n ? P.key[t0 + lane] : (uint32_t)P.V;
+  const uint32_t pos = lane < n ? P.pos[t0 + lane] : 0;
+  const uint32_t prev = t0 > 0 ? P.key[t0 - 1] : 0xffffffffu;
+  const uint32_t next = t0 + kRun < P.T ? P.key[t0 + kRun] : 0xffffffffu;
+  float acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  bool first = true;                 // still in the run that the chunk begins with
+  const TY* dy = static_cast<const TY*>(P.dy) + c;
+  constexpr int kAhead = 8;
+  for (int t = 0; t < n; t += kAhead) {
+    Row8<TY> r[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t p = (uint32_t)__builtin_amdgcn_readlane((int)pos, t + u < n ? t + u : t);
+      if (on) r[u].load(dy + p * P.dy_st);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (t + u >= n) break;
+      const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key, t + u);
+      if (k >= (uint32_t)P.V) return;   // the last ones have no gradient
+      float f[8];
+      if (on) r[u].get(f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += f[e];
+      const bool last = t + u == n - 1;
+      const uint32_t k1 = last ? next : (uint32_t)__builtin_amdgcn_readlane((int)key, t + u + 1);
+      if (k1 == k && !last) continue;
+      const bool from_before = first && k == prev, goes_on = k1 == k;
+      if (on) {
+        if (from_before || goes_on) {
+          float* p = P.part + ((int64_t)chunk * 2 + (from_before ? 0 : 1)) * P.cols + c;
+          Row8<float>::store(p, acc);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] *= P.scale;
+          Row8<TG>::store(static_cast<TG*>(P.grad) + (int64_t)k * P.cols + c, acc);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+      first = false;
+    }
+  }
+}
+
+// Wave = (chunk, 512 columns): the run that goes on behind the chunk, if it began there, is added up
+// over the following chunks, in order.
+template <class TG>
+__global__ __launch_bounds__(256) void join_kernel(SumParams P) {
+  const int cblk = (P.cols + 511) / 512, lane = threadIdx.x & 63;
+  const int64_t w = __builtin_amdgcn_readfirstlane((int)((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)));
+  const int chunk = (int)(w / cblk);
+  if (chunk >= P.chunks - 1) return;
+  const int c = (int)(w - (int64_t)chunk * cblk) * 512 + lane * 8;
+  const int64_t t1 = (int64_t)(chunk + 1) * kRun;   // the next chunk's first token
+  const uint32_t k = P.key[t1 - 1];
+  if (k >= (uint32_t)P.V || P.key[t1] != k) return;
+  if (chunk > 0 && P.key[t1 - kRun] == k && P.key[t1 - kRun - 1] == k) return;   // it began earlier
+  if (c >= P.cols) return;
+  // the chunks after this one that it reaches
+  int end = chunk + 2;
+  while (end < P.chunks && P.key[(int64_t)end * kRun] == k && P.key[(int64_t)end * kRun - 1] == k) ++end;
+  float acc[8];
+  Row8<float> r;
+  r.load(P.part + ((int64_t)chunk * 2 + 1) * P.cols + c);
+  r.get(acc);
+  for (int g = chunk + 1; g < end; ++g) {
+    float f[8];
+    r.load(P.part + (int64_t)g * 2 * P.cols + c);
+    r.get(f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += f[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] *= P.scale;
+  Row8<TG>::store(static_cast<TG*>(P.grad) + (int64_t)k * P.cols + c, acc);
+}
+
+}  // namespace emb
+}  // namespace prefixlm

@@ -630,6 +630,8 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
 // once); then each half-wave adds every other split's o, lane % 32 holding four of the 128
 // columns. Bound by memory latency: with a serial walk over the splits, which paid a round
 // trip each, 12.9 us for 1024 rows x 8 splits and 7.0 us for 16 rows x 23; now 5.0 and 4.2.
+// CLAMP: lengths outside [0, Smax] count as the nearest of the two (the 8-bit cache's).
+template <bool CLAMP = false>
 __global__ __launch_bounds__(256) void combine_kernel(Params P) {
   const int64_t w = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 6;
   const int lane = threadIdx.x & 63;
@@ -669,7 +671,8 @@ __global__ __launch_bounds__(256) void combine_kernel(Params P) {
   for (int m = 1; m < 64; m <<= 1) L += __shfl_xor(L, m);
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] += wave_xor32(acc[e]);
-  const float inv = row_inv(keys_seen(P, cache_len(P, b), i), L);
+  const int len = cache_len(P, b);
+  const float inv = row_inv(keys_seen(P, CLAMP ? min(max(len, 0), P.Smax) : len, i), L);
   if (lane < 32)
     *reinterpret_cast<bf16x4*>(P.out + b * P.o_sb + i * P.o_ss + h * P.o_sh + 4 * lane) =
         cvt4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);

@@ -22,8 +22,11 @@
 #include "plan.h"
 #include "rope.h"
 #include "kvcache.h"
+#include "kvcache8.h"
 #include "norm_mlp.h"
 #include "gemm.h"
+#include "logprob.h"
+#include "embed.h"
 
 using namespace prefixlm;
 
@@ -1118,6 +1121,71 @@ static int64_t kv_nsplit(int64_t B, int S, int64_t H, int64_t Smax) {
   return one <= split ? 1 : n;
 }
 
+// The reference's prefill, an empty cache and a packed batch of new rows: the varlen forward over
+// them; with `append` the launch also writes them to the bf16 caches.
+static bool kv_prefills(const kvc::Params& P) {
+  const int64_t S = P.S;
+  const bool packed = P.B == 1 || (P.q_sb == S * P.q_ss && P.k_sb == S * P.k_ss && P.v_sb == S * P.v_ss &&
+                                   P.o_sb == S * P.o_ss);
+  return !P.seqlens && P.seqlen_const == 0 && P.s_new && packed && P.S <= P.Smax &&
+         (int64_t)P.B * P.S < 0x7fffffff && P.q_ss >= kvc::D && P.k_ss >= kvc::D && P.v_ss >= kvc::D && P.o_ss >= kvc::D;
+}
+static int kv_prefill(const kvc::Params& P, bool append, hipStream_t stream) {
+  const int B = P.B, S = P.S, H = P.H;
+  const int64_t T = (int64_t)B * S;
+  // one launch: the sequences are equal, so the forward needs no metadata and no work list, and
+  // workgroups past its items append the new rows (append, metadata, work list and forward as
+  // four launches took 46.8 us a call for 2 x 1021 rows x 16 heads, now 32.7)
+  const void* fp[] = {P.q, P.k, P.v, P.out};
+  const int64_t fs[] = {P.q_ss, P.q_sh, P.k_ss,   P.k_sh,
+                        P.v_ss, P.v_sh, P.o_ss, P.o_sh};
+  const int rc = check_common(fp, 4, fs, 4, (int32_t)T, H, kvc::D, (int32_t)T, 0, S, 0, nullptr, nullptr, nullptr);
+  if (rc) return rc;
+  fwd::Params F{};
+  F.q = P.q;
+  F.k = P.k;
+  F.v = P.v;
+  F.o = P.out;
+  F.q_st = P.q_ss; F.q_sh = P.q_sh;
+  F.k_st = P.k_ss; F.k_sh = P.k_sh;
+  F.v_st = P.v_ss; F.v_sh = P.v_sh;
+  F.o_st = P.o_ss; F.o_sh = P.o_sh;
+  F.T = F.total = (int)T;
+  F.H = H;
+  F.is_causal = P.causal;
+  F.numseqs = B;
+  F.scale_log2 = P.scale_log2;
+  F.seq_len = S;
+  F.kc = P.kc;
+  F.vc = P.vc;
+  F.kc_sb = P.kc_sb; F.kc_ss = P.kc_ss; F.kc_sh = P.kc_sh;
+  F.vc_sb = P.vc_sb; F.vc_ss = P.vc_ss; F.vc_sh = P.vc_sh;
+  const int64_t items = (int64_t)B * ((S + fwd::BM - 1) / fwd::BM), nblk = unit_grid(items, H);
+  bool split = false;
+  int cus = 0;
+  int rc2 = fwd_splits_keys(nblk, S, &split);
+  if (!rc2) rc2 = persistent_grid(&cus);
+  if (rc2) return rc2;
+  // More workgroups than the CUs hold at once (three each), all with the same keys to walk: one
+  // sequence after another, so that those running together share its keys and values in L2 (8 x
+  // 4100 rows x 16 heads 1327 us with the tiles of all sequences mixed, 1205 so; below that
+  // number 8 x 300 rows 18.5 and 19.1)
+  F.seq_major = !P.causal && nblk > 3 * (int64_t)cus;
+  const int nt = fwd::NT * (split ? 2 : 1), per = nt * fwd::kAppend;
+  const int64_t nappend = append ? (T * H * 16 + per - 1) / per : 0;
+  if (nblk + nappend > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "grid too large");
+  F.n_main = (int)nblk;
+  if (split)
+    hipLaunchKernelGGL((fwd::prefixlm_fwd_kernel<kvc::D, true, 2>), dim3((unsigned)(nblk + nappend)), dim3(nt),
+                       2 * fwd::Geo<kvc::D>::LDS_BYTES, stream, F);
+  else
+    hipLaunchKernelGGL((fwd::prefixlm_fwd_kernel<kvc::D, true>), dim3((unsigned)(nblk + nappend)), dim3(nt),
+                       fwd::Geo<kvc::D>::LDS_BYTES, stream, F);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "prefill launch: %s", hipGetErrorString(e));
+  return PREFIXLM_OK;
+}
+
 size_t prefixlm_kvcache_workspace_size(int32_t batch, int32_t seqlen_q, int32_t num_heads, int32_t head_dim,
                                        int32_t max_seqlen_cache) {
   (void)head_dim;
@@ -1180,15 +1248,7 @@ int prefixlm_kvcache_fwd(const prefixlm_kvcache_args* a, void* stream_) {
   P.scale_log2 = a->softmax_scale * kLog2e;
 
   (void)hipGetLastError();
-  // the reference's prefill: an empty cache and a packed batch of new rows
-  const bool packed = B == 1 || (a->q_stride_b == (int64_t)S * a->q_stride_s &&
-                                 a->k_stride_b == (int64_t)S * a->k_stride_s &&
-                                 a->v_stride_b == (int64_t)S * a->v_stride_s &&
-                                 a->out_stride_b == (int64_t)S * a->out_stride_s);
-  const int64_t T = (int64_t)B * S;
-  const bool prefill = !a->cache_seqlens && a->cache_seqlen == 0 && has_new && packed && S <= Smax &&
-                       T < 0x7fffffff && a->q_stride_s >= kvc::D && a->k_stride_s >= kvc::D &&
-                       a->v_stride_s >= kvc::D && a->out_stride_s >= kvc::D;
+  const bool prefill = kv_prefills(P);
   // The decode and extend kernels read the new rows from k, v and write them to the caches in
   // one launch; that needs cache rows of its own for every (b, row, head) and two caches (a
   // row shared between batch rows would be read by one while the other writes it).
@@ -1205,57 +1265,7 @@ int prefixlm_kvcache_fwd(const prefixlm_kvcache_args* a, void* stream_) {
   if (g_attr_err != hipSuccess)
     return fail(PREFIXLM_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(g_attr_err));
   if (prefill) {
-    // one launch: the sequences are equal, so the forward needs no metadata and no work list, and
-    // workgroups past its items append the new rows (append, metadata, work list and forward as
-    // four launches took 46.8 us a call for 2 x 1021 rows x 16 heads, now 32.7)
-    const void* fp[] = {a->q, a->k, a->v, a->out};
-    const int64_t fs[] = {a->q_stride_s, a->q_stride_h, a->k_stride_s,   a->k_stride_h,
-                          a->v_stride_s, a->v_stride_h, a->out_stride_s, a->out_stride_h};
-    const int rc = check_common(fp, 4, fs, 4, (int32_t)T, H, kvc::D, (int32_t)T, 0, S, 0, nullptr, nullptr, nullptr);
-    if (rc) return rc;
-    fwd::Params F{};
-    F.q = P.q;
-    F.k = P.k;
-    F.v = P.v;
-    F.o = P.out;
-    F.q_st = a->q_stride_s; F.q_sh = a->q_stride_h;
-    F.k_st = a->k_stride_s; F.k_sh = a->k_stride_h;
-    F.v_st = a->v_stride_s; F.v_sh = a->v_stride_h;
-    F.o_st = a->out_stride_s; F.o_sh = a->out_stride_h;
-    F.T = F.total = (int)T;
-    F.H = H;
-    F.is_causal = a->is_causal ? 1 : 0;
-    F.numseqs = B;
-    F.scale_log2 = P.scale_log2;
-    F.seq_len = S;
-    F.kc = P.kc;
-    F.vc = P.vc;
-    F.kc_sb = P.kc_sb; F.kc_ss = P.kc_ss; F.kc_sh = P.kc_sh;
-    F.vc_sb = P.vc_sb; F.vc_ss = P.vc_ss; F.vc_sh = P.vc_sh;
-    const int64_t items = (int64_t)B * ((S + fwd::BM - 1) / fwd::BM), nblk = unit_grid(items, H);
-    bool split = false;
-    int cus = 0;
-    int rc2 = fwd_splits_keys(nblk, S, &split);
-    if (!rc2) rc2 = persistent_grid(&cus);
-    if (rc2) return rc2;
-    // More workgroups than the CUs hold at once (three each), all with the same keys to walk: one
-    // sequence after another, so that those running together share its keys and values in L2 (8 x
-    // 4100 rows x 16 heads 1327 us with the tiles of all sequences mixed, 1205 so; below that
-    // number 8 x 300 rows 18.5 and 19.1)
-    F.seq_major = !a->is_causal && nblk > 3 * (int64_t)cus;
-    const int nt = fwd::NT * (split ? 2 : 1), per = nt * fwd::kAppend;
-    const int64_t nappend = (T * H * 16 + per - 1) / per;
-    if (nblk + nappend > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "grid too large");
-    F.n_main = (int)nblk;
-    if (split)
-      hipLaunchKernelGGL((fwd::prefixlm_fwd_kernel<kvc::D, true, 2>), dim3((unsigned)(nblk + nappend)), dim3(nt),
-                         2 * fwd::Geo<kvc::D>::LDS_BYTES, stream, F);
-    else
-      hipLaunchKernelGGL((fwd::prefixlm_fwd_kernel<kvc::D, true>), dim3((unsigned)(nblk + nappend)), dim3(nt),
-                         fwd::Geo<kvc::D>::LDS_BYTES, stream, F);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "prefill launch: %s", hipGetErrorString(e));
-    return PREFIXLM_OK;
+    return kv_prefill(P, true, stream);
   }
   {
     const int64_t units = (int64_t)B * H * P.nsplit, nblk = S == 1 ? units : (units + 7) / 8 * 8 * P.nqb;
@@ -1275,7 +1285,7 @@ int prefixlm_kvcache_fwd(const prefixlm_kvcache_args* a, void* stream_) {
       hipLaunchKernelGGL(kvc::extend_kernel<4>, dim3((unsigned)nblk), dim3(kvc::NT), kvc::ExtGeo<4>::LDS_BYTES, stream, P);
     if (P.nsplit > 1) {
       const int64_t waves = (int64_t)B * S * H;
-      hipLaunchKernelGGL(kvc::combine_kernel, dim3((unsigned)((waves * 64 + 255) / 256)), dim3(256), 0, stream, P);
+      hipLaunchKernelGGL(kvc::combine_kernel<>, dim3((unsigned)((waves * 64 + 255) / 256)), dim3(256), 0, stream, P);
     }
   }
   const hipError_t e = hipGetLastError();
@@ -1354,6 +1364,412 @@ int prefixlm_timer_read(void* timer, float* total_ms, int32_t* launches) {
   }
   t->recs.clear();
   return rc;
+}
+
+}  // extern "C"
+
+// ---- log probabilities ---------------------------------------------------------------
+// Splits of a row: 512 workgroups where the rows alone are fewer than the CUs, of at least two
+// vectors a thread each.
+static int lp_nsplit(int64_t rows, int64_t V, int32_t top) {
+  if (rows < 1 || rows >= 256) return 1;
+  const int64_t most = std::max<int64_t>(1, V / (16 * lp::NT)), want = (512 + rows - 1) / rows;
+  const int64_t fit = top > 0 ? lp::kCand / top : lp::kMaxSplits;
+  return (int)std::min({most, want, fit, (int64_t)lp::kMaxSplits});
+}
+
+static size_t lp_workspace(int64_t rows, int64_t vocab, int32_t top_k) {
+  if (rows < 1 || vocab < 1 || top_k < 0) return 0;
+  const int n = lp_nsplit(rows, vocab, top_k);
+  return n == 1 ? 0 : align_up((size_t)rows * n * 16) + align_up((size_t)rows * n * top_k * 8);
+}
+
+template <class T, bool ENT, bool TOP>
+static void lp_fwd_launch(const lp::Params& P, hipStream_t stream) {
+  hipLaunchKernelGGL((lp::forward_kernel<T, ENT, TOP>), dim3((unsigned)(P.rows * P.nsplit)), dim3(lp::NT), 0, stream, P);
+  if (P.nsplit > 1)
+    hipLaunchKernelGGL((lp::combine_kernel<T, ENT, TOP>), dim3((unsigned)P.rows), dim3(256), 0, stream, P);
+}
+template <class T>
+static void lp_fwd_launch(const lp::Params& P, hipStream_t stream) {
+  if (P.entropy)
+    P.top ? lp_fwd_launch<T, true, true>(P, stream) : lp_fwd_launch<T, true, false>(P, stream);
+  else
+    P.top ? lp_fwd_launch<T, false, true>(P, stream) : lp_fwd_launch<T, false, false>(P, stream);
+}
+
+static int lp_call(const prefixlm_logprob_args* a, void* stream_, bool backward) {
+  if (!a) return fail(PREFIXLM_ERR_INVALID, "args is null");
+  if (a->rows < 0 || a->vocab < 1 || a->vocab > 0x7fffffff)
+    return fail(PREFIXLM_ERR_INVALID, "rows=%lld vocab=%lld: vocab must be in [1, 2^31)", (long long)a->rows,
+                (long long)a->vocab);
+  if (!backward && (a->top_k < 0 || a->top_k > lp::kMaxTop || a->top_k > a->vocab))
+    return fail(PREFIXLM_ERR_INVALID, "top_k=%d must be in [0, min(%d, vocab)]", a->top_k, lp::kMaxTop);
+  if (a->rows == 0) return PREFIXLM_OK;   // empty tensors may have null pointers
+  const uintptr_t size = a->x_fp32 ? 4 : 2;
+  if (!a->x || (uintptr_t)a->x % size) return fail(PREFIXLM_ERR_INVALID, "x is null or not aligned to its element");
+  if (a->x_stride < 0) return fail(PREFIXLM_ERR_INVALID, "x_stride (%lld) must be >= 0", (long long)a->x_stride);
+  if (!a->stats) return fail(PREFIXLM_ERR_INVALID, "stats is null");
+  if (!a->targets && (a->logprob || (backward && a->dlogprob)))
+    return fail(PREFIXLM_ERR_INVALID, "targets is null");
+  lp::Params P{};
+  P.x = a->x;
+  P.targets = a->targets;
+  P.stats = a->stats;
+  P.entropy = a->entropy;
+  P.x_st = a->x_stride;
+  P.rows = a->rows;
+  P.V = a->vocab;
+  P.ignore = a->ignore_index;
+  P.wide_targets = !a->targets_int32;
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  if (backward) {
+    if (!a->dx || (uintptr_t)a->dx % size) return fail(PREFIXLM_ERR_INVALID, "dx is null or not aligned to its element");
+    if (a->dx_stride < a->vocab)
+      return fail(PREFIXLM_ERR_INVALID, "dx_stride (%lld) must be >= vocab", (long long)a->dx_stride);
+    if (a->dentropy && !a->entropy) return fail(PREFIXLM_ERR_INVALID, "dentropy needs the forward's entropy");
+    P.dx = a->dx;
+    P.dx_st = a->dx_stride;
+    P.g = a->dlogprob;
+    P.h = a->dentropy;
+    const int64_t nblk = (a->vocab + 8 * 256 * lp::kUnroll - 1) / (8 * 256 * lp::kUnroll);
+    if (a->rows * nblk > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many elements");
+    (void)hipGetLastError();
+    auto* k = a->x_fp32 ? (P.h ? lp::backward_kernel<float, true> : lp::backward_kernel<float, false>)
+                        : (P.h ? lp::backward_kernel<bf16, true> : lp::backward_kernel<bf16, false>);
+    hipLaunchKernelGGL(k, dim3((unsigned)(a->rows * nblk)), dim3(256), 0, stream, P, (int)nblk);
+  } else {
+    if (a->targets && !a->logprob) return fail(PREFIXLM_ERR_INVALID, "logprob is null");
+    if (a->top_k && (!a->top_logprobs || !a->top_ids))
+      return fail(PREFIXLM_ERR_INVALID, "top_logprobs or top_ids is null");
+    P.logprob = a->logprob;
+    P.top = a->top_k;
+    P.top_val = a->top_logprobs;
+    P.top_id = a->top_ids;
+    P.nsplit = lp_nsplit(a->rows, a->vocab, a->top_k);
+    if (P.nsplit > 1) {
+      const size_t need = lp_workspace(a->rows, a->vocab, a->top_k);
+      if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need)
+        return fail(PREFIXLM_ERR_INVALID, "workspace of %zu bytes is null, unaligned or below %zu", a->workspace_bytes, need);
+      P.part = static_cast<float*>(a->workspace);
+      P.part_top = reinterpret_cast<unsigned long long*>(static_cast<char*>(a->workspace) +
+                                                         align_up((size_t)a->rows * P.nsplit * 16));
+    }
+    if (a->rows * P.nsplit > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many rows");
+    (void)hipGetLastError();
+    if (a->x_fp32)
+      lp_fwd_launch<float>(P, stream);
+    else
+      lp_fwd_launch<bf16>(P, stream);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "log probabilities launch: %s", hipGetErrorString(e));
+  return PREFIXLM_OK;
+}
+
+extern "C" {
+
+size_t prefixlm_logprob_workspace_size(int64_t rows, int64_t vocab, int32_t top_k) {
+  return lp_workspace(rows, vocab, top_k);
+}
+int prefixlm_logprob_fwd(const prefixlm_logprob_args* a, void* stream) { return lp_call(a, stream, false); }
+int prefixlm_logprob_bwd(const prefixlm_logprob_args* a, void* stream) { return lp_call(a, stream, true); }
+
+}  // extern "C"
+
+// ---- embedding -----------------------------------------------------------------------
+// The sort's tiles: 2048 tokens, or more where that would be over kMaxTiles of them
+static int emb_tile(int64_t T) {
+  const int64_t per = (T + emb::kMaxTiles - 1) / emb::kMaxTiles;
+  return (int)std::max<int64_t>(2048, (per + emb::kSortThreads - 1) / emb::kSortThreads * emb::kSortThreads);
+}
+struct EmbWorkspace {
+  size_t key[2], pos[2], hist, part, total;
+};
+static EmbWorkspace emb_workspace(int64_t T, int32_t cols) {
+  EmbWorkspace w{};
+  size_t at = 0;
+  auto take = [&at](size_t n) {
+    const size_t here = at;
+    at += align_up(n);
+    return here;
+  };
+  const int tile = emb_tile(T);
+  for (int i = 0; i < 2; ++i) {
+    w.key[i] = take((size_t)T * 4);
+    w.pos[i] = take((size_t)T * 4);
+  }
+  w.hist = take((size_t)((T + tile - 1) / tile) * emb::kBins * 4);
+  w.part = take((size_t)((T + emb::kRun - 1) / emb::kRun) * 2 * (size_t)cols * 4);
+  w.total = at;
+  return w;
+}
+
+extern "C" {
+
+size_t prefixlm_embedding_workspace_size(int64_t tokens, int64_t vocab, int32_t cols) {
+  (void)vocab;
+  return tokens < 1 || cols < 1 ? 0 : emb_workspace(tokens, cols).total;
+}
+
+static int emb_check(const prefixlm_embedding_args* a) {
+  if (!a) return fail(PREFIXLM_ERR_INVALID, "args is null");
+  if (a->tokens < 0 || a->tokens > 0x7fffffff || a->vocab < 1 || a->vocab >= (1 << 27))
+    return fail(PREFIXLM_ERR_INVALID, "tokens=%lld vocab=%lld: tokens must be below 2^31, vocab in [1, 2^27)",
+                (long long)a->tokens, (long long)a->vocab);
+  if (a->cols < 8 || a->cols % 8) return fail(PREFIXLM_ERR_INVALID, "cols=%d must be a positive multiple of 8", a->cols);
+  return PREFIXLM_OK;
+}
+static int emb_rows(const void* p, int64_t stride, int32_t fp32, int32_t cols, bool repeats, const char* name) {
+  if (!p || !aligned16(p)) return fail(PREFIXLM_ERR_INVALID, "%s is null or not 16-byte aligned", name);
+  if ((stride < cols && !(repeats && stride == 0)) || stride % (fp32 ? 4 : 8))
+    return fail(PREFIXLM_ERR_INVALID, "row stride of %s (%lld) must be 16-byte rows and >= cols", name, (long long)stride);
+  return PREFIXLM_OK;
+}
+
+int prefixlm_embedding_fwd(const prefixlm_embedding_args* a, void* stream_) {
+  int rc = emb_check(a);
+  if (rc) return rc;
+  if (a->tokens == 0) return PREFIXLM_OK;
+  if (!a->ids) return fail(PREFIXLM_ERR_INVALID, "ids is null");
+  rc = emb_rows(a->table, a->table_stride, a->table_fp32, a->cols, true, "table");
+  if (!rc) rc = emb_rows(a->y, a->y_stride, a->y_fp32, a->cols, false, "y");
+  if (rc) return rc;
+  const int64_t nblk = (a->tokens * (a->cols / 8) + 255) / 256;
+  if (nblk > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many elements");
+  const emb::FwdParams P{a->table, a->ids, a->y, a->table_stride, a->y_stride, a->tokens, a->vocab, a->cols,
+                         !a->ids_int32, a->scale};
+  (void)hipGetLastError();
+  auto* k = a->table_fp32 ? (a->y_fp32 ? emb::lookup_kernel<float, float> : emb::lookup_kernel<float, bf16>)
+                          : (a->y_fp32 ? emb::lookup_kernel<bf16, float> : emb::lookup_kernel<bf16, bf16>);
+  hipLaunchKernelGGL(k, dim3((unsigned)nblk), dim3(256), 0, reinterpret_cast<hipStream_t>(stream_), P);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "embedding launch: %s", hipGetErrorString(e));
+  return PREFIXLM_OK;
+}
+
+int prefixlm_embedding_bwd(const prefixlm_embedding_args* a, void* stream_) {
+  int rc = emb_check(a);
+  if (rc) return rc;
+  rc = emb_rows(a->grad, a->cols, a->table_fp32, a->cols, false, "grad");
+  if (!rc && a->tokens) rc = emb_rows(a->dy, a->dy_stride, a->y_fp32, a->cols, true, "dy");
+  if (rc) return rc;
+  if (a->tokens && !a->ids) return fail(PREFIXLM_ERR_INVALID, "ids is null");
+  const size_t need = prefixlm_embedding_workspace_size(a->tokens, a->vocab, a->cols);
+  if (a->tokens && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
+    return fail(PREFIXLM_ERR_INVALID, "workspace of %zu bytes is null, unaligned or below %zu", a->workspace_bytes, need);
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  const int64_t T = a->tokens, units = a->vocab * a->cols * (a->table_fp32 ? 4 : 2) / 16;
+  int bits = 1, passes = 1;
+  while ((a->vocab >> bits) != 0) ++bits;   // keys up to vocab
+  passes = T ? (bits + emb::kBits - 1) / emb::kBits : 0;
+  const int64_t waves = (T + emb::kRun - 1) / emb::kRun * ((a->cols + 511) / 512);
+  if (waves > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many elements");
+  const EmbWorkspace w = emb_workspace(T, a->cols);
+  char* ws = static_cast<char*>(a->workspace);
+  emb::SortParams P{};
+  P.zero = a->grad;
+  P.T = T;
+  P.V = a->vocab;
+  P.padding = a->padding_id;
+  P.wide_ids = !a->ids_int32;
+  P.tile = emb_tile(T);
+  P.tiles = (int)((T + P.tile - 1) / P.tile);
+  (void)hipGetLastError();
+  const int launches = std::max(1, 2 * passes);
+  int done = 0;
+  auto share = [&] {   // of the clearing, for the next launch; and its workgroups
+    P.zero_begin = units * done / launches;
+    P.zero_end = units * ++done / launches;
+    return (unsigned)(P.tiles + std::min<int64_t>(2048, (P.zero_end - P.zero_begin + 255) / 256));
+  };
+  if (T == 0) {
+    const unsigned n = share();
+    hipLaunchKernelGGL(emb::histogram_kernel, dim3(n), dim3(emb::kSortThreads), 0, stream, P);
+  }
+  for (int p = 0; p < passes; ++p) {
+    P.ids = p == 0 ? a->ids : nullptr;
+    P.key_in = reinterpret_cast<const uint32_t*>(ws + w.key[(p + 1) & 1]);
+    P.pos_in = reinterpret_cast<const uint32_t*>(ws + w.pos[(p + 1) & 1]);
+    P.key_out = reinterpret_cast<uint32_t*>(ws + w.key[p & 1]);
+    P.pos_out = reinterpret_cast<uint32_t*>(ws + w.pos[p & 1]);
+    P.hist = reinterpret_cast<uint32_t*>(ws + w.hist);
+    P.shift = p * emb::kBits;
+    unsigned n = share();
+    hipLaunchKernelGGL(emb::histogram_kernel, dim3(n), dim3(emb::kSortThreads), 0, stream, P);
+    n = share();
+    hipLaunchKernelGGL(emb::scatter_kernel, dim3(n), dim3(emb::kSortThreads), 0, stream, P);
+  }
+  if (T > 0) {
+    emb::SumParams S{};
+    S.key = P.key_out;
+    S.pos = P.pos_out;
+    S.dy = a->dy;
+    S.grad = a->grad;
+    S.part = reinterpret_cast<float*>(ws + w.part);
+    S.dy_st = a->dy_stride;
+    S.T = T;
+    S.V = a->vocab;
+    S.cols = a->cols;
+    S.chunks = (int)((T + emb::kRun - 1) / emb::kRun);
+    S.scale = a->scale;
+    auto* k = a->table_fp32 ? (a->y_fp32 ? emb::sum_kernel<float, float> : emb::sum_kernel<bf16, float>)
+                            : (a->y_fp32 ? emb::sum_kernel<float, bf16> : emb::sum_kernel<bf16, bf16>);
+    hipLaunchKernelGGL(k, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream, S);
+    if (S.chunks > 1)
+      hipLaunchKernelGGL(a->table_fp32 ? emb::join_kernel<float> : emb::join_kernel<bf16>,
+                         dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, stream, S);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "embedding gradient launch: %s", hipGetErrorString(e));
+  return PREFIXLM_OK;
+}
+
+}  // extern "C"
+
+// ---- attention over an 8-bit cache -----------------------------------------------------------
+// Splits of the keys; those of several queries as for bf16 (the tiles and their chain are the same).
+static int64_t kv8_nsplit(int64_t B, int S, int64_t H, int64_t Smax) {
+  if (S > 1) return kv_nsplit(B, S, H, Smax);
+  const int64_t units = B * H, most = std::min<int64_t>(kvc::kMaxSplits, (Smax + 127) / 128);
+  return std::max<int64_t>(1, std::min((1024 + units - 1) / units, most));
+}
+
+template <class C>
+static void kv8_launch(const kv8::Params& P, int64_t nblk, hipStream_t stream) {
+  const dim3 g((unsigned)nblk), n(kvc::NT);
+  if (P.S == 1)
+    hipLaunchKernelGGL((kv8::decode_kernel<C, kvc::NT>), g, n, 0, stream, P);
+  else if (ext_qw(P.S) == 1)
+    hipLaunchKernelGGL((kv8::extend_kernel<C, 1>), g, n, kvc::ExtGeo<1>::LDS_BYTES, stream, P);
+  else if (ext_qw(P.S) == 2)
+    hipLaunchKernelGGL((kv8::extend_kernel<C, 2>), g, n, kvc::ExtGeo<2>::LDS_BYTES, stream, P);
+  else
+    hipLaunchKernelGGL((kv8::extend_kernel<C, 4>), g, n, kvc::ExtGeo<4>::LDS_BYTES, stream, P);
+}
+
+// Dynamic LDS above the default limit has to be allowed once per kernel and device
+static int kv8_allow_lds() {
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = -1;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "hipGetDevice: %s", hipGetErrorString(e));
+  if (dev < 0 || dev >= 64) return fail(PREFIXLM_ERR_INVALID, "device %d >= 64", dev);
+  std::lock_guard<std::mutex> g(mu);
+  if (done[dev]) return PREFIXLM_OK;
+  const std::pair<const void*, int> kernels[] = {
+      {(const void*)kv8::extend_kernel<kv8::E4M3, 1>, kvc::ExtGeo<1>::LDS_BYTES},
+      {(const void*)kv8::extend_kernel<kv8::E4M3, 2>, kvc::ExtGeo<2>::LDS_BYTES},
+      {(const void*)kv8::extend_kernel<kv8::E4M3, 4>, kvc::ExtGeo<4>::LDS_BYTES},
+      {(const void*)kv8::extend_kernel<kv8::Int8, 1>, kvc::ExtGeo<1>::LDS_BYTES},
+      {(const void*)kv8::extend_kernel<kv8::Int8, 2>, kvc::ExtGeo<2>::LDS_BYTES},
+      {(const void*)kv8::extend_kernel<kv8::Int8, 4>, kvc::ExtGeo<4>::LDS_BYTES}};
+  for (const auto& k : kernels) {
+    e = hipFuncSetAttribute(k.first, hipFuncAttributeMaxDynamicSharedMemorySize, k.second);
+    if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  }
+  done[dev] = true;
+  return PREFIXLM_OK;
+}
+
+extern "C" {
+
+size_t prefixlm_kvcache8_workspace_size(int32_t batch, int32_t seqlen_q, int32_t num_heads, int32_t max_seqlen_cache) {
+  if (batch < 1 || seqlen_q < 1 || num_heads < 1 || max_seqlen_cache < 1) return 0;
+  const int64_t nsplit = kv8_nsplit(batch, seqlen_q, num_heads, max_seqlen_cache);
+  return nsplit == 1 ? 0 : align_up(sizeof(float) * (size_t)batch * seqlen_q * num_heads * nsplit * kvc::kPart);
+}
+
+int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* a, void* stream_) {
+  if (!a) return fail(PREFIXLM_ERR_INVALID, "args is null");
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  const int B = a->batch, S = a->seqlen_q, H = a->num_heads, Smax = a->max_seqlen_cache;
+  if (a->head_dim != kvc::D) return fail(PREFIXLM_ERR_INVALID, "head_dim must be 128 (got %d)", a->head_dim);
+  if (B < 1 || S < 1 || H < 1 || Smax < 1 || Smax % kv8::kBlock)
+    return fail(PREFIXLM_ERR_INVALID,
+                "batch=%d seqlen_q=%d num_heads=%d must be >= 1 and max_seqlen_cache=%d a positive multiple of %d", B, S, H,
+                Smax, kv8::kBlock);
+  if (S > 0x7fffffff - Smax) return fail(PREFIXLM_ERR_INVALID, "seqlen_q=%d is too large", S);
+  const bool has_new = a->k != nullptr;
+  if ((a->k == nullptr) != (a->v == nullptr)) return fail(PREFIXLM_ERR_INVALID, "k and v must be given together");
+  if (!a->cache_seqlens && (a->cache_seqlen < 0 || a->cache_seqlen > Smax))
+    return fail(PREFIXLM_ERR_INVALID, "cache_seqlen=%d outside [0, %d]", a->cache_seqlen, Smax);
+  const void* ptrs[] = {a->q, a->k_codes, a->v_codes, a->k_scale, a->v_scale, a->k_recent, a->v_recent, a->out, a->k, a->v};
+  for (int i = 0; i < (has_new ? 10 : 8); ++i)
+    if (!ptrs[i] || (i == 3 || i == 4 ? (uintptr_t)ptrs[i] % 4 != 0 : !aligned16(ptrs[i])))
+      return fail(PREFIXLM_ERR_INVALID, "tensor pointer %d is null or not aligned (16 bytes, scales 4)", i);
+  const int64_t st[] = {a->q_stride_b, a->q_stride_s, a->q_stride_h, a->out_stride_b, a->out_stride_s, a->out_stride_h,
+                        a->k_stride_b, a->k_stride_s, a->k_stride_h, a->v_stride_b,   a->v_stride_s,   a->v_stride_h};
+  for (int i = 0; i < (has_new ? 12 : 6); ++i)
+    if (st[i] < 0 || st[i] % 8)
+      return fail(PREFIXLM_ERR_INVALID, "stride %d (%lld) must be a non-negative multiple of 8", i, (long long)st[i]);
+  const size_t need = prefixlm_kvcache8_workspace_size(B, S, H, Smax);
+  if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
+    return fail(PREFIXLM_ERR_INVALID, "workspace of %zu bytes is null, unaligned or below %zu", a->workspace_bytes, need);
+
+  kv8::Params P{};
+  P.q = static_cast<const bf16*>(a->q);
+  P.k = static_cast<const bf16*>(a->k);
+  P.v = static_cast<const bf16*>(a->v);
+  P.kc = static_cast<uint8_t*>(a->k_codes);
+  P.vc = static_cast<uint8_t*>(a->v_codes);
+  P.ks = a->k_scale;
+  P.vs = a->v_scale;
+  P.kr = static_cast<bf16*>(a->k_recent);
+  P.vr = static_cast<bf16*>(a->v_recent);
+  P.out = static_cast<bf16*>(a->out);
+  P.part = static_cast<float*>(a->workspace);
+  P.seqlens = a->cache_seqlens;
+  P.q_sb = a->q_stride_b; P.q_ss = a->q_stride_s; P.q_sh = a->q_stride_h;
+  P.k_sb = a->k_stride_b; P.k_ss = a->k_stride_s; P.k_sh = a->k_stride_h;
+  P.v_sb = a->v_stride_b; P.v_ss = a->v_stride_s; P.v_sh = a->v_stride_h;
+  P.o_sb = a->out_stride_b; P.o_ss = a->out_stride_s; P.o_sh = a->out_stride_h;
+  P.B = B; P.S = S; P.H = H; P.Smax = Smax;
+  P.nsplit = (int)kv8_nsplit(B, S, H, Smax);
+  P.nqb = kv_nqb(S);
+  P.causal = a->is_causal ? 1 : 0;
+  P.seqlen_const = a->cache_seqlen;
+  P.s_new = has_new ? S : 0;
+  P.scale_log2 = a->softmax_scale * kLog2e;
+  // the same queries, rows, lengths and partials, for the kernels shared with the bf16 cache
+  kvc::Params Q{};
+  Q.q = P.q; Q.k = P.k; Q.v = P.v; Q.out = P.out; Q.part = P.part; Q.seqlens = P.seqlens;
+  Q.q_sb = P.q_sb; Q.q_ss = P.q_ss; Q.q_sh = P.q_sh;
+  Q.k_sb = P.k_sb; Q.k_ss = P.k_ss; Q.k_sh = P.k_sh;
+  Q.v_sb = P.v_sb; Q.v_ss = P.v_ss; Q.v_sh = P.v_sh;
+  Q.o_sb = P.o_sb; Q.o_ss = P.o_ss; Q.o_sh = P.o_sh;
+  Q.B = B; Q.S = S; Q.H = H; Q.Smax = Smax; Q.nsplit = P.nsplit;
+  Q.causal = P.causal; Q.seqlen_const = P.seqlen_const; Q.s_new = P.s_new; Q.scale_log2 = P.scale_log2;
+
+  const int64_t units = (int64_t)B * H * P.nsplit, nblk = S == 1 ? units : (units + 7) / 8 * 8 * P.nqb;
+  const int64_t touched = std::max<int64_t>(1, ((int64_t)S + kv8::kBlock - 1) / kv8::kBlock);
+  const int64_t waves = (int64_t)B * S * H;
+  if (nblk > 0x7fffffff || (int64_t)B * H * touched > 0x7fffffff || (waves * 64 + 255) / 256 > 0x7fffffff)
+    return fail(PREFIXLM_ERR_INVALID, "grid too large");
+  (void)hipGetLastError();
+  if (kv_prefills(Q)) {
+    set_kernel_attrs();
+    if (g_attr_err != hipSuccess)
+      return fail(PREFIXLM_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(g_attr_err));
+    const int rc = kv_prefill(Q, false, stream);
+    if (rc) return rc;
+  } else {
+    const int rc = kv8_allow_lds();
+    if (rc) return rc;
+    if (a->code_int8)
+      kv8_launch<kv8::Int8>(P, nblk, stream);
+    else
+      kv8_launch<kv8::E4M3>(P, nblk, stream);
+    if (P.nsplit > 1)
+      hipLaunchKernelGGL(kvc::combine_kernel<true>, dim3((unsigned)((waves * 64 + 255) / 256)), dim3(256), 0, stream, Q);
+  }
+  if (has_new && (S > 1 || kv_prefills(Q)))
+    hipLaunchKernelGGL(a->code_int8 ? kv8::append_kernel<kv8::Int8> : kv8::append_kernel<kv8::E4M3>,
+                       dim3((unsigned)(B * H * touched)), dim3(kvc::NT), 0, stream, P, (int)touched);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "8-bit kv-cache launch: %s", hipGetErrorString(e));
+  return PREFIXLM_OK;
 }
 
 }  // extern "C"

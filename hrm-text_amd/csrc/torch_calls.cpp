@@ -63,6 +63,14 @@ struct Lib {
   decltype(&prefixlm_proj_gemm_scaled) proj_gemm_scaled;
   decltype(&prefixlm_kvcache_workspace_size) kv_ws;
   decltype(&prefixlm_kvcache_fwd) kv_fwd;
+  decltype(&prefixlm_kvcache8_workspace_size) kv8_ws;
+  decltype(&prefixlm_kvcache8_fwd) kv8_fwd;
+  decltype(&prefixlm_logprob_workspace_size) lp_ws;
+  decltype(&prefixlm_logprob_fwd) lp_fwd;
+  decltype(&prefixlm_logprob_bwd) lp_bwd;
+  decltype(&prefixlm_embedding_workspace_size) emb_ws;
+  decltype(&prefixlm_embedding_fwd) emb_fwd;
+  decltype(&prefixlm_embedding_bwd) emb_bwd;
   decltype(&prefixlm_last_error) last_error;
 } lib{};
 std::vector<int64_t> g_ds_cap;            // per device: an eighth of its memory
@@ -659,6 +667,210 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   }
 };
 
+// ---- log probabilities ------------------------------------------------------------------------
+// logits as [rows, V] with unit stride over V, or undefined
+Tensor logit_rows(const Tensor& x) {
+  if ((x.scalar_type() != at::kBFloat16 && x.scalar_type() != at::kFloat) || x.dim() < 1 || x.numel() == 0) return Tensor();
+  const Tensor r = x.dim() == 2 ? x : x.is_contiguous() ? x.view({-1, x.size(-1)}) : Tensor();
+  return r.defined() && (r.stride(1) == 1 || r.size(1) == 1) ? r : Tensor();
+}
+bool whole_rows(const Tensor& t, at::IntArrayRef sizes, const Tensor& like) {   // ids or targets
+  return (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt) && t.sizes() == sizes && t.is_contiguous() &&
+         t.device() == like.device();
+}
+struct LogprobCall {
+  Tensor targets;
+  bool entropy = false;
+  int64_t top = 0, ignore = 0;
+};
+struct LogprobOut {
+  Tensor lp, ent, stats, top, ids;
+};
+LogprobOut logprob_forward(const Tensor& x, const Tensor& x2, const LogprobCall& c) {
+  const Recorded call("prefixlm::token_logprobs_fwd", {x});
+  const int64_t rows = x2.size(0), V = x2.size(1);
+  const auto shape = x.sizes().slice(0, x.dim() - 1);
+  LogprobOut r;
+  prefixlm_logprob_args a{};
+  auto two = shape.vec();
+  two.push_back(2);
+  r.stats = empty_like_on(x, two, at::kFloat);
+  a.stats = r.stats.data_ptr<float>();
+  if (c.targets.defined()) {
+    r.lp = empty_like_on(x, shape, at::kFloat);
+    a.logprob = r.lp.data_ptr<float>();
+    a.targets = c.targets.const_data_ptr();
+    a.targets_int32 = c.targets.scalar_type() == at::kInt;
+  }
+  if (c.entropy) {
+    r.ent = empty_like_on(x, shape, at::kFloat);
+    a.entropy = r.ent.data_ptr<float>();
+  }
+  if (c.top) {
+    auto wide = shape.vec();
+    wide.push_back(c.top);
+    r.top = empty_like_on(x, wide, at::kFloat);
+    r.ids = empty_like_on(x, wide, at::kLong);
+    a.top_logprobs = r.top.data_ptr<float>();
+    a.top_ids = r.ids.data_ptr<int64_t>();
+  }
+  a.workspace_bytes = lib.lp_ws(rows, V, (int32_t)c.top);
+  Tensor ws;
+  if (a.workspace_bytes) {
+    ws = empty_like_on(x, {(int64_t)a.workspace_bytes}, at::kByte);
+    a.workspace = ws.data_ptr();
+  }
+  a.x = x2.const_data_ptr();
+  a.x_stride = x2.stride(0);
+  a.rows = rows;
+  a.vocab = V;
+  a.ignore_index = c.ignore;
+  a.top_k = (int32_t)c.top;
+  a.x_fp32 = x.scalar_type() == at::kFloat;
+  check(lib.lp_fwd(&a, stream_of(x)), "prefixlm_logprob_fwd");
+  return r;
+}
+// Outputs: those of lp, ent, top, ids that were asked for
+struct Logprobs : torch::autograd::Function<Logprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& x2, const LogprobCall& c) {
+    const LogprobOut r = logprob_forward(x, x2, c);
+    ctx->save_for_backward({x, c.targets, r.stats, r.ent});
+    ctx->saved_data["ignore"] = c.ignore;
+    ctx->saved_data["entropy"] = c.entropy;
+    ctx->set_materialize_grads(false);
+    variable_list out;
+    for (const Tensor& t : {r.lp, r.ent, r.top, r.ids})
+      if (t.defined()) out.push_back(t);
+    if (c.top) ctx->mark_non_differentiable({r.top, r.ids});
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &targets = s[1], &stats = s[2], &ent = s[3];
+    const int64_t ignore = ctx->saved_data["ignore"].toInt();
+    size_t at = 0;
+    Tensor g, h;
+    if (targets.defined()) g = grads[at++];
+    if (ctx->saved_data["entropy"].toBool()) h = grads[at++];
+    if (!g.defined() && !h.defined()) return {Tensor(), Tensor(), Tensor()};
+    bool direct = !at::GradMode::is_enabled() && plain_state();
+    for (const Tensor& t : {x, targets, stats, ent, g, h})
+      if (t.defined() && !plain_tensor(t)) direct = false;
+    Tensor x2;
+    if (direct) {
+      const auto shape = x.dim() ? x.sizes().slice(0, x.dim() - 1) : x.sizes();
+      auto two = shape.vec();
+      two.push_back(2);
+      x2 = logit_rows(x);
+      direct = x2.defined() && is_array(stats, at::kFloat, two, x) && stats.is_contiguous() &&
+               (!targets.defined() || whole_rows(targets, shape, x)) &&
+               (!g.defined() || is_array(g, at::kFloat, shape, x)) &&
+               (!h.defined() || (is_array(h, at::kFloat, shape, x) && is_array(ent, at::kFloat, shape, x) &&
+                                 ent.is_contiguous()));
+    }
+    if (direct) {
+      const Recorded call("prefixlm::token_logprobs_bwd", {x});
+      const c10::DeviceGuard guard(x.device());
+      const Tensor dx = empty_like_on(x, x.sizes(), x.scalar_type());
+      const Tensor gc = g.defined() ? g.contiguous() : g, hc = h.defined() ? h.contiguous() : h;
+      prefixlm_logprob_args a{};
+      a.x = x2.const_data_ptr();
+      a.stats = stats.data_ptr<float>();
+      if (targets.defined()) {
+        a.targets = targets.const_data_ptr();
+        a.targets_int32 = targets.scalar_type() == at::kInt;
+      }
+      if (gc.defined()) a.dlogprob = gc.const_data_ptr<float>();
+      if (hc.defined()) {
+        a.dentropy = hc.const_data_ptr<float>();
+        a.entropy = ent.data_ptr<float>();
+      }
+      a.dx = dx.data_ptr();
+      a.x_stride = x2.stride(0);
+      a.dx_stride = a.vocab = x2.size(1);
+      a.rows = x2.size(0);
+      a.ignore_index = ignore;
+      a.x_fp32 = x.scalar_type() == at::kFloat;
+      check(lib.lp_bwd(&a, stream_of(x)), "prefixlm_logprob_bwd");
+      return {dx, Tensor(), Tensor()};
+    }
+    const auto maybe = [](const Tensor& t) { return t.defined() ? c10::IValue(t) : c10::IValue(); };
+    torch::jit::Stack st{x, maybe(targets), stats, ent.defined() ? ent : at::empty({0}, stats.options()), maybe(g), maybe(h), ignore};
+    return {call_op("prefixlm::token_logprobs_bwd", std::move(st))[0], Tensor(), Tensor()};
+  }
+};
+
+// ---- the embedding ------------------------------------------------------------------------------
+bool float_rows(const Tensor& x, int64_t cols) {   // bf16 or fp32 [., cols] with 16-byte rows
+  return (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat) && x.dim() == 2 && x.size(1) == cols &&
+         x.stride(1) == 1 && x.stride(0) >= cols && x.stride(0) * x.element_size() % 16 == 0 && aligned(x, 16);
+}
+Tensor embedding_forward(const Tensor& ids, const Tensor& table, double scale, at::ScalarType dt) {
+  const Recorded call("prefixlm::embedding_fwd", {ids, table});
+  auto sizes = ids.sizes().vec();
+  sizes.push_back(table.size(1));
+  const Tensor y = empty_like_on(table, sizes, dt);
+  prefixlm_embedding_args a{};
+  a.ids = ids.const_data_ptr();
+  a.table = table.const_data_ptr();
+  a.y = y.data_ptr();
+  a.table_stride = table.stride(0);
+  a.y_stride = a.cols = (int32_t)table.size(1);
+  a.tokens = ids.numel();
+  a.vocab = table.size(0);
+  a.padding_id = -1;
+  a.table_fp32 = table.scalar_type() == at::kFloat;
+  a.y_fp32 = dt == at::kFloat;
+  a.ids_int32 = ids.scalar_type() == at::kInt;
+  a.scale = (float)scale;
+  check(lib.emb_fwd(&a, stream_of(table)), "prefixlm_embedding_fwd");
+  return y;
+}
+struct Embedding : torch::autograd::Function<Embedding> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& table, double scale, at::ScalarType dt,
+                        int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["args"] = std::vector<int64_t>{table.size(0), (int64_t)table.scalar_type(), padding};
+    ctx->saved_data["scale"] = scale;
+    return embedding_forward(ids, table, scale, dt);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const auto v = ctx->saved_data["args"].toIntVector();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const Tensor &ids = s[0], &dy = grads[0];
+    const auto dt = (at::ScalarType)v[1];
+    const int64_t D = dy.size(-1);
+    Tensor grad;
+    if (!at::GradMode::is_enabled() && plain_state() && plain_tensor(ids) && plain_tensor(dy) && dy.numel() > 0 &&
+        dy.is_contiguous() && whole_rows(ids, dy.sizes().slice(0, dy.dim() - 1), dy) && float_rows(dy.view({-1, D}), D)) {
+      const Recorded call("prefixlm::embedding_bwd", {ids, dy});
+      const c10::DeviceGuard guard(dy.device());
+      grad = empty_like_on(dy, {v[0], D}, dt);
+      prefixlm_embedding_args a{};
+      a.workspace_bytes = lib.emb_ws(ids.numel(), v[0], (int32_t)D);
+      const Tensor ws = empty_like_on(dy, {(int64_t)a.workspace_bytes}, at::kByte);
+      a.workspace = ws.data_ptr();
+      a.ids = ids.const_data_ptr();
+      a.dy = dy.const_data_ptr();
+      a.grad = grad.data_ptr();
+      a.dy_stride = D;
+      a.tokens = ids.numel();
+      a.vocab = v[0];
+      a.padding_id = v[2];
+      a.cols = (int32_t)D;
+      a.table_fp32 = dt == at::kFloat;
+      a.y_fp32 = dy.scalar_type() == at::kFloat;
+      a.ids_int32 = ids.scalar_type() == at::kInt;
+      a.scale = (float)scale;
+      check(lib.emb_bwd(&a, stream_of(dy)), "prefixlm_embedding_bwd");
+    } else {
+      grad = call_op("prefixlm::embedding_bwd", {ids, dy, v[0], scale, (int64_t)dt, v[2]})[0];
+    }
+    return {Tensor(), grad, Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ---- Python entry points ------------------------------------------------------------------------
 // Each returns None for a call that is not plain. The interpreter lock is released around the
 // call itself.
@@ -778,6 +990,173 @@ PyObject* py_kvcache(PyObject*, PyObject* const* a, Py_ssize_t n) {
     vc.unsafeGetTensorImpl()->bump_version();
   }
   return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// q, the cache's six tensors, k, v, cache_seqlens (int or tensor), softmax_scale (float or None), causal
+PyObject* py_kvcache_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, c[6], k, v, lens;
+  bool causal;
+  double scale;
+  int64_t len = 0;
+  if (!ready(n, 12) || c10::InferenceMode::is_enabled() || !get_tensor(a[0], &q)) return none();
+  for (int i = 0; i < 6; ++i)
+    if (!get_tensor(a[1 + i], &c[i]) || wants_grad(c[i])) return none();
+  const bool has_new = a[7] != Py_None;
+  if (has_new != (a[8] != Py_None) || (has_new && (!get_tensor(a[7], &k) || !get_tensor(a[8], &v)))) return none();
+  for (const Tensor* t : {&q, &k, &v})
+    if (t->defined() && (!cache_layout(*t) || t->device() != q.device() || t->numel() == 0 || wants_grad(*t))) return none();
+  const int64_t B = q.size(0), S = q.size(1), H = q.size(2), D = q.size(3);
+  if (D != 128 || c[0].dim() != 4 || (has_new && (k.sizes() != q.sizes() || v.sizes() != q.sizes()))) return none();
+  const int64_t Smax = c[0].size(2);
+  const auto code = c[0].scalar_type();
+  if (Smax < 1 || Smax % 64 || Smax > INT32_MAX || (code != at::kChar && code != at::kFloat8_e4m3fn)) return none();
+  for (int i = 0; i < 6; ++i) {
+    const bool fits = i < 2   ? is_array(c[i], code, {B, H, Smax, D}, q)
+                      : i < 4 ? is_array(c[i], at::kFloat, {B, H, Smax / 64}, q)
+                              : is_array(c[i], at::kBFloat16, {B, H, 128, D}, q);
+    if (!fits || !c[i].is_contiguous() || !aligned(c[i], i == 2 || i == 3 ? 4 : 16)) return none();
+    for (int j = 0; j < i; ++j) {
+      const char *x = static_cast<const char*>(c[i].const_data_ptr()), *y = static_cast<const char*>(c[j].const_data_ptr());
+      if (x < y + c[j].nbytes() && y < x + c[i].nbytes()) return none();
+    }
+  }
+  if (PyLong_CheckExact(a[9])) {
+    Scalar s;
+    if (!get_scalar(a[9], &s) || s.v < 0 || s.v > Smax) return none();
+    len = s.v;
+  } else if (!get_tensor(a[9], &lens) || !meta(lens, q) || lens.numel() != B) {
+    return none();
+  }
+  if (a[10] == Py_None)
+    scale = 1.0 / std::sqrt((double)D);
+  else if (!get_double(a[10], &scale))
+    return none();
+  if (!get_bool(a[11], &causal)) return none();
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const Recorded call("prefixlm::kvcache_q8_attn", {q, c[0], c[1]});
+    const c10::DeviceGuard guard(q.device());
+    out = empty_like_on(q, {B, S, H, D}, at::kBFloat16);
+    prefixlm_kvcache8_args p{};
+    p.workspace_bytes = lib.kv8_ws(B, S, H, Smax);
+    Tensor ws;
+    if (p.workspace_bytes) {
+      ws = empty_like_on(q, {(int64_t)p.workspace_bytes}, at::kByte);
+      p.workspace = ws.data_ptr();
+    }
+    p.q = q.const_data_ptr();
+    p.k_codes = c[0].data_ptr();
+    p.v_codes = c[1].data_ptr();
+    p.k_scale = c[2].data_ptr<float>();
+    p.v_scale = c[3].data_ptr<float>();
+    p.k_recent = c[4].data_ptr();
+    p.v_recent = c[5].data_ptr();
+    p.out = out.data_ptr();
+    p.q_stride_b = q.stride(0), p.q_stride_s = q.stride(1), p.q_stride_h = q.stride(2);
+    if (has_new) {
+      p.k = k.const_data_ptr();
+      p.v = v.const_data_ptr();
+      p.k_stride_b = k.stride(0), p.k_stride_s = k.stride(1), p.k_stride_h = k.stride(2);
+      p.v_stride_b = v.stride(0), p.v_stride_s = v.stride(1), p.v_stride_h = v.stride(2);
+    }
+    p.out_stride_b = S * H * D, p.out_stride_s = H * D, p.out_stride_h = D;
+    p.cache_seqlens = lens.defined() ? lens.const_data_ptr<int32_t>() : nullptr;
+    p.cache_seqlen = (int32_t)len;
+    p.batch = (int32_t)B;
+    p.seqlen_q = (int32_t)S;
+    p.num_heads = (int32_t)H;
+    p.head_dim = (int32_t)D;
+    p.max_seqlen_cache = (int32_t)Smax;
+    p.code_int8 = code == at::kChar;
+    p.is_causal = i32(causal);
+    p.softmax_scale = (float)scale;
+    check(lib.kv8_fwd(&p, stream_of(q)), "prefixlm_kvcache8_fwd");
+    for (const Tensor& t : c) t.unsafeGetTensorImpl()->bump_version();   // the op writes them in place
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// logits, targets (tensor or None), entropy, top_k, ignore_index -> (logprob, entropy, top_logprobs,
+// top_ids), None where not asked for
+PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x, x2;
+  LogprobCall c;
+  if (!ready(n, 5) || c10::InferenceMode::is_enabled() || !get_tensor(a[0], &x)) return none();
+  if (a[1] != Py_None && !get_tensor(a[1], &c.targets)) return none();
+  if (!get_bool(a[2], &c.entropy) || !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[4])) return none();
+  c.top = PyLong_AsLongLong(a[3]);
+  c.ignore = PyLong_AsLongLong(a[4]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  {
+    pybind11::gil_scoped_release no_gil;
+    const at::NoGradGuard no_grad;
+    x2 = logit_rows(x);
+  }
+  if (!x2.defined() || c.top < 0 || c.top > 64 || c.top > x2.size(1) || x2.size(1) > INT32_MAX ||
+      (c.targets.defined() && !whole_rows(c.targets, x.sizes().slice(0, x.dim() - 1), x)))
+    return none();
+  Tensor out[4];
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(x.device());
+    if (wants_grad(x)) {
+      const variable_list r = Logprobs::apply(x, x2.detach(), c);
+      size_t at = 0;
+      if (c.targets.defined()) out[0] = r[at++];
+      if (c.entropy) out[1] = r[at++];
+      if (c.top) {
+        out[2] = r[at++];
+        out[3] = r[at++];
+      }
+    } else {
+      const LogprobOut r = logprob_forward(x, x2, c);
+      out[0] = r.lp;
+      out[1] = r.ent;
+      out[2] = r.top;
+      out[3] = r.ids;
+    }
+  }
+  PyObject* t = PyTuple_New(4);
+  if (!t) return nullptr;
+  for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(t, i, out[i].defined() ? THPVariable_Wrap(out[i]) : none());
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// ids, table, scale, whether the rows are fp32, padding id
+PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor ids, table;
+  double scale;
+  bool wide;
+  if (!ready(n, 5) || c10::InferenceMode::is_enabled()) return none();
+  if (!get_tensor(a[0], &ids) || !get_tensor(a[1], &table) || !get_double(a[2], &scale) || !get_bool(a[3], &wide) ||
+      !PyLong_CheckExact(a[4]))
+    return none();
+  const int64_t padding = PyLong_AsLongLong(a[4]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  if (ids.numel() == 0 || !whole_rows(ids, ids.sizes(), table) || table.dim() != 2 || !float_rows(table, table.size(1)) ||
+      table.size(1) % 8 || table.numel() == 0 || table.size(1) > INT32_MAX)
+    return none();
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(table.device());
+    const auto dt = wide ? at::kFloat : at::kBFloat16;
+    y = wants_grad(table) ? Embedding::apply(ids, table, scale, dt, padding) : embedding_forward(ids, table, scale, dt);
+  }
+  return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
@@ -978,6 +1357,9 @@ PyMethodDef methods[] = {
     {"varlen", FAST(py_varlen), nullptr},
     {"layer", FAST(py_layer), nullptr},
     {"kvcache", FAST(py_kvcache), nullptr},
+    {"kvcache_q8", FAST(py_kvcache_q8), nullptr},
+    {"token_logprobs", FAST(py_token_logprobs), nullptr},
+    {"embedding", FAST(py_embedding), nullptr},
     {"swiglu", FAST(py_swiglu), nullptr},
     {"rms_norm", FAST(py_rms_norm), nullptr},
     {"add_rmsnorm", FAST(py_add_rmsnorm), nullptr},

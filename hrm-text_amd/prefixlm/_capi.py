@@ -145,6 +145,41 @@ class ProjGemmArgs(ctypes.Structure):
     ]
 
 
+class Kvcache8Args(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("k", c_vp), ("v", c_vp), ("k_codes", c_vp), ("v_codes", c_vp), ("k_scale", c_vp),
+        ("v_scale", c_vp), ("k_recent", c_vp), ("v_recent", c_vp), ("out", c_vp),
+        ("q_stride_b", c_i64), ("q_stride_s", c_i64), ("q_stride_h", c_i64),
+        ("k_stride_b", c_i64), ("k_stride_s", c_i64), ("k_stride_h", c_i64),
+        ("v_stride_b", c_i64), ("v_stride_s", c_i64), ("v_stride_h", c_i64),
+        ("out_stride_b", c_i64), ("out_stride_s", c_i64), ("out_stride_h", c_i64),
+        ("cache_seqlens", c_vp), ("cache_seqlen", c_i32),
+        ("batch", c_i32), ("seqlen_q", c_i32), ("num_heads", c_i32), ("head_dim", c_i32),
+        ("max_seqlen_cache", c_i32), ("code_int8", c_i32), ("is_causal", c_i32), ("softmax_scale", c_f32),
+        ("workspace", c_vp), ("workspace_bytes", c_sz),
+    ]
+
+
+class LogprobArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("targets", c_vp), ("logprob", c_vp), ("entropy", c_vp), ("stats", c_vp),
+        ("top_logprobs", c_vp), ("top_ids", c_vp), ("dlogprob", c_vp), ("dentropy", c_vp), ("dx", c_vp),
+        ("x_stride", c_i64), ("dx_stride", c_i64), ("rows", c_i64), ("vocab", c_i64), ("ignore_index", c_i64),
+        ("top_k", c_i32), ("x_fp32", c_i32), ("targets_int32", c_i32),
+        ("workspace", c_vp), ("workspace_bytes", c_sz),
+    ]
+
+
+class EmbeddingArgs(ctypes.Structure):
+    _fields_ = [
+        ("ids", c_vp), ("table", c_vp), ("y", c_vp), ("dy", c_vp), ("grad", c_vp),
+        ("table_stride", c_i64), ("y_stride", c_i64), ("dy_stride", c_i64),
+        ("tokens", c_i64), ("vocab", c_i64), ("padding_id", c_i64),
+        ("cols", c_i32), ("table_fp32", c_i32), ("y_fp32", c_i32), ("ids_int32", c_i32), ("scale", c_f32),
+        ("workspace", c_vp), ("workspace_bytes", c_sz),
+    ]
+
+
 # every symbol include/prefixlm.h declares, with (restype, argtypes)
 SIGNATURES = {
     "prefixlm_fwd_workspace_size": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32]),
@@ -169,6 +204,14 @@ SIGNATURES = {
     "prefixlm_proj_gemm": (ctypes.c_int, [ctypes.POINTER(ProjGemmArgs), c_vp]),
     "prefixlm_kvcache_workspace_size": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32]),
     "prefixlm_kvcache_fwd": (ctypes.c_int, [ctypes.POINTER(KvcacheArgs), c_vp]),
+    "prefixlm_kvcache8_workspace_size": (c_sz, [c_i32, c_i32, c_i32, c_i32]),
+    "prefixlm_kvcache8_fwd": (ctypes.c_int, [ctypes.POINTER(Kvcache8Args), c_vp]),
+    "prefixlm_logprob_workspace_size": (c_sz, [c_i64, c_i64, c_i32]),
+    "prefixlm_logprob_fwd": (ctypes.c_int, [ctypes.POINTER(LogprobArgs), c_vp]),
+    "prefixlm_logprob_bwd": (ctypes.c_int, [ctypes.POINTER(LogprobArgs), c_vp]),
+    "prefixlm_embedding_workspace_size": (c_sz, [c_i64, c_i64, c_i32]),
+    "prefixlm_embedding_fwd": (ctypes.c_int, [ctypes.POINTER(EmbeddingArgs), c_vp]),
+    "prefixlm_embedding_bwd": (ctypes.c_int, [ctypes.POINTER(EmbeddingArgs), c_vp]),
     "prefixlm_plan_build": (ctypes.c_int, [_c_i32p, _c_i32p, _c_i32p, c_i32, c_i32, c_i32, c_i32, c_vp, c_sz]),
     "prefixlm_last_error": (ctypes.c_char_p, []),
     "prefixlm_version": (c_i32, []),

@@ -25,7 +25,10 @@ _ENTRY_POINTS = ("prefixlm_fwd", "prefixlm_bwd", "prefixlm_fwd_q_amax_count", "p
                  "prefixlm_bwd_workspace_size", "prefixlm_bwd_ds_bytes", "prefixlm_bwd_ds_bytes_blocks",
                  "prefixlm_rope", "prefixlm_swiglu_fwd", "prefixlm_swiglu_bwd", "prefixlm_rmsnorm_fwd",
                  "prefixlm_rmsnorm_bwd", "prefixlm_add_rmsnorm", "prefixlm_proj_gemm", "prefixlm_proj_gemm_scaled",
-                 "prefixlm_kvcache_workspace_size", "prefixlm_kvcache_fwd", "prefixlm_last_error")
+                 "prefixlm_kvcache_workspace_size", "prefixlm_kvcache_fwd", "prefixlm_kvcache8_workspace_size",
+                 "prefixlm_kvcache8_fwd", "prefixlm_logprob_workspace_size", "prefixlm_logprob_fwd",
+                 "prefixlm_logprob_bwd", "prefixlm_embedding_workspace_size", "prefixlm_embedding_fwd",
+                 "prefixlm_embedding_bwd", "prefixlm_last_error")
 
 _lock = threading.Lock()
 _module = None

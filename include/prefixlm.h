@@ -367,6 +367,111 @@ size_t prefixlm_kvcache_workspace_size(int32_t batch, int32_t seqlen_q, int32_t 
                                        int32_t max_seqlen_cache);
 int prefixlm_kvcache_fwd(const prefixlm_kvcache_args* args, void* stream);
 
+/* KV-cache attention over a cache held in 8 bits (see prefixlm_kvcache_fwd for the queries, the new
+ * rows, the lengths and the masks). The cache, contiguous, of B batch rows and H heads:
+ *   k_codes, v_codes    [B, H, Smax, 128]   e4m3 or int8; row j of a block of 64 is scale * code
+ *   k_scale, v_scale    fp32 [B, H, Smax / 64]
+ *   k_recent, v_recent  bf16 [B, H, 128, 128], row j in slot j % 128
+ * Smax is a multiple of 64. Rows below len / 64 * 64 are attended from the codes, rows from there to
+ * len - 1 from k_recent, v_recent, the call's new rows as given. Afterwards the blocks that the new
+ * rows complete are rounded: scale = max(largest magnitude times the fp32 value of 1/448 (e4m3) or
+ * 1/127 (int8), 2^-126), code = round(row / scale) to nearest, ties to even; and the new rows among the last 64 before the
+ * incomplete block and those in it are written to k_recent, v_recent. So up to 64 rows can be taken
+ * back by calling with a smaller len. Lengths outside [0, Smax] count as the nearest of the two. */
+typedef struct prefixlm_kvcache8_args {
+  const void* q;
+  const void* k;                 /* new rows, or NULL (k and v together): attend the cache only */
+  const void* v;
+  void* k_codes;
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  void* k_recent;
+  void* v_recent;
+  void* out;
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  int64_t out_stride_b, out_stride_s, out_stride_h;
+  const int32_t* cache_seqlens;  /* device int32 [B], or NULL */
+  int32_t cache_seqlen;          /* used when cache_seqlens is NULL */
+  int32_t batch;                 /* B */
+  int32_t seqlen_q;              /* S */
+  int32_t num_heads;             /* H */
+  int32_t head_dim;              /* 128 */
+  int32_t max_seqlen_cache;      /* Smax */
+  int32_t code_int8;             /* codes: 0 e4m3, 1 int8 */
+  int32_t is_causal;
+  float softmax_scale;
+  void* workspace;               /* >= prefixlm_kvcache8_workspace_size(...) bytes */
+  size_t workspace_bytes;
+} prefixlm_kvcache8_args;
+size_t prefixlm_kvcache8_workspace_size(int32_t batch, int32_t seqlen_q, int32_t num_heads, int32_t max_seqlen_cache);
+int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* args, void* stream);
+
+/* Log probabilities of given tokens from logits, with the entropy and the top alternatives (the
+ * cross entropy of models/lm_head.py:52 is -logprob), and the gradient of the logits. x: bf16 or
+ * fp32 [rows, vocab], unit stride over the vocabulary, any row stride, aligned to its element.
+ * Forward: stats [rows, 2], each row's largest logit and the log of its sum of e^(logit - largest)
+ * (kept for the backward); logprob [rows] of targets[row], 0 where the target
+ * is ignore_index and NaN where it is any other index outside the vocabulary; entropy [rows] unless
+ * NULL; the top_k largest logits' log probabilities and indices [rows, top_k], largest first, the
+ * lower index first among equal ones. targets (int64, or int32 with targets_int32) may be NULL with
+ * logprob. fp32 statistics. Backward: dx [rows, vocab] in x's type from the gradients dlogprob and
+ * dentropy (either may be NULL; dentropy needs the forward's entropy). A forward without entropy
+ * and top_k does not read the rows whose target is ignore_index (their stats are 0). */
+typedef struct prefixlm_logprob_args {
+  const void* x;
+  const void* targets;
+  float* logprob;
+  float* entropy;
+  float* stats;
+  float* top_logprobs;           /* fp32 [rows, top_k], with top_k > 0 */
+  int64_t* top_ids;              /* [rows, top_k], with top_k > 0 */
+  const float* dlogprob;         /* backward only */
+  const float* dentropy;         /* backward only */
+  void* dx;                      /* backward only */
+  int64_t x_stride, dx_stride;
+  int64_t rows, vocab;
+  int64_t ignore_index;
+  int32_t top_k;                 /* 0 to min(64, vocab) */
+  int32_t x_fp32;                /* x and dx: 0 bf16, 1 fp32 */
+  int32_t targets_int32;
+  void* workspace;               /* forward: >= prefixlm_logprob_workspace_size(...) bytes */
+  size_t workspace_bytes;
+} prefixlm_logprob_args;
+size_t prefixlm_logprob_workspace_size(int64_t rows, int64_t vocab, int32_t top_k);
+int prefixlm_logprob_fwd(const prefixlm_logprob_args* args, void* stream);
+int prefixlm_logprob_bwd(const prefixlm_logprob_args* args, void* stream);
+
+/* Scaled embedding lookup (models/lm_head.py:34-43) and the gradient of its table.
+ * Forward: y[i] = scale * table[ids[i]], fp32 product, one rounding; ids outside [0, vocab) give
+ * NaN rows. Backward: grad[v] = scale * sum of dy[i] over the tokens with ids[i] = v, added in fp32
+ * in the order of i and rounded once; the whole [vocab, cols] gradient is written, zero where no
+ * token is. Ids outside the table and padding_id (negative: none) have no gradient. Bitwise
+ * deterministic. table and grad, and y and dy, bf16 or fp32; ids int64, or int32 with ids_int32.
+ * Unit column stride, cols % 8 == 0, rows 16-byte aligned; grad contiguous; vocab < 2^27. */
+typedef struct prefixlm_embedding_args {
+  const void* ids;
+  const void* table;             /* forward only */
+  void* y;                       /* forward output [tokens, cols] */
+  const void* dy;                /* backward only [tokens, cols] */
+  void* grad;                    /* backward output [vocab, cols] */
+  int64_t table_stride, y_stride, dy_stride;
+  int64_t tokens, vocab;
+  int64_t padding_id;            /* backward only */
+  int32_t cols;
+  int32_t table_fp32;            /* table and grad: 0 bf16, 1 fp32 */
+  int32_t y_fp32;                /* y and dy */
+  int32_t ids_int32;
+  float scale;
+  void* workspace;               /* backward: >= prefixlm_embedding_workspace_size(...) bytes */
+  size_t workspace_bytes;
+} prefixlm_embedding_args;
+size_t prefixlm_embedding_workspace_size(int64_t tokens, int64_t vocab, int32_t cols);
+int prefixlm_embedding_fwd(const prefixlm_embedding_args* args, void* stream);
+int prefixlm_embedding_bwd(const prefixlm_embedding_args* args, void* stream);
+
 /* Synchronizes `stream` and reports the metadata error word the last call on this
  * workspace recorded (0 = consistent). Returns PREFIXLM_ERR_METADATA if it is nonzero.
  * The reference asserts instead (models/flash_attention_prefixlm_v2.py:103,169). */
