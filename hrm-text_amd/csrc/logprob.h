@@ -42,9 +42,12 @@ struct Params {
   int top, wide_targets, nsplit;
 };
 
-// 8 consecutive elements, at any address that suits one element: the target handles 16-byte
-// accesses at any alignment
-typedef u32x4 u32x4_u __attribute__((aligned(2)));
+// 8 consecutive elements, a row's vectors. The row's edges are what lies before the first vector and
+// behind the last whole one, at most 14 elements, each of which one thread takes. A row may begin at
+// any element. The forward's vectors begin with the row, so that a row's sums are added in one order
+// wherever it lies (and cost a sixth more off 16 bytes: 1021 rows of 50257 logits 27.6 us, of 50256
+// 24.0); the gradient's, which have no order, at its first 16-byte address.
+typedef u32x4 u32x4_u __attribute__((aligned(2)));   // the target handles these at any alignment
 typedef f32x4 f32x4_u __attribute__((aligned(4)));
 template <class T>
 struct Vec;
@@ -63,6 +66,17 @@ struct Vec<float> {
   }
   __device__ __forceinline__ float get(int e) const { return w[e >> 2][e & 3]; }
 };
+struct Edges {
+  int lead, rest;      // elements before the vectors, and behind
+  int64_t nvec;
+  __device__ __forceinline__ Edges(int lead_, int64_t V) {
+    lead = (int)(lead_ < V ? lead_ : V);
+    nvec = (V - lead) / 8;
+    rest = (int)(V - lead - 8 * nvec);
+  }
+  __device__ __forceinline__ int count() const { return lead + rest; }
+  __device__ __forceinline__ int64_t at(int i) const { return i < lead ? i : 8 * nvec + i; }
+};
 __device__ __forceinline__ float as_f32(bf16 x) { return (float)x; }
 __device__ __forceinline__ float as_f32(float x) { return x; }
 
@@ -78,6 +92,10 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 // larger value first, then lower index; never 0
 __device__ __forceinline__ unsigned long long key_of(float x, int64_t j) {
   return ((unsigned long long)order_of(x) << 32) | (0xffffffffu - (uint32_t)j);
+}
+
+__device__ __forceinline__ float first_lane(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
 }
 
 // The running (m, S, W): S and W against ref(m), 0 where m is -inf
@@ -105,9 +123,9 @@ __device__ __forceinline__ void join(Stat& a, Stat b) {
   if (ENT) a.w += b.w;
 }
 
-// a takes the N values f
+// a takes the N values f, whose largest is returned
 template <bool ENT, int N>
-__device__ __forceinline__ void take(Stat& a, const float (&f)[N]) {
+__device__ __forceinline__ float take(Stat& a, const float (&f)[N]) {
   float mx = f[0];
 #pragma unroll
   for (int e = 1; e < N; ++e) mx = fmaxf(mx, f[e]);
@@ -119,6 +137,7 @@ __device__ __forceinline__ void take(Stat& a, const float (&f)[N]) {
     a.s += ex;
     if (ENT) a.w += ex * below(d);
   }
+  return mx;
 }
 
 __device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long x) {
@@ -129,30 +148,13 @@ __device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long x)
   }
   return x;
 }
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t x) {
-  auto step = [&](auto ctrl) {
-    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xF, 0xF, false);
-    x = y > x ? y : x;
-  };
-  step(std::integral_constant<int, 0xB1>{});
-  step(std::integral_constant<int, 0x4E>{});
-  step(std::integral_constant<int, 0x141>{});
-  step(std::integral_constant<int, 0x140>{});
-  uint32_t r = 0;
-#pragma unroll
-  for (int l = 0; l < 64; l += 16) {
-    const uint32_t y = (uint32_t)__builtin_amdgcn_readlane((int)x, l);
-    r = y > r ? y : r;
-  }
-  return r;
-}
-
 // What a workgroup holds while it picks the top elements
+constexpr int kGroups = 8;        // of a thread's vectors, by their turn
 struct TopShared {
   unsigned long long cand[kCand];
-  uint32_t keys[NT];
+  float largest[kGroups][NT];     // of each thread's values in a group
+  uint32_t keys[NT / 8];
   unsigned long long best[NT / 64];
-  uint32_t thr;
   int n;
 };
 
@@ -167,41 +169,47 @@ __device__ __forceinline__ void sorted_top(const unsigned long long* cand, int n
   }
 }
 
-// What a row's result is, from its statistics
-__device__ __forceinline__ void finish_row(const Params& P, int64_t row, const Stat& a, float xt, bool counted, bool valid) {
-  const float ln_s = logf(a.s), r = ref_of(a.m);   // all logits -inf: ln 0
-  P.stats[2 * row] = r;
-  P.stats[2 * row + 1] = ln_s;
-  if (P.logprob) P.logprob[row] = !counted ? 0.f : !valid ? __builtin_nanf("") : (xt - r) - ln_s;
-  if (P.entropy) P.entropy[row] = a.s == 0.f ? __builtin_nanf("") : ln_s - a.w / a.s;
-}
 __device__ __forceinline__ int64_t target_of(const Params& P, int64_t row) {
   return P.wide_targets ? static_cast<const int64_t*>(P.targets)[row] : (int64_t) static_cast<const int32_t*>(P.targets)[row];
 }
+// A row's target and its logit
+struct Target {
+  bool counted, valid;
+  float x;
+};
 template <class T>
-__device__ __forceinline__ void finish(const Params& P, int64_t row, const Stat& a) {
-  bool counted = false, valid = false;
-  float xt = 0.f;
+__device__ __forceinline__ Target target_at(const Params& P, int64_t row) {
+  Target r{false, false, 0.f};
   if (P.targets) {
     const int64_t t = target_of(P, row);
-    counted = t != P.ignore;
-    valid = t >= 0 && t < P.V;
-    if (counted && valid) xt = as_f32(static_cast<const T*>(P.x)[row * P.x_st + t]);
+    r.counted = t != P.ignore;
+    r.valid = t >= 0 && t < P.V;
+    if (r.counted && r.valid) r.x = as_f32(static_cast<const T*>(P.x)[row * P.x_st + t]);
   }
-  finish_row(P, row, a, xt, counted, valid);
+  return r;
+}
+
+// What a row's result is, from its statistics
+__device__ __forceinline__ void finish_row(const Params& P, int64_t row, const Stat& a, const Target& t) {
+  const float ln_s = logf(a.s), r = ref_of(a.m);   // all logits -inf: ln 0
+  P.stats[2 * row] = r;
+  P.stats[2 * row + 1] = ln_s;
+  if (P.logprob) P.logprob[row] = !t.counted ? 0.f : !t.valid ? __builtin_nanf("") : (t.x - r) - ln_s;
+  if (P.entropy) P.entropy[row] = a.s == 0.f ? __builtin_nanf("") : ln_s - a.w / a.s;
 }
 
 // Workgroup = (row, split of its vectors); thread = every NT-th vector of 8 logits, with a running
 // (m, S, W) of its own, joined at the end. One pass over the row.
 //
-// TOP: each thread's largest value is known after the pass. The k-th largest of those is reached by
-// at least k elements, so only threads whose largest reaches it look at their elements again (about
-// k of NT), and those elements, mostly little more than k, are ranked against each other. Where
-// they do not fit (rows of many equal values), or a NaN is among them, which the maxima pass over, a
-// walk finds the next largest k times.
+// TOP: after the pass the largest values of 64 sets of 8 threads are known. The k-th largest of those
+// is reached by at least k elements, so only threads whose own largest reaches it look at their
+// elements again, and only at the groups whose largest does; those that reach it, mostly few more
+// than k, are ranked against each other. Where they do not fit (rows of many equal values), or a NaN
+// is among them, which the maxima pass over, a walk finds the next largest k times.
 template <class T, bool ENT, bool TOP>
 __global__ __launch_bounds__(NT) void forward_kernel(Params P) {
   __shared__ Stat s_stat[NT / 64];
+  __shared__ TopShared t;   // unused without TOP
   const int64_t row = blockIdx.x / P.nsplit;
   const int split = (int)(blockIdx.x % P.nsplit);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -213,112 +221,150 @@ __global__ __launch_bounds__(NT) void forward_kernel(Params P) {
     }
     return;
   }
-  const int64_t nv = (P.V + 7) / 8, full = P.V / 8;   // the last vector may be partial
-  const int64_t per = (nv + P.nsplit - 1) / P.nsplit;
-  const int64_t v0 = split * per, v1 = v0 + per < nv ? v0 + per : nv, vf = v1 < full ? v1 : full;
+  const Edges edges(0, P.V);
+  const int64_t per = (edges.nvec + P.nsplit - 1) / P.nsplit;
+  const int64_t v0 = split * per < edges.nvec ? split * per : edges.nvec, v1 = v0 + per < edges.nvec ? v0 + per : edges.nvec;
+  const int n_edge = split == 0 ? edges.count() : 0;
 
+  Target target{false, false, 0.f};
+  if (tid == 0 && P.nsplit == 1) target = target_at<T>(P, row);
+  if (TOP)
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) t.largest[i][tid] = -INFINITY;
+  // groups of kUnroll vectors a thread, the next one on its way while one is taken; vectors past the
+  // last one are read as that one and count as -inf
   Stat a = no_values();
-  int64_t v = v0 + tid;
-  for (; v + (kUnroll - 1) * NT < vf; v += kUnroll * NT) {
+  const float edge = tid < n_edge ? as_f32(x[edges.at(tid)]) : -INFINITY;
+  if (v0 < v1) {
     Vec<T> w[kUnroll];
+    auto load = [&](int64_t g) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) w[u].load(x + 8 * (v + u * NT));
-    float f[8 * kUnroll];
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t v = g + u * NT + tid;
+        w[u].load(x + 8 * (v < v1 ? v : v1 - 1));
+      }
+    };
+    load(v0);
+    int turn = 0;
+    for (int64_t g = v0; g < v1; g += kUnroll * NT) {
+      float f[8 * kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+      for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[8 * u + e] = w[u].get(e);
-    take<ENT>(a, f);
-  }
-  for (; v < v1; v += NT) {
-    if (v < full) {
-      Vec<T> w;
-      w.load(x + 8 * v);
-      float f[8];
+        for (int e = 0; e < 8; ++e) f[8 * u + e] = w[u].get(e);
+      if (g + kUnroll * NT < v1) load(g + kUnroll * NT);
+      if (g + kUnroll * NT > v1) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = w.get(e);
-      take<ENT>(a, f);
-    } else {
-      for (int64_t j = 8 * v; j < P.V; ++j) {
-        const float f[1] = {as_f32(x[j])};
-        take<ENT>(a, f);
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[8 * u + e] = g + u * NT + tid < v1 ? f[8 * u + e] : -INFINITY;
+      }
+      const float mx = take<ENT>(a, f);
+      if (TOP) {
+        float* l = &t.largest[turn & (kGroups - 1)][tid];
+        *l = turn < kGroups ? mx : fmaxf(*l, mx);
+        ++turn;
       }
     }
   }
+  if (tid < n_edge) {
+    const float f[1] = {edge};
+    take<ENT>(a, f);
+  }
   const float m_thread = a.m;
-  const bool any = v0 + tid < v1;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
+  const bool any = v0 + tid < v1 || tid < n_edge;
+  auto join_lanes = [&](int m) {
     Stat b;
     b.m = __shfl_xor(a.m, m);
     b.s = __shfl_xor(a.s, m);
     b.w = ENT ? __shfl_xor(a.w, m) : 0.f;
     join<ENT>(a, b);
-  }
+  };
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) join_lanes(m);
   if (lane == 0) s_stat[wave] = a;
   __syncthreads();
+  a = s_stat[lane & (NT / 64 - 1)];
+#pragma unroll
+  for (int m = 1; m < NT / 64; m <<= 1) join_lanes(m);
+  // the workgroup's: the first lane's, whose joins run in one order in every wave (the lanes' differ
+  // in their last bit, and which of them holds an alternative is not fixed)
+  a.m = first_lane(a.m);
+  a.s = first_lane(a.s);
+  a.w = first_lane(a.w);
   if (tid == 0) {
-    a = s_stat[0];
-    for (int g = 1; g < NT / 64; ++g) join<ENT>(a, s_stat[g]);
     if (P.nsplit == 1) {
-      finish<T>(P, row, a);
+      finish_row(P, row, a, target);
     } else {
       float* p = P.part + (row * P.nsplit + split) * 4;
       p[0] = a.m;
       p[1] = a.s;
       p[2] = a.w;
     }
-    s_stat[0] = a;
   }
   if (!TOP) return;
 
-  __shared__ TopShared t;
   const int top = P.top;
-  t.keys[tid] = any ? order_of(m_thread) : 0;
-  if (tid == 0) t.n = 0;
-  __syncthreads();   // and s_stat[0] is the workgroup's
-  if (wave == 0) {
-    // the top-th largest of the threads' largest
-    uint32_t mine[NT / 64];
+  {
+    uint32_t k = any ? order_of(m_thread) : 0;
+    auto step = [&](auto ctrl) {   // over each 8 lanes
+      const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)k, decltype(ctrl)::value, 0xF, 0xF, false);
+      k = y > k ? y : k;
+    };
+    step(std::integral_constant<int, 0xB1>{});
+    step(std::integral_constant<int, 0x4E>{});
+    step(std::integral_constant<int, 0x141>{});
+    if ((lane & 7) == 0) t.keys[tid >> 3] = k;
+    if (tid == 0) t.n = 0;
+  }
+  __syncthreads();
+  static_assert(NT / 8 == 64 && kMaxTop <= 64, "one set a lane, and a top-th largest of them");
+  uint32_t thr;
+  {
+    const uint32_t k = t.keys[lane];
+    int rank = 0;
 #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) mine[i] = t.keys[i * 64 + lane];
-    uint32_t thr = 0;
-    for (int r = 0; r < top; ++r) {
-      uint32_t b = mine[0];
+    for (int j = 0; j < 64; ++j) {
+      const uint32_t y = (uint32_t)__builtin_amdgcn_readlane((int)k, j);
+      rank += y > k || (y == k && j < lane);
+    }
+    thr = (uint32_t)__builtin_amdgcn_readlane((int)k, (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(rank == top - 1)));
+  }
+  // fewer sets with elements than `top`: every element (none of them NaN, or the walk decides)
+  const float least = thr ? value_of(thr) : -INFINITY;
+  if (any && m_thread >= least) {
+    auto look = [&](float f, int64_t j) {
+      if (f >= least) {
+        const int at = atomicAdd(&t.n, 1);   // the order does not matter: they are ranked
+        if (at < kCand) t.cand[at] = key_of(f, j);
+      }
+    };
+    for (int i = 0; i < kGroups; ++i) {
+      if (!(t.largest[i][tid] >= least)) continue;
+      for (int64_t g = v0 + (int64_t)i * kUnroll * NT; g < v1; g += kGroups * kUnroll * NT) {
+        Vec<T> w[kUnroll];
 #pragma unroll
-      for (int i = 1; i < NT / 64; ++i) b = mine[i] > b ? mine[i] : b;
-      thr = wave_max_u32(b);
-      // one of the threads that hold it is done
-      const unsigned long long who = __builtin_amdgcn_ballot_w64(b == thr);
-      if (lane == (int)__builtin_ctzll(who)) {
-        bool gone = false;
+        for (int u = 0; u < kUnroll; ++u)
+          if (g + u * NT + tid < v1) w[u].load(x + 8 * (g + u * NT + tid));
 #pragma unroll
-        for (int i = 0; i < NT / 64; ++i) {
-          const bool hit = !gone && mine[i] == thr;
-          gone |= hit;
-          mine[i] = hit ? 0 : mine[i];
+        for (int u = 0; u < kUnroll; ++u) {
+          if (g + u * NT + tid >= v1) break;
+          float m = w[u].get(0);
+#pragma unroll
+          for (int e = 1; e < 8; ++e) m = fmaxf(m, w[u].get(e));
+          if (m >= least)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) look(w[u].get(e), 8 * (g + u * NT + tid) + e);
         }
       }
     }
-    if (lane == 0) t.thr = thr;
+    if (tid < n_edge) look(edge, edges.at(tid));
   }
   __syncthreads();
-  const uint32_t thr = t.thr;
-  if (any && order_of(m_thread) >= thr) {
-    for (int64_t u = v0 + tid; u < v1; u += NT)
-      for (int64_t j = 8 * u; j < 8 * u + 8 && j < P.V; ++j) {
-        const float f = as_f32(x[j]);
-        if (order_of(f) >= thr) {
-          const int at = atomicAdd(&t.n, 1);   // the order does not matter: they are ranked
-          if (at < kCand) t.cand[at] = key_of(f, j);
-        }
-      }
-  }
-  __syncthreads();
-  const float ln_s = logf(s_stat[0].s), ref = ref_of(s_stat[0].m);
+  const float ln_s = logf(a.s), ref = ref_of(a.m);
   // a split may hold fewer elements than `top`: the rest of its list is empty
-  const int64_t held = (8 * v1 < P.V ? 8 * v1 : P.V) - 8 * v0;
-  const int want = held < top ? (held > 0 ? (int)held : 0) : top;
+  const int64_t held = 8 * (v1 - v0) + n_edge;
+  const int want = held < top ? (int)held : top;
   auto put = [&](int r, unsigned long long c) {
     if (P.nsplit == 1) {
       P.top_val[row * top + r] = (value_of((uint32_t)(c >> 32)) - ref) - ln_s;
@@ -329,18 +375,24 @@ __global__ __launch_bounds__(NT) void forward_kernel(Params P) {
   };
   if (P.nsplit > 1 && tid >= want && tid < top) P.part_top[(row * P.nsplit + split) * top + tid] = 0;
   const int n = t.n;
-  if (n >= want && n <= kCand && s_stat[0].s == s_stat[0].s) {
+  if (n >= want && n <= kCand && a.s == a.s) {
     sorted_top(t.cand, n, want, put);
     return;
   }
   unsigned long long last = ~0ull;
   for (int r = 0; r < want; ++r) {
     unsigned long long b = 0;
-    for (int64_t u = v0 + tid; u < v1; u += NT)
-      for (int64_t j = 8 * u; j < 8 * u + 8 && j < P.V; ++j) {
-        const unsigned long long c = key_of(as_f32(x[j]), j);
-        if (c < last && c > b) b = c;
-      }
+    auto look = [&](float f, int64_t j) {
+      const unsigned long long c = key_of(f, j);
+      if (c < last && c > b) b = c;
+    };
+    for (int64_t u = v0 + tid; u < v1; u += NT) {
+      Vec<T> w;
+      w.load(x + 8 * u);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) look(w.get(e), 8 * u + e);
+    }
+    if (tid < n_edge) look(edge, edges.at(tid));
     b = wave_max_u64(b);
     if (lane == 0) t.best[wave] = b;
     __syncthreads();
@@ -387,7 +439,7 @@ __global__ __launch_bounds__(256) void combine_kernel(Params P) {
     }
     if (tid == 0) {
       s_row = a;
-      finish<T>(P, row, a);
+      finish_row(P, row, a, target_at<T>(P, row));
     }
   }
   if (!TOP) return;
@@ -400,10 +452,13 @@ __global__ __launch_bounds__(256) void combine_kernel(Params P) {
   });
 }
 
-// thread = vectors of 8 logits of one row; blockIdx.x = (row, block of 256 kUnroll vectors)
+// thread = vectors of 8 logits of one row; blockIdx.x = (row, block of 256 kUnroll vectors). The
+// vectors begin where the gradient's row is aligned; the logits' row mostly is there too. The rows go
+// from the last to the first: what the forward read last is read first, and partly still in the
+// last-level cache.
 template <class T, bool ENT>
 __global__ __launch_bounds__(256) void backward_kernel(Params P, int nblk) {
-  const int64_t row = blockIdx.x / nblk;
+  const int64_t row = P.rows - 1 - blockIdx.x / nblk;
   const int64_t v0 = (int64_t)(blockIdx.x % nblk) * 256 * kUnroll + threadIdx.x;
   const T* x = static_cast<const T*>(P.x) + row * P.x_st;
   T* dx = static_cast<T*>(P.dx) + row * P.dx_st;
@@ -414,35 +469,37 @@ __global__ __launch_bounds__(256) void backward_kernel(Params P, int nblk) {
   const float h = ENT && P.h ? P.h[row] : 0.f, H = ENT ? P.entropy[row] : 0.f;
   const float m = P.stats[2 * row], ln_s = P.stats[2 * row + 1];
   const bool zero = g == 0.f && h == 0.f;
+  const Edges edges((int)((16 - ((uintptr_t)dx & 15)) % 16 / sizeof(T)), P.V);
   auto grad = [&](float f, int64_t j) {
     const float l = (f - m) - ln_s, p = __builtin_amdgcn_exp2f(l * kLog2e);
     float d = -g * p;
     if (ENT) d -= h * (p * (below(l) + H));
     return j == t ? d + g : d;
   };
+  Vec<T> w[kUnroll];
+  if (!zero) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (v0 + u * 256 < edges.nvec) w[u].load(x + edges.lead + 8 * (v0 + u * 256));
+  }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t j0 = 8 * (v0 + u * 256);
-    if (j0 + 8 <= P.V) {
-      float d[8];
+    if (v0 + u * 256 >= edges.nvec) break;
+    const int64_t j0 = edges.lead + 8 * (v0 + u * 256);
+    float d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = 0.f;
-      if (!zero) {
-        Vec<T> w;
-        w.load(x + j0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = grad(w.get(e), j0 + e);
-      }
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<u32x4_u*>(dx + j0) =
-            __builtin_bit_cast(u32x4, cvt8(d[0], d[1], d[2], d[3], d[4], d[5], d[6], d[7]));
-      } else {
-        reinterpret_cast<f32x4_u*>(dx + j0)[0] = f32x4{d[0], d[1], d[2], d[3]};
-        reinterpret_cast<f32x4_u*>(dx + j0)[1] = f32x4{d[4], d[5], d[6], d[7]};
-      }
+    for (int e = 0; e < 8; ++e) d[e] = zero ? 0.f : grad(w[u].get(e), j0 + e);
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<u32x4*>(dx + j0) =
+          __builtin_bit_cast(u32x4, cvt8(d[0], d[1], d[2], d[3], d[4], d[5], d[6], d[7]));
     } else {
-      for (int64_t j = j0; j < P.V; ++j) dx[j] = (T)(zero ? 0.f : grad(as_f32(x[j]), j));
+      reinterpret_cast<f32x4*>(dx + j0)[0] = f32x4{d[0], d[1], d[2], d[3]};
+      reinterpret_cast<f32x4*>(dx + j0)[1] = f32x4{d[4], d[5], d[6], d[7]};
     }
+  }
+  if (blockIdx.x % nblk == 0 && (int)threadIdx.x < edges.count()) {
+    const int64_t j = edges.at(threadIdx.x);
+    dx[j] = (T)(zero ? 0.f : grad(as_f32(x[j]), j));
   }
 }
 

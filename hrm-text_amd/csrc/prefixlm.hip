@@ -1369,11 +1369,13 @@ int prefixlm_timer_read(void* timer, float* total_ms, int32_t* launches) {
 }  // extern "C"
 
 // ---- log probabilities ---------------------------------------------------------------
-// Splits of a row: 512 workgroups where the rows alone are fewer than the CUs, of at least two
-// vectors a thread each.
+// Splits of a row, where the rows alone are fewer than the CUs and long enough to pay for the second
+// launch: 512 workgroups, of at least 8192 logits each. One split against several: 8 rows of 65536 logits
+// 7.1 and 9.5 us, of 131072 10.1 and 11.2, of 262144 17.1 and 10.6; with alternatives, whose search is
+// shorter in a split, of 65536 11.9 and 11.9, of 131072 15.3 and 13.5.
 static int lp_nsplit(int64_t rows, int64_t V, int32_t top) {
-  if (rows < 1 || rows >= 256) return 1;
-  const int64_t most = std::max<int64_t>(1, V / (16 * lp::NT)), want = (512 + rows - 1) / rows;
+  if (rows < 1 || rows >= 256 || V < (top > 0 ? 98304 : 163840)) return 1;
+  const int64_t most = V / (16 * lp::NT), want = (512 + rows - 1) / rows;
   const int64_t fit = top > 0 ? lp::kCand / top : lp::kMaxSplits;
   return (int)std::min({most, want, fit, (int64_t)lp::kMaxSplits});
 }
