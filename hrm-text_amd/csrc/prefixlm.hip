@@ -1400,6 +1400,13 @@ static void lp_fwd_launch(const lp::Params& P, hipStream_t stream) {
     P.top ? lp_fwd_launch<T, false, true>(P, stream) : lp_fwd_launch<T, false, false>(P, stream);
 }
 
+template <class T>
+static void lp_bwd_launch(const lp::Params& P, bool nt, int nblk, hipStream_t stream) {
+  auto* k = P.h ? (nt ? lp::backward_kernel<T, true, true> : lp::backward_kernel<T, true, false>)
+                : (nt ? lp::backward_kernel<T, false, true> : lp::backward_kernel<T, false, false>);
+  hipLaunchKernelGGL(k, dim3((unsigned)(P.rows * nblk)), dim3(256), 0, stream, P, nblk);
+}
+
 static int lp_call(const prefixlm_logprob_args* a, void* stream_, bool backward) {
   if (!a) return fail(PREFIXLM_ERR_INVALID, "args is null");
   if (a->rows < 0 || a->vocab < 1 || a->vocab > 0x7fffffff)
@@ -1437,9 +1444,11 @@ static int lp_call(const prefixlm_logprob_args* a, void* stream_, bool backward)
     const int64_t nblk = (a->vocab + 8 * 256 * lp::kUnroll - 1) / (8 * 256 * lp::kUnroll);
     if (a->rows * nblk > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many elements");
     (void)hipGetLastError();
-    auto* k = a->x_fp32 ? (P.h ? lp::backward_kernel<float, true> : lp::backward_kernel<float, false>)
-                        : (P.h ? lp::backward_kernel<bf16, true> : lp::backward_kernel<bf16, false>);
-    hipLaunchKernelGGL(k, dim3((unsigned)(a->rows * nblk)), dim3(256), 0, stream, P, (int)nblk);
+    const bool nt = 2 * a->rows * a->vocab * (int64_t)size > lp::kNtBytes;
+    if (a->x_fp32)
+      lp_bwd_launch<float>(P, nt, (int)nblk, stream);
+    else
+      lp_bwd_launch<bf16>(P, nt, (int)nblk, stream);
   } else {
     if (a->targets && !a->logprob) return fail(PREFIXLM_ERR_INVALID, "logprob is null");
     if (a->top_k && (!a->top_logprobs || !a->top_ids))
