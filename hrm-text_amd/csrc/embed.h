@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(FwdParams P) {
 constexpr int kBits = 9, kBins = 1 << kBits;   // a digit; two cover 2^18 ids
 constexpr int kSortThreads = 256, kSortWaves = kSortThreads / 64;
 constexpr int kMaxTiles = 128;
-constexpr int kRun = 64;                       // sorted tokens per wave of the sum
+constexpr int kMinRun = 16;                    // sorted tokens per wave of the sum: 16 or 32 (a lane has one)
 
 struct SortParams {
   const void* ids;          // first pass: the caller's ids; else null
@@ -107,21 +107,38 @@ __device__ __forceinline__ uint32_t key_at(const SortParams& P, int64_t i) {
   return id >= 0 && id < P.V && id != P.padding ? (uint32_t)id : (uint32_t)P.V;
 }
 
-// Workgroups past the sort's clear the gradient: the sort is a chain of short launches that leaves
-// the memory idle, and the clearing needs nothing from it.
-__device__ __forceinline__ bool clears(const SortParams& P) {
-  const int b = (int)blockIdx.x - P.tiles;
+// Workgroups past the sort's `sorting` clear the gradient: the sort is a chain of short steps that
+// leaves the memory idle, and the clearing needs nothing from it.
+template <int NTH>
+__device__ __forceinline__ bool clears(const SortParams& P, int sorting) {
+  const int b = (int)blockIdx.x - sorting;
   if (b < 0) return false;
-  const int64_t n = (int64_t)(gridDim.x - P.tiles) * kSortThreads;
+  const int64_t n = (int64_t)(gridDim.x - sorting) * NTH * 4;
   const u32x4 z = {0u, 0u, 0u, 0u};
-  for (int64_t i = P.zero_begin + (int64_t)b * kSortThreads + threadIdx.x; i < P.zero_end; i += n)
-    __builtin_nontemporal_store(z, static_cast<u32x4*>(P.zero) + i);
+  u32x4* const to = static_cast<u32x4*>(P.zero);
+  for (int64_t i = P.zero_begin + (int64_t)b * NTH * 4 + threadIdx.x; i < P.zero_end; i += n)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * NTH < P.zero_end) to[i + u * NTH] = z;
   return true;
+}
+
+// The lanes of this wave that are `in` and have this lane's digit: each sets its bit in the digit's
+// word of `same` (the wave's own, all zero before and again after), in LDS. Nine ballots and 64-bit
+// selects, the way without memory, take three times the instructions.
+__device__ __forceinline__ unsigned long long lanes_with(unsigned long long* same, uint32_t digit, bool in, int lane) {
+  if (in) atomicOr(&same[digit], 1ull << lane);
+  __builtin_amdgcn_wave_barrier();
+  const unsigned long long m = in ? same[digit] : 0;
+  __builtin_amdgcn_wave_barrier();
+  if (in && (m >> lane) == 1ull) same[digit] = 0;
+  __builtin_amdgcn_wave_barrier();
+  return m;
 }
 
 // How many of each digit a tile holds
 __global__ __launch_bounds__(kSortThreads) void histogram_kernel(SortParams P) {
-  if (clears(P)) return;
+  if (clears<kSortThreads>(P, P.tiles)) return;
   __shared__ uint32_t n[kBins];
   for (int d = threadIdx.x; d < kBins; d += kSortThreads) n[d] = 0;
   __syncthreads();
@@ -136,15 +153,19 @@ __global__ __launch_bounds__(kSortThreads) void histogram_kernel(SortParams P) {
 // of tokens with a lower digit, plus those of the same digit in earlier tiles, in earlier waves'
 // parts of this tile, and before it in its wave's part.
 __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortParams P) {
-  if (clears(P)) return;
+  if (clears<kSortThreads>(P, P.tiles)) return;
   static_assert(kBins == 2 * kSortThreads, "a thread has two digits");
   __shared__ uint32_t place[kSortWaves][kBins];
+  __shared__ unsigned long long masks[kSortWaves][kBins];
   __shared__ uint32_t wave_sum[kSortWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t i0 = (int64_t)blockIdx.x * P.tile, i1 = i0 + P.tile < P.T ? i0 + P.tile : P.T;
   const int part = P.tile / kSortWaves;                     // a multiple of 64
   const int64_t w0 = i0 + (int64_t)wave * part, w1 = w0 + part < i1 ? w0 + part : i1;
-  for (int d = tid; d < kSortWaves * kBins; d += kSortThreads) (&place[0][0])[d] = 0;
+  for (int d = tid; d < kSortWaves * kBins; d += kSortThreads) {
+    (&place[0][0])[d] = 0;
+    (&masks[0][0])[d] = 0;
+  }
   __syncthreads();
   for (int64_t i = w0 + lane; i < w1; i += 64) atomicAdd(&place[wave][(key_at(P, i) >> P.shift) & (kBins - 1)], 1u);
   // digits 2 tid and 2 tid + 1: all tiles' tokens, and those of earlier tiles
@@ -179,27 +200,74 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortParams P) {
     }
   }
   __syncthreads();
-  // each wave takes 64 tokens at a time; lanes with one digit share its place
-  for (int64_t i = w0; i < w1; i += 64) {
-    const bool in = i + lane < w1;
-    const uint32_t key = in ? key_at(P, i + lane) : 0;
-    const uint32_t digit = (key >> P.shift) & (kBins - 1);
-    unsigned long long same = __builtin_amdgcn_ballot_w64(in);
+  // each wave takes 64 tokens at a time, lanes with one digit share its place; kHeld of them loaded ahead
+  constexpr int kHeld = 8;
+  for (int64_t i0w = w0; i0w < w1; i0w += 64 * kHeld) {
+    uint32_t key[kHeld], pos[kHeld];
 #pragma unroll
-    for (int b = 0; b < kBits; ++b) {
-      const unsigned long long ones = __builtin_amdgcn_ballot_w64((digit >> b) & 1);
-      same &= (digit >> b) & 1 ? ones : ~ones;
+    for (int u = 0; u < kHeld; ++u) {
+      const int64_t i = i0w + 64 * u + lane;
+      key[u] = i < w1 ? key_at(P, i) : 0;
+      pos[u] = i < w1 && !P.ids ? P.pos_in[i] : (uint32_t)i;
     }
-    if (in) {
-      const int rank = __builtin_popcountll(same & ((1ull << lane) - 1));
-      const uint32_t at = place[wave][digit] + (uint32_t)rank;
-      P.key_out[at] = key;
-      P.pos_out[at] = P.ids ? (uint32_t)(i + lane) : P.pos_in[i + lane];
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      if (i0w + 64 * u >= w1) continue;
+      const bool in = i0w + 64 * u + lane < w1;
+      const uint32_t digit = (key[u] >> P.shift) & (kBins - 1);
+      const uint32_t first = place[wave][digit];
+      const unsigned long long same = lanes_with(masks[wave], digit, in, lane);
+      if (in) {
+        const uint32_t at = first + (uint32_t)__builtin_popcountll(same & ((1ull << lane) - 1));
+        P.key_out[at] = key[u];
+        P.pos_out[at] = pos[u];
+        // the last lane of each digit moves its place on
+        if ((same >> lane) == 1ull) place[wave][digit] = first + (uint32_t)__builtin_popcountll(same);
+      }
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_wave_barrier();
-    // the last lane of each digit moves its place on
-    if (in && (same >> lane) == 1ull) place[wave][digit] += (uint32_t)__builtin_popcountll(same);
-    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The whole sort in one launch, for up to 2^14 tokens and ids below 2^18: a token is one word, id <<
+// 14 | i, and its place is the number of smaller words. Workgroup = 64 tokens; its 16 waves hold 64 R
+// of all words each, and one compare of a token's word (a scalar) with 64 of them, whose lanes are
+// counted as scalars, is all that a token and 64 others take: bound by the compares, T^2 / 64 of
+// them, on all CUs (16384 tokens 0.27 G pairs). A radix sort in one workgroup took 35 to 45 us for
+// those, bound by LDS, one in four launches 28; the gradient is cleared beside it.
+constexpr int kRankBits = 14, kRankThreads = 1024, kRankWaves = kRankThreads / 64;
+constexpr int64_t kRankTokens = 1 << kRankBits, kRankIds = ((int64_t)1 << (32 - kRankBits)) - 1;
+
+template <int R>
+__global__ __launch_bounds__(kRankThreads) __attribute__((amdgpu_waves_per_eu(8, 8))) void rank_kernel(SortParams P) {
+  if (clears<kRankThreads>(P, P.tiles)) return;
+  __shared__ int count[kRankWaves][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int T = (int)P.T, i = blockIdx.x * 64 + lane;
+  uint32_t x[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int j = (wave * R + r) * 64 + lane;
+    x[r] = j < T ? key_at(P, j) << kRankBits | (uint32_t)j : 0xffffffffu;   // above every token's
+  }
+  const uint32_t mine = i < T ? key_at(P, i) << kRankBits | (uint32_t)i : 0xffffffffu;
+  int n = 0;
+#pragma unroll 2
+  for (int l = 0; l < 64; ++l) {
+    const uint32_t w = (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
+    int c = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[r] < w));
+    n = lane == l ? c : n;
+  }
+  count[wave][lane] = n;
+  __syncthreads();
+  if (wave == 0 && i < T) {
+    int at = 0;
+#pragma unroll
+    for (int g = 0; g < kRankWaves; ++g) at += count[g][lane];
+    P.key_out[at] = mine >> kRankBits;
+    P.pos_out[at] = (uint32_t)i;
   }
 }
 
@@ -210,11 +278,11 @@ struct SumParams {
   void* grad;
   float* part;              // [chunks, 2, cols]: the runs that a chunk's first and last token belong to
   int64_t dy_st, T, V;
-  int cols, chunks;
+  int cols, chunks, run;
   float scale;
 };
 
-// Wave = (chunk of kRun sorted tokens, 512 columns). Runs that lie inside the chunk are written; a
+// Wave = (chunk of `run` sorted tokens, 512 columns). Runs that lie inside the chunk are written; a
 // run that goes on in a neighbour leaves its sum in `part` (slot 0: the run the chunk begins with,
 // if it began earlier; slot 1: the run that goes on behind it, if it began here).
 template <class TY, class TG>
@@ -225,12 +293,12 @@ __global__ __launch_bounds__(256) void sum_kernel(SumParams P) {
   if (chunk >= P.chunks) return;
   const int c = (int)(w - (int64_t)chunk * cblk) * 512 + lane * 8;
   const bool on = c < P.cols;
-  const int64_t t0 = (int64_t)chunk * kRun;
-  const int n = (int)(P.T - t0 < kRun ? P.T - t0 : kRun);
+  const int64_t t0 = (int64_t)chunk * P.run;
+  const int n = (int)(P.T - t0 < P.run ? P.T - t0 : P.run);
   const uint32_t key = lane < n ? P.key[t0 + lane] : (uint32_t)P.V;
   const uint32_t pos = lane < n ? P.pos[t0 + lane] : 0;
   const uint32_t prev = t0 > 0 ? P.key[t0 - 1] : 0xffffffffu;
-  const uint32_t next = t0 + kRun < P.T ? P.key[t0 + kRun] : 0xffffffffu;
+  const uint32_t next = t0 + P.run < P.T ? P.key[t0 + P.run] : 0xffffffffu;
   float acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
@@ -283,24 +351,38 @@ __global__ __launch_bounds__(256) void join_kernel(SumParams P) {
   const int chunk = (int)(w / cblk);
   if (chunk >= P.chunks - 1) return;
   const int c = (int)(w - (int64_t)chunk * cblk) * 512 + lane * 8;
-  const int64_t t1 = (int64_t)(chunk + 1) * kRun;   // the next chunk's first token
+  const int64_t t1 = (int64_t)(chunk + 1) * P.run;   // the next chunk's first token
   const uint32_t k = P.key[t1 - 1];
   if (k >= (uint32_t)P.V || P.key[t1] != k) return;
-  if (chunk > 0 && P.key[t1 - kRun] == k && P.key[t1 - kRun - 1] == k) return;   // it began earlier
-  if (c >= P.cols) return;
-  // the chunks after this one that it reaches
+  if (chunk > 0 && P.key[t1 - P.run] == k && P.key[t1 - P.run - 1] == k) return;   // it began earlier
+  // the chunks after this one that it reaches: those whose first token is k's
   int end = chunk + 2;
-  while (end < P.chunks && P.key[(int64_t)end * kRun] == k && P.key[(int64_t)end * kRun - 1] == k) ++end;
+  for (;;) {
+    const bool more = end + lane < P.chunks && P.key[(int64_t)(end + lane) * P.run] == k;
+    const unsigned long long not_k = ~__builtin_amdgcn_ballot_w64(more);
+    if (not_k) {
+      end += (int)__builtin_ctzll(not_k);
+      break;
+    }
+    end += 64;
+  }
+  if (c >= P.cols) return;
   float acc[8];
   Row8<float> r;
   r.load(P.part + ((int64_t)chunk * 2 + 1) * P.cols + c);
   r.get(acc);
-  for (int g = chunk + 1; g < end; ++g) {
-    float f[8];
-    r.load(P.part + (int64_t)g * 2 * P.cols + c);
-    r.get(f);
+  constexpr int kAhead = 8;
+  for (int g = chunk + 1; g < end; g += kAhead) {
+    Row8<float> ahead[kAhead];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += f[e];
+    for (int u = 0; u < kAhead; ++u) ahead[u].load(P.part + (int64_t)(g + u < end ? g + u : end - 1) * 2 * P.cols + c);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      float f[8];
+      ahead[u].get(f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = g + u < end ? acc[e] + f[e] : acc[e];
+    }
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] *= P.scale;
