@@ -1663,17 +1663,28 @@ int prefixlm_embedding_bwd(const prefixlm_embedding_args* a, void* stream_) {
 }  // extern "C"
 
 // ---- attention over an 8-bit cache -----------------------------------------------------------
-// Splits of the keys; those of several queries as for bf16 (the tiles and their chain are the same).
+// Splits of the keys. Several queries: as for bf16 (the tiles and their chain are the same). One query:
+// one split for caches of up to 1536 rows, whose keys take less time than the combine's launch (16
+// pairs x 920 of 1536 rows 8.7 us, 11.3 with three splits; 128 x 800 of 1024 9.9 and 12.8; 64 x 1800
+// of 2048 14.8, 13.2 with four), and from 192 pairs on, one for each CU nearly (256 x 12288 of 16384
+// ragged rows 128.7, 131.3 with twelve; 256 x 1500 of 2048 19.8 and 22.7). Else 768 workgroups (48
+// pairs x 23000 of 32768 rows 51.3 with 16 splits, 54.8 with eight; 80 x 4096 20.1 with twelve, 24.2
+// with two), of at least two blocks each.
 static int64_t kv8_nsplit(int64_t B, int S, int64_t H, int64_t Smax) {
   if (S > 1) return kv_nsplit(B, S, H, Smax);
-  const int64_t units = B * H, most = std::min<int64_t>(kvc::kMaxSplits, (Smax + 127) / 128);
-  return std::max<int64_t>(1, std::min((1024 + units - 1) / units, most));
+  const int64_t units = B * H;
+  if (Smax <= 1536 || units >= 192) return 1;
+  return std::min({(768 + units - 1) / units, Smax / (2 * kv8::kBlock), (int64_t)kvc::kMaxSplits});
 }
 
 template <class C>
 static void kv8_launch(const kv8::Params& P, int64_t nblk, hipStream_t stream) {
   const dim3 g((unsigned)nblk), n(kvc::NT);
-  if (P.S == 1)
+  // one split: eight waves (16 pairs x 920 rows 10.4 -> 8.7 us, 128 x 800 11.8 -> 9.9, 2048 x 800 70.4
+  // -> 67.7), unless many pairs have short caches (1024 x 200 of 256 rows 15.9, with four 12.7)
+  if (P.S == 1 && P.nsplit == 1 && !((int64_t)P.B * P.H > 512 && P.Smax <= 512))
+    hipLaunchKernelGGL((kv8::decode_kernel<C, 512>), g, dim3(512), 0, stream, P);
+  else if (P.S == 1)
     hipLaunchKernelGGL((kv8::decode_kernel<C, kvc::NT>), g, n, 0, stream, P);
   else if (ext_qw(P.S) == 1)
     hipLaunchKernelGGL((kv8::extend_kernel<C, 1>), g, n, kvc::ExtGeo<1>::LDS_BYTES, stream, P);
