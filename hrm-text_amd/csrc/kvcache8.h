@@ -19,7 +19,8 @@
 //             and the new one, puts that one into the ring and rounds a block it completes;
 //   extend  : several queries per row, on the matrix cores: codes become bf16 on their way into
 //             LDS, exactly; the scales go to the scores and, for V, to the probabilities;
-//   append  : new rows of an extend or prefill into ring, codes and scales, behind the attention.
+//   append  : new rows of an extend or prefill into ring, codes and scales: beside the attention of up
+//             to 64 rows, behind that of more.
 // The splits' partials and their combine are kvcache.h's.
 #pragma once
 #include "common.h"
@@ -55,6 +56,7 @@ struct Params {
   int B, S, H, Smax, nsplit, causal, seqlen_const;
   int s_new;              // rows appended by this call: S, or 0 without new k, v
   int nqb;                // extend: query blocks of 32 QW rows
+  int n_main, touched;    // extend: workgroups from n_main on append, `touched` blocks per (b, h)
   float scale_log2;
 };
 
@@ -163,36 +165,31 @@ __device__ __forceinline__ void round_block(uint8_t* codes, float* scale, int bl
   }
 }
 
-// Workgroup = (b, h, touched block, first one of the touched blocks first): rounds its block if it
-// is complete now; the first one then also puts the last rows into the ring, after it has read the
-// ring's old rows.
+// Workgroup `wg` = (b, h, touched block, keys or values): rounds its block if it is complete now; the
+// first touched block's also puts the last rows into the ring, after it has read the ring's old rows.
 template <class C>
-__global__ __launch_bounds__(NT) void append_kernel(Params P, int nblk) {
-  __shared__ uint32_t s_mag[NT / 64];
-  const int bh = blockIdx.x / nblk, i = blockIdx.x - bh * nblk;
+__device__ __forceinline__ void append(const Params& P, int wg, int nblk, uint32_t* s_mag) {
+  const int n = wg & 1, bh = (wg >> 1) / nblk, i = (wg >> 1) - bh * nblk;
   const int b = bh / P.H, h = bh - b * P.H;
   const int len = cache_len(P, b), end = min(P.Smax, len + P.s_new);
   const int blk = len / kBlock + i;
-  bf16* const ring[2] = {P.kr + (int64_t)bh * kRing * D, P.vr + (int64_t)bh * kRing * D};
-  const bf16* const fresh[2] = {P.k + b * P.k_sb + h * P.k_sh, P.v + b * P.v_sb + h * P.v_sh};
-  const int64_t st[2] = {P.k_ss, P.v_ss};
-  if (blk < end / kBlock) {
-#pragma unroll 1
-    for (int n = 0; n < 2; ++n) {
-      const bf16 *const old = ring[n], *const now = fresh[n];
-      const int64_t ss = st[n];
-      round_block<C, NT>((n ? P.vc : P.kc) + (int64_t)bh * P.Smax * D, (n ? P.vs : P.ks) + (int64_t)bh * (P.Smax / kBlock),
-                         blk, s_mag, [&](int j) { return j < len ? old + (j & (kRing - 1)) * D : now + (j - len) * ss; });
-    }
-  }
+  bf16* const ring = (n ? P.vr : P.kr) + (int64_t)bh * kRing * D;
+  const bf16* const fresh = n ? P.v + b * P.v_sb + h * P.v_sh : P.k + b * P.k_sb + h * P.k_sh;
+  const int64_t st = n ? P.v_ss : P.k_ss;
+  if (blk < end / kBlock)
+    round_block<C, NT>((n ? P.vc : P.kc) + (int64_t)bh * P.Smax * D, (n ? P.vs : P.ks) + (int64_t)bh * (P.Smax / kBlock),
+                       blk, s_mag, [&](int j) { return j < len ? ring + (j & (kRing - 1)) * D : fresh + (j - len) * st; });
   if (i) return;
   __syncthreads();   // every thread has read the ring
   const int j0 = max(len, end / kBlock * kBlock - kBlock), c = 8 * (threadIdx.x & 15);
   for (int j = j0 + (threadIdx.x >> 4); j < end; j += NT / 16)
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-      *reinterpret_cast<u32x4*>(ring[n] + (j & (kRing - 1)) * D + c) =
-          *reinterpret_cast<const u32x4*>(fresh[n] + (j - len) * st[n] + c);
+    *reinterpret_cast<u32x4*>(ring + (j & (kRing - 1)) * D + c) =
+        *reinterpret_cast<const u32x4*>(fresh + (j - len) * st + c);
+}
+template <class C>
+__global__ __launch_bounds__(NT) void append_kernel(Params P, int nblk) {
+  __shared__ uint32_t s_mag[NT / 64];
+  append<C>(P, blockIdx.x, nblk, s_mag);
 }
 
 // ---- one query per row ------------------------------------------------------------------------
@@ -445,7 +442,14 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
   constexpr int KW = G::KW, TK = G::TK, TILE = G::TILE, NS = D / 16, NP = TK / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int bad;   // some value, scale or score is not finite, or a score could not be formed
-
+  __shared__ uint32_t s_mag[NT / 64];
+  // Up to 64 new rows go into the cache beside the attention, which reads none of what this writes: the
+  // blocks they complete begin at or behind the first one it takes in bf16, and the ring rows that
+  // it reads, from that block's first on, are less than 128 before the last new one.
+  if ((int)blockIdx.x >= P.n_main) {
+    append<C>(P, (int)blockIdx.x - P.n_main, P.touched, s_mag);
+    return;
+  }
   // unit u = (b, h, split); its query blocks sit 8 grid indices apart, on one XCD
   const int qb = (blockIdx.x >> 3) % P.nqb;
   const int u = (int)((blockIdx.x >> 3) / P.nqb) * 8 + (blockIdx.x & 7);

@@ -1778,6 +1778,7 @@ int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* a, void* stream_) {
   P.seqlen_const = a->cache_seqlen;
   P.s_new = has_new ? S : 0;
   P.scale_log2 = a->softmax_scale * kLog2e;
+  P.touched = (S + kv8::kBlock - 1) / kv8::kBlock;
   // the same queries, rows, lengths and partials, for the kernels shared with the bf16 cache
   kvc::Params Q{};
   Q.q = P.q; Q.k = P.k; Q.v = P.v; Q.out = P.out; Q.part = P.part; Q.seqlens = P.seqlens;
@@ -1789,12 +1790,15 @@ int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* a, void* stream_) {
   Q.causal = P.causal; Q.seqlen_const = P.seqlen_const; Q.s_new = P.s_new; Q.scale_log2 = P.scale_log2;
 
   const int64_t units = (int64_t)B * H * P.nsplit, nblk = S == 1 ? units : (units + 7) / 8 * 8 * P.nqb;
-  const int64_t touched = std::max<int64_t>(1, ((int64_t)S + kv8::kBlock - 1) / kv8::kBlock);
+  const int64_t nappend = has_new ? 2 * (int64_t)B * H * P.touched : 0;
+  // with rows of one block at most the attention's launch appends (see the kernel)
+  const bool prefill = kv_prefills(Q), beside = S > 1 && S <= kv8::kBlock && !prefill;
+  P.n_main = (int)std::min<int64_t>(nblk, 0x7fffffff);
   const int64_t waves = (int64_t)B * S * H;
-  if (nblk > 0x7fffffff || (int64_t)B * H * touched > 0x7fffffff || (waves * 64 + 255) / 256 > 0x7fffffff)
+  if (nblk + nappend > 0x7fffffff || (waves * 64 + 255) / 256 > 0x7fffffff)
     return fail(PREFIXLM_ERR_INVALID, "grid too large");
   (void)hipGetLastError();
-  if (kv_prefills(Q)) {
+  if (prefill) {
     set_kernel_attrs();
     if (g_attr_err != hipSuccess)
       return fail(PREFIXLM_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(g_attr_err));
@@ -1804,15 +1808,15 @@ int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* a, void* stream_) {
     const int rc = kv8_allow_lds();
     if (rc) return rc;
     if (a->code_int8)
-      kv8_launch<kv8::Int8>(P, nblk, stream);
+      kv8_launch<kv8::Int8>(P, nblk + (beside ? nappend : 0), stream);
     else
-      kv8_launch<kv8::E4M3>(P, nblk, stream);
+      kv8_launch<kv8::E4M3>(P, nblk + (beside ? nappend : 0), stream);
     if (P.nsplit > 1)
       hipLaunchKernelGGL(kvc::combine_kernel<true>, dim3((unsigned)((waves * 64 + 255) / 256)), dim3(256), 0, stream, Q);
   }
-  if (has_new && (S > 1 || kv_prefills(Q)))
+  if (has_new && !beside && (S > 1 || prefill))
     hipLaunchKernelGGL(a->code_int8 ? kv8::append_kernel<kv8::Int8> : kv8::append_kernel<kv8::E4M3>,
-                       dim3((unsigned)(B * H * touched)), dim3(kvc::NT), 0, stream, P, (int)touched);
+                       dim3((unsigned)nappend), dim3(kvc::NT), 0, stream, P, P.touched);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "8-bit kv-cache launch: %s", hipGetErrorString(e));
   return PREFIXLM_OK;

@@ -119,7 +119,8 @@ def _args(**kw):
     (dict(cache_seqlen=-1), "cache_seqlen"), (dict(cache_seqlen=1025), "cache_seqlen"), (dict(q=0), "null"),
     (dict(k_codes=(1 << 20) + 8), "aligned"), (dict(k_scale=(1 << 20) + 2), "aligned"), (dict(v_recent=0), "null"),
     (dict(k=(1 << 20) + 2), "aligned"), (dict(q_stride_h=4), "stride"), (dict(v_stride_s=-8), "stride"),
-    (dict(workspace_bytes=8), "workspace"), (dict(workspace=0), "workspace"), (dict(seqlen_q=0x7fffffff), "too large"),
+    (dict(workspace_bytes=8, max_seqlen_cache=4096), "workspace"),
+    (dict(workspace=0, max_seqlen_cache=4096), "workspace"), (dict(seqlen_q=0x7fffffff), "too large"),
 ])
 def test_entry_point_rejects(lib, kw, needle):
     assert lib.prefixlm_kvcache8_fwd(ctypes.byref(_args(**kw)), None) == 1
