@@ -120,6 +120,26 @@ __device__ __forceinline__ float block_scale(uint32_t mag) {
   return s < 0x1p-126f ? 0x1p-126f : s;   // NaN stays
 }
 
+// x / s for many x, correctly rounded, with a few operations each where the compiler's division takes
+// a dozen (the rounding of 2 x 16 x 1021 rows 11.2 -> 9.4 us): y = 1 / s rounded
+// (one Newton step from the 1-ulp reciprocal), q = x y, and q + (x - q s) y rounds to x / s as long as
+// the residual x - q s is exact, which a scale below 2^-60 is multiplied up for. Scales and rows come
+// from bf16, so there are 128 mantissas of each: the tests take them all.
+struct Divisor {
+  float s, y, up;
+  __device__ __forceinline__ explicit Divisor(float scale) {
+    up = scale < 0x1p-60f ? 0x1p64f : 1.f;
+    s = scale * up;
+    const float y0 = __builtin_amdgcn_rcpf(s);
+    y = __builtin_fmaf(__builtin_fmaf(-s, y0, 1.f), y0, y0);
+  }
+  __device__ __forceinline__ float divides(float x) const {
+    x *= up;
+    const float q = x * y;
+    return __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-q, s, x), y, q), x);   // -0 stays
+  }
+};
+
 // ---- taking rows into the cache ------------------------------------------------------------
 // The workgroup rounds the complete block `blk` of (b, h), whose row j is row(j) (256 bytes of
 // bf16), into 8 bits: threads of 16 columns, NTH / 8 rows at a time.
@@ -147,6 +167,7 @@ __device__ __forceinline__ void round_block(uint8_t* codes, float* scale, int bl
   for (int g2 = 1; g2 < NTH / 64; ++g2) mag = max(mag, s_mag[g2]);
   const float s = block_scale<C>(mag);
   if (tid == 0) scale[blk] = s;
+  const Divisor by(s);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     u32x4 w;
@@ -156,8 +177,8 @@ __device__ __forceinline__ void round_block(uint8_t* codes, float* scale, int bl
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint32_t y = x[r][i >> 1][2 * (i & 1) + e];
-        f[2 * e] = bf16lo(y) / s;
-        f[2 * e + 1] = bf16hi(y) / s;
+        f[2 * e] = by.divides(bf16lo(y));
+        f[2 * e + 1] = by.divides(bf16hi(y));
       }
       w[i] = C::put(f);
     }

@@ -250,6 +250,32 @@ def test_extreme_rows(S, dtype):
     assert big > 1e38
 
 
+@pytest.mark.parametrize("dtype", CODES)
+@pytest.mark.parametrize("exponent", [0, 127, 90, -50, -59, -60, -61, -80, -105, -126])
+def test_every_mantissa_is_rounded_as_by_division(exponent, dtype):
+    """Blocks with each of the 128 mantissas of their largest magnitude (and so of their scale) and rows
+    of all mantissas, signs and 24 binades below it: codes equal those of the division."""
+    m = torch.arange(128, dtype=torch.int32)
+    sign = torch.tensor([0, 1], dtype=torch.int32)
+    e = torch.arange(1, 25, dtype=torch.int32)
+    biased = (exponent + 127 - e).clamp_min(0)
+    bits = (sign[:, None, None] << 15) | (biased[None, :, None] << 7) | m[None, None, :]       # 2 * 24 * 128
+    rows = torch.zeros(128, 64, 128, dtype=torch.int32)
+    rows[:, :48] = bits.reshape(48, 128)
+    rows[:, 63, 0] = (max(exponent + 127, 0) << 7) | m
+    rows = rows.to(torch.int16).view(torch.bfloat16)                                            # [block, 64, 128]
+    B = 8
+    k = rows.reshape(B, 16 * 64, 1, 128)
+    dev = kvcache_q8(B, 16 * 64, 1, dtype=dtype)
+    flash_attn_with_kvcache_q8(k.to(DEV), dev, k.to(DEV), k.flip(0).to(DEV), 0)
+    for codes, scale, x in ((dev.k_codes, dev.k_scale, k), (dev.v_codes, dev.v_scale, k.flip(0))):
+        for b in range(B):
+            for blk in range(16):
+                c, s = oracle.round_block(x[b, blk * 64:blk * 64 + 64, 0], dtype)
+                assert scale[b, 0, blk].item() == s.item()
+                assert torch.equal(_bits(codes[b, 0, blk * 64:blk * 64 + 64].cpu()), _bits(c)), (b, blk)
+
+
 def test_strided_rows():
     """q, k and v as the slices of one projection, and the keys of one token for every row."""
     B, S, H, n = 2, 3, 4, 100
