@@ -188,7 +188,7 @@ __device__ __forceinline__ void round_block(uint8_t* codes, float* scale, int bl
 
 // Workgroup `wg` = (b, h, touched block, keys or values): rounds its block if it is complete now; the
 // first touched block's also puts the last rows into the ring, after it has read the ring's old rows.
-template <class C>
+template <class C, int NTH = NT>
 __device__ __forceinline__ void append(const Params& P, int wg, int nblk, uint32_t* s_mag) {
   const int n = wg & 1, bh = (wg >> 1) / nblk, i = (wg >> 1) - bh * nblk;
   const int b = bh / P.H, h = bh - b * P.H;
@@ -198,19 +198,23 @@ __device__ __forceinline__ void append(const Params& P, int wg, int nblk, uint32
   const bf16* const fresh = n ? P.v + b * P.v_sb + h * P.v_sh : P.k + b * P.k_sb + h * P.k_sh;
   const int64_t st = n ? P.v_ss : P.k_ss;
   if (blk < end / kBlock)
-    round_block<C, NT>((n ? P.vc : P.kc) + (int64_t)bh * P.Smax * D, (n ? P.vs : P.ks) + (int64_t)bh * (P.Smax / kBlock),
-                       blk, s_mag, [&](int j) { return j < len ? ring + (j & (kRing - 1)) * D : fresh + (j - len) * st; });
+    round_block<C, NTH>((n ? P.vc : P.kc) + (int64_t)bh * P.Smax * D, (n ? P.vs : P.ks) + (int64_t)bh * (P.Smax / kBlock),
+                        blk, s_mag, [&](int j) { return j < len ? ring + (j & (kRing - 1)) * D : fresh + (j - len) * st; });
   if (i) return;
   __syncthreads();   // every thread has read the ring
   const int j0 = max(len, end / kBlock * kBlock - kBlock), c = 8 * (threadIdx.x & 15);
-  for (int j = j0 + (threadIdx.x >> 4); j < end; j += NT / 16)
+  for (int j = j0 + (threadIdx.x >> 4); j < end; j += NTH / 16)
     *reinterpret_cast<u32x4*>(ring + (j & (kRing - 1)) * D + c) =
         *reinterpret_cast<const u32x4*>(fresh + (j - len) * st + c);
 }
+// A thread has 16 columns of one row: bound by its chain of loads, maximum, barrier and stores (2 x 16
+// heads x 1021 rows, 25 MB: 8.9 us, 9.8 with two rows a thread, 12.2 with four; as workgroups of the
+// prefill's launch, whose LDS and registers let few of them run at once, 3 us more than so).
+constexpr int kAppendThreads = 512;
 template <class C>
-__global__ __launch_bounds__(NT) void append_kernel(Params P, int nblk) {
-  __shared__ uint32_t s_mag[NT / 64];
-  append<C>(P, blockIdx.x, nblk, s_mag);
+__global__ __launch_bounds__(kAppendThreads) void append_kernel(Params P, int nblk) {
+  __shared__ uint32_t s_mag[kAppendThreads / 64];
+  append<C, kAppendThreads>(P, blockIdx.x, nblk, s_mag);
 }
 
 // ---- one query per row ------------------------------------------------------------------------
@@ -457,6 +461,13 @@ __device__ __forceinline__ void extend_block_valu(const Params& P, int b, int h,
 // Workgroup = (b, h, 32 QW queries, split of the keys), waves and tiles as in kvcache.h. A strip of
 // 16 staged rows is either codes or bf16 rows, and the 32 keys that a wave multiplies at a time
 // have one scale, as blocks begin at multiples of 64.
+//
+// The probabilities go into P V as two bf16 terms, 16 of their 24 bits: what that leaves, 2^-17 of
+// the sum of p |v|, is 2^-8 of what the output's rounding to bf16 does and less than the rows' own
+// rounding to 8 bits (three terms: 26.6 us for 4 x 16 heads x 45 queries on 2000 rows, two 25.8).
+// Bound by each wave's chain, 2.6 us a tile of 64 keys and 64 queries: half the cache's bytes, the
+// next tile but one on its way as well, change nothing.
+constexpr int kTerms = 2;
 template <class C, int QW>
 __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
   using G = ExtGeo<QW>;
@@ -626,11 +637,11 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
         u32x4 xt[8];
         xt[0] = lds_read_xt(vt, 0, 0);
         xt[1] = lds_read_xt(vt, 0, 1);
-        // 16 keys at a time: P's three terms (n = 0 first), times V
+        // 16 keys at a time: P's terms (n = 0 first), times V
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           float e[8], ps = 0.f;
-          bf16x8 pt[3];
+          bf16x8 pt[kTerms];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             e[i] = __builtin_amdgcn_exp2f(sacc[8 * half + i] - m_use);
@@ -640,7 +651,7 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) e[i] *= unit_v;
 #pragma unroll
-          for (int n = 0; n < 3; ++n) {
+          for (int n = 0; n < kTerms; ++n) {
             u32x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -656,7 +667,7 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
             const int x = 4 * half + dt;
             if (x + 2 < 8) xt[x + 2] = lds_read_xt(vt, (x + 2) / 4, (x + 2) % 4);
 #pragma unroll
-            for (int n = 0; n < 3; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[x]), pt[n], oacc[dt]);
+            for (int n = 0; n < kTerms; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[x]), pt[n], oacc[dt]);
           }
         }
       }

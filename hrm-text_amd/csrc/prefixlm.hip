@@ -1816,7 +1816,7 @@ int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* a, void* stream_) {
   }
   if (has_new && !beside && (S > 1 || prefill))
     hipLaunchKernelGGL(a->code_int8 ? kv8::append_kernel<kv8::Int8> : kv8::append_kernel<kv8::E4M3>,
-                       dim3((unsigned)nappend), dim3(kvc::NT), 0, stream, P, P.touched);
+                       dim3((unsigned)nappend), dim3(kv8::kAppendThreads), 0, stream, P, P.touched);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "8-bit kv-cache launch: %s", hipGetErrorString(e));
   return PREFIXLM_OK;
