@@ -20,6 +20,11 @@ end to end inside the H/L cycles (benchmark config 5):
   gradients (H calls first, at least one L call; :75-89); the earlier calls run
   under ``torch.set_grad_enabled(False)``. The reference's default is 2.
 
+With ``vocab_size`` the stack also has the model's token ends (models/lm_head.py:34-52): a scaled
+embedding in front and a projection to the vocabulary behind, and ``score`` runs tokens to log
+probabilities; with ``fused_elementwise`` through ``prefixlm.embedding`` and
+``prefixlm.token_logprobs``.
+
 The attention callable is injected, so the same weights run with the HIP op
 (bf16) or with a float32 reference attention in tests. Wrapped in ``FusedLayer``
 the callable instead receives the projection output [T, 4H, D] and cos/sin and
@@ -71,6 +76,10 @@ class HRMStackConfig:
     # library GEMM after the norm kernel: at 2048 -> 8192 columns that pair is faster
     # than the fused GEMM (rms_norm_linear stays available on its own).
     fused_gemm: bool = False
+    # rows of the embedding and of the head; 0: the stack runs on hidden states only
+    vocab_size: int = 0
+    # what embedded tokens are multiplied by; None: sqrt(hidden_size)
+    embed_scale: Optional[float] = None
 
     @property
     def head_dim(self) -> int:
@@ -262,6 +271,9 @@ class HRMStack(nn.Module):
         self.L = _Module(cfg)
         # bf16 whatever the stack's dtype, as in the reference (a buffer, not trained)
         self.register_buffer("zL_init", torch.zeros(cfg.hidden_size, dtype=torch.bfloat16))
+        if cfg.vocab_size:
+            self.embed = nn.Parameter(torch.empty(cfg.vocab_size, cfg.hidden_size))
+            self.head = nn.Parameter(torch.empty(cfg.vocab_size, cfg.hidden_size))
 
     @torch.no_grad()
     def init_weights(self, seed: int):
@@ -299,6 +311,32 @@ class HRMStack(nn.Module):
             with torch.set_grad_enabled(grad_on and i in h_grad):
                 z_H = self.H(z_H, z_L, cos, sin, attn, seq_info)
         return z_H
+
+
+    def embed_tokens(self, ids: Tensor) -> Tensor:
+        """scale * embed[ids], in the head's dtype (the embedding may be kept in float32)."""
+        cfg = self.cfg
+        scale = math.sqrt(cfg.hidden_size) if cfg.embed_scale is None else cfg.embed_scale
+        if cfg.fused_elementwise:
+            from .embedding import embedding
+            return embedding(ids, self.embed, scale, dtype=self.head.dtype)
+        return (F.embedding(ids, self.embed) * scale).to(self.head.dtype)
+
+    def score(self, ids: Tensor, targets: Tensor, position_ids: Tensor, attn: AttnFn, seq_info: dict,
+              bp_steps: Optional[int] = 2, entropy: bool = False, top_k: int = 0, ignore_index: int = -100):
+        """``TokenLogprobs`` of the targets given the packed tokens (``prefixlm.token_logprobs``). The
+        embedding enters the first module call: it has a gradient where the window reaches that one
+        (``bp_steps=None``)."""
+        from .logprob import TokenLogprobs, token_logprobs
+        logits = F.linear(self(self.embed_tokens(ids), position_ids, attn, seq_info, bp_steps), self.head)
+        if self.cfg.fused_elementwise:
+            return token_logprobs(logits, targets, entropy=entropy, top_k=top_k, ignore_index=ignore_index)
+        logp = torch.log_softmax(logits.float(), -1)
+        counted = targets != ignore_index
+        lp = torch.where(counted, logp.gather(-1, torch.where(counted, targets, 0)[..., None])[..., 0], 0.0)
+        ent = -(logp.exp() * logp).sum(-1) if entropy else None
+        top = torch.sort(logp, dim=-1, descending=True, stable=True) if top_k else None
+        return TokenLogprobs(lp, ent, top.values[..., :top_k] if top_k else None, top.indices[..., :top_k] if top_k else None)
 
 
 def packed_position_ids(prefix, causal, T: int, device) -> Tensor:

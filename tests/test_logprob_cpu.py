@@ -100,7 +100,7 @@ def _args(**kw):
     (dict(vocab=0), "vocab"), (dict(rows=-1), "rows"), (dict(x=0), "x is null"), (dict(x=(1 << 20) + 1), "x is null"),
     (dict(x=(1 << 20) + 2, x_fp32=1), "aligned"), (dict(x_stride=-1), "x_stride"), (dict(stats=0), "stats"),
     (dict(targets=0), "targets"), (dict(logprob=0), "logprob"), (dict(top_k=65), "top_k"),
-    (dict(top_k=-1), "top_k"), (dict(top_k=3), "top_logprobs"), (dict(rows=4, vocab=50000), "workspace"),
+    (dict(top_k=-1), "top_k"), (dict(top_k=3), "top_logprobs"), (dict(rows=4, vocab=200000), "workspace"),
 ])
 def test_forward_entry_point_rejects(lib, kw, needle):
     assert lib.prefixlm_logprob_fwd(ctypes.byref(_args(**kw)), None) == 1
