@@ -1368,6 +1368,9 @@ int prefixlm_timer_read(void* timer, float* total_ms, int32_t* launches) {
 
 }  // extern "C"
 
+// A launch has fewer than 2^32 threads
+static bool launchable(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll / threads && blocks <= 0x7fffffff; }
+
 // ---- log probabilities ---------------------------------------------------------------
 // Splits of a row, where the rows alone are fewer than the CUs and long enough to pay for the second
 // launch: 512 workgroups, of at least 8192 logits each. One split against several: 8 rows of 65536 logits
@@ -1442,7 +1445,7 @@ static int lp_call(const prefixlm_logprob_args* a, void* stream_, bool backward)
     P.g = a->dlogprob;
     P.h = a->dentropy;
     const int64_t nblk = (a->vocab + 8 * 256 * lp::kUnroll - 1) / (8 * 256 * lp::kUnroll);
-    if (a->rows * nblk > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many elements");
+    if (a->rows > 0x7fffffff || !launchable(a->rows * nblk, 256)) return fail(PREFIXLM_ERR_INVALID, "too many elements");
     (void)hipGetLastError();
     const bool nt = 2 * a->rows * a->vocab * (int64_t)size > lp::kNtBytes;
     if (a->x_fp32)
@@ -1466,7 +1469,7 @@ static int lp_call(const prefixlm_logprob_args* a, void* stream_, bool backward)
       P.part_top = reinterpret_cast<unsigned long long*>(static_cast<char*>(a->workspace) +
                                                          align_up((size_t)a->rows * P.nsplit * 16));
     }
-    if (a->rows * P.nsplit > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many rows");
+    if (a->rows > 0x7fffffff || !launchable(a->rows * P.nsplit, lp::NT)) return fail(PREFIXLM_ERR_INVALID, "too many rows");
     (void)hipGetLastError();
     if (a->x_fp32)
       lp_fwd_launch<float>(P, stream);
@@ -1554,7 +1557,7 @@ int prefixlm_embedding_fwd(const prefixlm_embedding_args* a, void* stream_) {
   if (!rc) rc = emb_rows(a->y, a->y_stride, a->y_fp32, a->cols, false, "y");
   if (rc) return rc;
   const int64_t nblk = (a->tokens * (a->cols / 8) + 255) / 256;
-  if (nblk > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many elements");
+  if (!launchable(nblk, 256)) return fail(PREFIXLM_ERR_INVALID, "too many elements");
   const emb::FwdParams P{a->table, a->ids, a->y, a->table_stride, a->y_stride, a->tokens, a->vocab, a->cols,
                          !a->ids_int32, a->scale};
   (void)hipGetLastError();
@@ -1583,7 +1586,7 @@ int prefixlm_embedding_bwd(const prefixlm_embedding_args* a, void* stream_) {
   passes = T ? (bits + emb::kBits - 1) / emb::kBits : 0;
   const int run = emb_run(T, a->cols);
   const int64_t waves = (T + run - 1) / run * ((a->cols + 511) / 512);
-  if (waves > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "too many elements");
+  if (!launchable((waves + 3) / 4, 256)) return fail(PREFIXLM_ERR_INVALID, "too many elements");
   const EmbWorkspace w = emb_workspace(T, a->cols);
   char* ws = static_cast<char*>(a->workspace);
   emb::SortParams P{};
@@ -1795,7 +1798,7 @@ int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* a, void* stream_) {
   const bool prefill = kv_prefills(Q), beside = S > 1 && S <= kv8::kBlock && !prefill;
   P.n_main = (int)std::min<int64_t>(nblk, 0x7fffffff);
   const int64_t waves = (int64_t)B * S * H;
-  if (nblk + nappend > 0x7fffffff || (waves * 64 + 255) / 256 > 0x7fffffff)
+  if (!launchable(nblk + nappend, 512) || !launchable((waves + 3) / 4, 256))
     return fail(PREFIXLM_ERR_INVALID, "grid too large");
   (void)hipGetLastError();
   if (prefill) {

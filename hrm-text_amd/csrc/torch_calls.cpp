@@ -1021,6 +1021,13 @@ PyObject* py_kvcache_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const char *x = static_cast<const char*>(c[i].const_data_ptr()), *y = static_cast<const char*>(c[j].const_data_ptr());
       if (x < y + c[j].nbytes() && y < x + c[i].nbytes()) return none();
     }
+    for (const Tensor* t : {&q, &k, &v}) {   // read while the cache is written
+      if (!t->defined()) continue;
+      int64_t n = 1;
+      for (int d = 0; d < 4; ++d) n += (t->size(d) - 1) * t->stride(d);
+      const char *x = static_cast<const char*>(c[i].const_data_ptr()), *y = static_cast<const char*>(t->const_data_ptr());
+      if (x < y + 2 * n && y < x + c[i].nbytes()) return none();
+    }
   }
   if (PyLong_CheckExact(a[9])) {
     Scalar s;

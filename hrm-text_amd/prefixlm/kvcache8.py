@@ -60,8 +60,14 @@ def kvcache_q8(batch: int, max_seqlen: int, num_heads: int, head_dim: int = 128,
         *(torch.zeros((*lead, RECENT, head_dim), dtype=torch.bfloat16, device=device) for _ in range(2)))
 
 
-def _check_cache(c, B: int, H: int, D: int, dev) -> int:
-    """Smax of a cache that fits q."""
+def _span(x: Tensor):
+    """The addresses that x's elements lie in."""
+    n = sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1
+    return x.data_ptr(), x.data_ptr() + n * x.element_size()
+
+
+def _check_cache(c, B: int, H: int, D: int, dev, others) -> int:
+    """Smax of a cache that fits q and shares no memory with it and the new rows."""
     codes = c[0]
     if codes.dtype not in _CODES or codes.dim() != 4:
         raise ValueError(f"k_codes must be float8_e4m3fn or int8 [B, H, Smax, 128] (got {codes.dtype} {tuple(codes.shape)})")
@@ -76,10 +82,13 @@ def _check_cache(c, B: int, H: int, D: int, dev) -> int:
             raise ValueError(f"{name} must be {dtype} {shape} on {dev} (got {x.dtype} {tuple(x.shape)} on {x.device})")
         if not x.is_contiguous() or x.data_ptr() % (4 if dtype == torch.float32 else 16):
             raise ValueError(f"{name} must be contiguous and 16-byte aligned (got strides {x.stride()})")
-        at.append((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()))
+        at.append(_span(x))
     at.sort()
     if any(a[1] > b[0] for a, b in zip(at, at[1:])):
         raise ValueError("the cache's tensors overlap")
+    # they are read while the cache is written
+    if any(a[0] < s[1] and s[0] < a[1] for s in map(_span, others) for a in at):
+        raise ValueError("q, k or v overlap the cache")
     return Smax
 
 
@@ -95,11 +104,11 @@ def kvcache_q8_attn(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], k_codes
         raise ValueError(f"q must be [B, S, H, 128], none of them 0 (got {tuple(q.shape)})")
     dev = q.device
     cache = (k_codes, v_codes, k_scale, v_scale, k_recent, v_recent)
-    Smax = _check_cache(cache, B, H, D, dev)
     if (k is None) != (v is None):
         raise ValueError("k and v must be given together")
+    Smax = _check_cache(cache, B, H, D, dev, (q,) if k is None else (q, k, v))
     if k is not None:
-        k, v = k.contiguous() if k.data_ptr() % 16 else k, v.contiguous() if v.data_ptr() % 16 else v
+        k, v = (x.clone(memory_format=torch.contiguous_format) if x.data_ptr() % 16 else x for x in (k, v))
         for name, x in (("k", k), ("v", v)):
             _check4(x, name)
             if tuple(x.shape) != (B, S, H, D) or x.device != dev:
@@ -107,6 +116,8 @@ def kvcache_q8_attn(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], k_codes
     if cache_seqlens is not None:
         if cache_seqlens.dtype not in (torch.int32, torch.int64) or cache_seqlens.numel() != B:
             raise ValueError(f"cache_seqlens must hold {B} int32 (got {cache_seqlens.dtype} {tuple(cache_seqlens.shape)})")
+        if cache_seqlens.dtype == torch.int64:   # outside int32 is outside the cache
+            cache_seqlens = cache_seqlens.clamp(0, Smax)
         cache_seqlens = cache_seqlens.to(device=dev, dtype=torch.int32).contiguous()
     elif not 0 <= cache_seqlen <= Smax:
         raise ValueError(f"cache_seqlens = {cache_seqlen} is outside [0, {Smax}]")

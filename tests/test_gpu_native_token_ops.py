@@ -319,3 +319,37 @@ def test_two_streams_at_once():
         for a, b in zip(want, got):
             for u, v in zip(a, b):
                 assert torch.equal(u, v)
+
+
+def test_cache_operands_that_share_memory_are_refused(path):
+    """Queries or rows that lie in the cache would be read while it is written."""
+    cache = kvcache_q8(2, 128, 2)
+    q, k, v = (_rand(2, 3, 2, 128, seed=i) for i in range(3))
+    inside = cache.k_recent.transpose(1, 2)[:, :3]     # [B, 3, H, 128]
+    for args in ((inside, k, v), (q, inside, v), (q, k, inside), (inside, None, None)):
+        with pytest.raises(ValueError, match="overlap"):
+            flash_attn_with_kvcache_q8(args[0], cache, args[1], args[2], 0)
+    # one allocation that holds all, without sharing
+    whole = torch.zeros(2 * cache.k_recent.numel() + q.numel(), dtype=BF, device=DEV)
+    n = cache.k_recent.numel()
+    beside = cache._replace(k_recent=whole[:n].view_as(cache.k_recent), v_recent=whole[n + q.numel():].view_as(cache.k_recent))
+    row = whole[n:n + q.numel()].view_as(q)
+    row.copy_(k)
+    assert torch.equal(flash_attn_with_kvcache_q8(q, beside, row, v, 0), flash_attn_with_kvcache_q8(q, cache, k, v, 0))
+    assert torch.equal(beside.k_recent, cache.k_recent)
+
+
+def test_wide_lengths_and_rows_off_alignment(path):
+    q, k, v = (_rand(3, 2, 2, 128, seed=i) for i in range(3))
+    off = torch.cat((k.flatten()[:1], k.flatten()))[1:].view_as(k)
+    assert off.data_ptr() % 16
+    lens = torch.tensor([2 ** 32 + 7, -(2 ** 33), 100], device=DEV)
+    out = []
+    for n, kk in ((lens, off), (torch.tensor([128, 0, 100], dtype=torch.int32, device=DEV), k)):
+        cache = kvcache_q8(3, 128, 2)
+        for j in range(0, 100, 50):
+            flash_attn_with_kvcache_q8(_rand(3, 50, 2, 128, seed=j), cache, _rand(3, 50, 2, 128, seed=j + 1),
+                                       _rand(3, 50, 2, 128, seed=j + 2), j)
+        out.append((flash_attn_with_kvcache_q8(q, cache, kk, v, n), *cache))
+    for a, b in zip(*out):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
