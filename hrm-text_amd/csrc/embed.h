@@ -230,11 +230,12 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(SortParams P) {
 }
 
 // The whole sort in one launch, for up to 2^14 tokens and ids below 2^18: a token is one word, id <<
-// 14 | i, and its place is the number of smaller words. Workgroup = 64 tokens; its 16 waves hold 64 R
-// of all words each, and one compare of a token's word (a scalar) with 64 of them, whose lanes are
-// counted as scalars, is all that a token and 64 others take: bound by the compares, T^2 / 64 of
-// them, on all CUs (16384 tokens 0.27 G pairs). A radix sort in one workgroup took 35 to 45 us for
-// those, bound by LDS, one in four launches 28; the gradient is cleared beside it.
+// 14 | i, and its place is the number of smaller words. Workgroup = `tile` tokens, 16 to 64 of them, so
+// that there are up to one for each CU; its 16 waves hold 64 R of all words each, and one compare of a
+// token's word (a scalar) with 64 of them, whose lanes are counted as scalars, is all that a token and
+// 64 others take: bound by those compares and counts, T^2 / 64 (16384 tokens, with 32 MB cleared
+// beside them, 32 us, 4999 11). A radix sort in one workgroup took 35 to 45 us for 16384, bound by
+// LDS, one in four launches 28 without the clearing.
 constexpr int kRankBits = 14, kRankThreads = 1024, kRankWaves = kRankThreads / 64;
 constexpr int64_t kRankTokens = 1 << kRankBits, kRankIds = ((int64_t)1 << (32 - kRankBits)) - 1;
 
@@ -243,26 +244,29 @@ __global__ __launch_bounds__(kRankThreads) __attribute__((amdgpu_waves_per_eu(8,
   if (clears<kRankThreads>(P, P.tiles)) return;
   __shared__ int count[kRankWaves][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int T = (int)P.T, i = blockIdx.x * 64 + lane;
+  const int T = (int)P.T, per = P.tile, i = blockIdx.x * per + lane;
+  const bool in = lane < per && i < T;
   uint32_t x[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int j = (wave * R + r) * 64 + lane;
     x[r] = j < T ? key_at(P, j) << kRankBits | (uint32_t)j : 0xffffffffu;   // above every token's
   }
-  const uint32_t mine = i < T ? key_at(P, i) << kRankBits | (uint32_t)i : 0xffffffffu;
+  const uint32_t mine = in ? key_at(P, i) << kRankBits | (uint32_t)i : 0xffffffffu;
   int n = 0;
-#pragma unroll 2
-  for (int l = 0; l < 64; ++l) {
-    const uint32_t w = (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
-    int c = 0;
+  for (int l0 = 0; l0 < per; l0 += 2) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[r] < w));
-    n = lane == l ? c : n;
+    for (int l = l0; l < l0 + 2; ++l) {
+      const uint32_t w = (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
+      int c = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) c += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[r] < w));
+      n = lane == l ? c : n;
+    }
   }
   count[wave][lane] = n;
   __syncthreads();
-  if (wave == 0 && i < T) {
+  if (wave == 0 && in) {
     int at = 0;
 #pragma unroll
     for (int g = 0; g < kRankWaves; ++g) at += count[g][lane];

@@ -1612,13 +1612,17 @@ int prefixlm_embedding_bwd(const prefixlm_embedding_args* a, void* stream_) {
     P.pos_out = reinterpret_cast<uint32_t*>(ws + w.pos[0]);
     P.zero_begin = 0;
     P.zero_end = units;
-    P.tiles = (int)((T + 63) / 64);
+    // one workgroup a CU at most: 4999 tokens 13.4 us (64 a workgroup 20.9)
+    P.tile = (int)std::max<int64_t>(16, (T + 511) / 512 * 2);
+    P.tiles = (int)((T + P.tile - 1) / P.tile);
     const int64_t n = P.tiles + std::min<int64_t>(256, (units + 4 * emb::kRankThreads - 1) / (4 * emb::kRankThreads));
     auto* k = T <= 1024   ? emb::rank_kernel<1>
               : T <= 2048 ? emb::rank_kernel<2>
               : T <= 4096 ? emb::rank_kernel<4>
+              : T <= 6144 ? emb::rank_kernel<6>
               : T <= 8192 ? emb::rank_kernel<8>
-                          : emb::rank_kernel<16>;
+              : T <= 12288 ? emb::rank_kernel<12>
+                           : emb::rank_kernel<16>;
     hipLaunchKernelGGL(k, dim3((unsigned)n), dim3(emb::kRankThreads), 0, stream, P);
   } else if (T == 0) {
     const unsigned n = share();

@@ -222,3 +222,19 @@ def test_refusals_on_the_gpu():
                                    (i, t[:0], {}, "V in")):
         with pytest.raises(ValueError, match=needle):
             embedding(ids, table, **kw)
+
+
+@pytest.mark.parametrize("T", [15, 16, 17, 32, 33, 1023, 1024, 1025, 2048, 4095, 4097, 5119, 6144, 6145, 8192, 8193, 9727, 12288,
+                               12289, 16383, 16384, 16385])
+def test_sorts_of_every_size(T):
+    """Small whole numbers, whose sums are exact in any order: the gradient is the integer sum. Ids at
+    both ends, some outside the table; the largest table of the one-launch sort and the next."""
+    print(f"[case] sort {T}", flush=True)
+    for V in (7, 262143, 262144):
+        g = torch.Generator().manual_seed(T)
+        ids = torch.randint(-1, V + 1, (T,), generator=g)
+        ids[0], ids[-1] = V - 1, 0
+        dy = torch.randint(-8, 9, (T, 8), generator=g)
+        want = torch.zeros(V + 2, 8, dtype=torch.int64).index_add_(0, ids + 1, dy)[1:-1]
+        got = embedding_bwd(ids.to(DEV), dy.to(BF).to(DEV), V, 1.0, F32, -1)
+        assert torch.equal(got.cpu(), want.float())
