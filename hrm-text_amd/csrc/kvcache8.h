@@ -462,11 +462,13 @@ __device__ __forceinline__ void extend_block_valu(const Params& P, int b, int h,
 // 16 staged rows is either codes or bf16 rows, and the 32 keys that a wave multiplies at a time
 // have one scale, as blocks begin at multiples of 64.
 //
-// The probabilities go into P V as two bf16 terms, 16 of their 24 bits: what that leaves, 2^-17 of
-// the sum of p |v|, is 2^-8 of what the output's rounding to bf16 does and less than the rows' own
-// rounding to 8 bits (three terms: 26.6 us for 4 x 16 heads x 45 queries on 2000 rows, two 25.8).
-// Bound by each wave's chain, 2.6 us a tile of 64 keys and 64 queries: half the cache's bytes, the
-// next tile but one on its way as well, change nothing.
+// The probabilities go into P V as two bf16 terms, each cut: that leaves less than 2^-15 of each, and on
+// average 2^-17 of the sum of p |v|, 2^-8 of what the output's rounding to bf16 does and less than the
+// rows' own rounding to 8 bits (a third term took 0.8 us of 26.6 for 4 x 16 heads x 45 queries on 2000
+// rows).
+// Bound by each wave's chain of LDS, products and exponentials, 1.7 us a tile of 64 keys and 64
+// queries (45 of them on 4051 keys of 64 pairs 33 us, with a cache in bf16 42): fewer address
+// operations change nothing.
 constexpr int kTerms = 2;
 template <class C, int QW>
 __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
@@ -520,37 +522,66 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
 
   // staging: thread = 16-byte chunk sch of rows srow + 16 r; V rows in permuted order
   const int srow = tid >> 4, sch = tid & 15, vrow = perm_row(srow);
-  u32x4 ks[NP], vs[NP];
-  const u32x4 zero = {0u, 0u, 0u, 0u};
+  // Rows past k1 are loaded as the last one below it and masked; a row has its first 8 bytes loaded, all
+  // of a code row's, and a bf16 row the others. So no register is written on two paths, and all loads
+  // of a tile are on their way together until the tile is stored (as 16 bytes on two paths, with
+  // zeroed registers past k1, every 16 rows waited for those before them: 4 x 16 heads x 45 queries on
+  // 2000 rows 28.0 us, now 24.3; 16 x 16 x 32 on 2157 92.8 and 61.8).
+  // pointers that meet from two paths have to say that they are of global memory, or the loads do not know
+  typedef const __attribute__((address_space(1))) char* gbytes;
+  typedef const __attribute__((address_space(1))) u32x2* gu32x2;
+  u32x2 klo[NP], khi[NP], vlo[NP], vhi[NP];
+  float next_k, next_v;   // the scales of this wave's 32 keys of the tile
   auto load_kv = [&](int t0) {
+    gbytes pk[NP], pv[NP];
+    const bool coded = t0 + TK <= nfull;
+    if (coded) {
 #pragma unroll
-    for (int r = 0; r < NP; ++r) {
-      const int jk = t0 + 16 * r + srow, jv = t0 + 16 * r + vrow;
-      ks[r] = vs[r] = zero;
-      if (t0 + 16 * r < nfull) {
-        if (jk < k1) {   // k1 may end a tile of codes early, where another split goes on
-          const u32x2 kw8 = *reinterpret_cast<const u32x2*>(kc + (int64_t)jk * D + 8 * sch);
-          ks[r] = u32x4{kw8[0], kw8[1], 0u, 0u};
-        }
-        if (jv < k1) {
-          const u32x2 vw8 = *reinterpret_cast<const u32x2*>(vc + (int64_t)jv * D + 8 * sch);
-          vs[r] = u32x4{vw8[0], vw8[1], 0u, 0u};
-        }
-      } else {
-        if (jk < k1) ks[r] = *reinterpret_cast<const u32x4*>(k_row(jk) + 8 * sch);
-        if (jv < k1) vs[r] = *reinterpret_cast<const u32x4*>(v_row(jv) + 8 * sch);
+      for (int r = 0; r < NP; ++r) {
+        pk[r] = (gbytes)(kc + (int64_t)min(t0 + 16 * r + srow, k1 - 1) * D + 8 * sch);
+        pv[r] = (gbytes)(vc + (int64_t)min(t0 + 16 * r + vrow, k1 - 1) * D + 8 * sch);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < NP; ++r) {
+        const int jk = min(t0 + 16 * r + srow, k1 - 1), jv = min(t0 + 16 * r + vrow, k1 - 1);
+        pk[r] = jk < nfull ? (gbytes)(kc + (int64_t)jk * D + 8 * sch)
+                           : (gbytes)(k_row(jk) + 8 * sch);
+        pv[r] = jv < nfull ? (gbytes)(vc + (int64_t)jv * D + 8 * sch)
+                           : (gbytes)(v_row(jv) + 8 * sch);
       }
     }
+#pragma unroll
+    for (int r = 0; r < NP; ++r) {
+      klo[r] = *(gu32x2)(pk[r]);
+      vlo[r] = *(gu32x2)(pv[r]);
+    }
+    if (!coded) {
+#pragma unroll
+      for (int r = 0; r < NP; ++r) {   // a code row's bytes again, unused
+        khi[r] = *(gu32x2)(pk[r] + (min(t0 + 16 * r, k1 - 1) < nfull ? 0 : 8));
+        vhi[r] = *(gu32x2)(pv[r] + (min(t0 + 16 * r, k1 - 1) < nfull ? 0 : 8));
+      }
+    }
+    const int blk = max(min(t0 + 32 * kw, nfull - 1), 0) / kBlock;
+    next_k = ksc[blk];
+    next_v = vsc[blk];
   };
   auto store_kv = [&](int buf, int t0) {
     char* base = smem + buf * G::BUF + srow * RS + sch * 16;
+    u32x4 vs[NP];
 #pragma unroll
     for (int r = 0; r < NP; ++r) {
-      if (t0 + 16 * r < nfull) {
-        ks[r] = codes_bf16<C>(u32x2{ks[r][0], ks[r][1]});
-        vs[r] = codes_bf16<C>(u32x2{vs[r][0], vs[r][1]});
+      // a strip whose first row is clamped is one whose rows all are: its codes or rows are the last one's
+      u32x4 k;
+      if (min(t0 + 16 * r, k1 - 1) < nfull) {
+        k = codes_bf16<C>(klo[r]);
+        vs[r] = codes_bf16<C>(vlo[r]);
+      } else {
+        k = u32x4{klo[r][0], klo[r][1], khi[r][0], khi[r][1]};
+        vs[r] = u32x4{vlo[r][0], vlo[r][1], vhi[r][0], vhi[r][1]};
       }
-      *reinterpret_cast<u32x4*>(base + 16 * r * RS) = ks[r];
+      *reinterpret_cast<u32x4*>(base + 16 * r * RS) = k;
       *reinterpret_cast<u32x4*>(base + TILE + 16 * r * RS) = vs[r];
     }
     u16x2 m = {0, 0};
@@ -589,6 +620,7 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
     if (qm[0] >= 0x7180 || qm[1] >= 0x7180) bad = 1;
     for (int t = 0; t < nt; ++t) {
       const int buf = G::NBUF == 2 ? t & 1 : 0;
+      const float this_k = next_k, this_v = next_v;
       load_kv(k0 + (t + 1) * TK);
       const int kk = k0 + t * TK + 32 * kw;   // first key of this wave's 32
       if (kk < kend_w) {
@@ -610,7 +642,7 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
         // key kk + 8 (r / 4) + 4 hh + r % 4 is seen iff it is below kq
         const int tk = kq - kk - 4 * hh;
         const bool coded = kk < nfull;
-        const float unit_k = coded ? ksc[kk / kBlock] : 1.f, unit_v = coded ? vsc[kk / kBlock] : 1.f;
+        const float unit_k = coded ? this_k : 1.f, unit_v = coded ? this_v : 1.f;
         if (!(unit_k < INFINITY && unit_v < INFINITY)) bad = 1;
         const float c = P.scale_log2 * unit_k;
 #pragma unroll

@@ -1077,10 +1077,10 @@ static bool rows_apart(int64_t B, int64_t N, int64_t H, int64_t sb, int64_t sn, 
 }
 
 // Query waves of the extend kernel for S new rows, its query blocks, and the key splits of
-// either kernel.
+// either kernel. one_round (the 8-bit cache's): above six splits, 512 workgroups at most.
 static int ext_qw(int S) { return S <= 32 ? 1 : S <= 64 ? 2 : 4; }
 static int kv_nqb(int S) { return S == 1 ? 1 : (S + 32 * ext_qw(S) - 1) / (32 * ext_qw(S)); }
-static int64_t kv_nsplit(int64_t B, int S, int64_t H, int64_t Smax) {
+static int64_t kv_nsplit(int64_t B, int S, int64_t H, int64_t Smax, bool one_round = false) {
   if (S == 1) {
     // Few (row, head) pairs: 512 workgroups, at least one 64-key step each (16 pairs x 4096
     // keys 13.1 us at 512, 14.2 at 1024, 12.0 at 256; 64 pairs 26.1, 26.7, 28.4). Many: 1024,
@@ -1104,7 +1104,9 @@ static int64_t kv_nsplit(int64_t B, int S, int64_t H, int64_t Smax) {
   // 512 workgroups fill the chip (two per CU); more splits mostly add partials to write and
   // merge: 4 x 16 heads x 45 queries 31 us at 512, 41 at 1024, 58 at 2048, and 2 x 16 x 300 on
   // 8192 rows 119 us at 256, 103 at 512, 97 at 1024, 115 at 2048
-  const int64_t want = (512 + units - 1) / units, most = (Smax + tk - 1) / tk;
+  int64_t want = (512 + units - 1) / units;
+  const int64_t most = (Smax + tk - 1) / tk;
+  if (one_round && want > 6) want = 512 / units;
   const int64_t n = std::max<int64_t>(1, std::min({want, most, (int64_t)kvc::kMaxSplits}));
   // One split instead where the tiles it walks more cost less than the combine's launch and the
   // partials, which n splits write and read for every query. The estimate: a tile of 32, 64 or 128
@@ -1670,7 +1672,11 @@ int prefixlm_embedding_bwd(const prefixlm_embedding_args* a, void* stream_) {
 }  // extern "C"
 
 // ---- attention over an 8-bit cache -----------------------------------------------------------
-// Splits of the keys. Several queries: as for bf16 (the tiles and their chain are the same). One query:
+// Splits of the keys. Several queries: as for bf16 (the tiles are the same), but above six splits no
+// more than 512 workgroups, as a second round of a few costs more than the longer splits (24 units x
+// 10569 keys of 2 rows, 100 queries, 71.8 us with 22 splits, 53.5 with 21; 60 x 4006, 90 queries 60.9
+// and 49.8; with fewer splits ragged rows want the more: 120 units x 4178 keys 94.7 with five, 110 with
+// four). One query:
 // one split for caches of up to 1536 rows, whose keys take less time than the combine's launch (16
 // pairs x 920 of 1536 rows 8.7 us, 11.3 with three splits; 128 x 800 of 1024 9.9 and 12.8; 64 x 1800
 // of 2048 14.8, 13.2 with four), and from 192 pairs on, one for each CU nearly (256 x 12288 of 16384
@@ -1678,7 +1684,7 @@ int prefixlm_embedding_bwd(const prefixlm_embedding_args* a, void* stream_) {
 // pairs x 23000 of 32768 rows 51.3 with 16 splits, 54.8 with eight; 80 x 4096 20.1 with twelve, 24.2
 // with two), of at least two blocks each.
 static int64_t kv8_nsplit(int64_t B, int S, int64_t H, int64_t Smax) {
-  if (S > 1) return kv_nsplit(B, S, H, Smax);
+  if (S > 1) return kv_nsplit(B, S, H, Smax, true);
   const int64_t units = B * H;
   if (Smax <= 1536 || units >= 192) return 1;
   return std::min({(768 + units - 1) / units, Smax / (2 * kv8::kBlock), (int64_t)kvc::kMaxSplits});

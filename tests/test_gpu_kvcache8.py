@@ -5,6 +5,8 @@ magnitudes A, and exponentials of scores off by d change each weight by d relati
 rows by 2 d of the sum of p |v|; n keys add n u more, and the splits' joins 100 u. out is rounded to
 bf16, 2^-8 relative. A call on an empty cache runs the training forward, which rounds the
 probabilities to bf16: 2^-8 of the sum of p |v| on top, and its exponentials' argument with it.
+Several queries multiply p scale as two bf16 terms, each cut: of 2^e m, 1 <= m < 2, the first leaves
+r < 2^(e-7), exactly, and the second less than 2^-7 of r's leading bit, at most 2^(e-8): 2^-15 of p.
 Codes, scales and bf16 rows are equal bit for bit.
 """
 import math
@@ -60,7 +62,7 @@ def _tol(q, cache, k, mag, want, n, prefill=False, softmax_scale=None):
               float(k.float().abs().max()) if k is not None else 0.0)      # the largest magnitude of a key
     s = 1.0 / math.sqrt(128) if softmax_scale is None else abs(softmax_scale)
     A = q.double().abs().sum(-1, keepdim=True) * top * s
-    rel = 2 * 140 * U * A + (n + 100) * U + (2.0 ** -7 if prefill else 0.0)
+    rel = 2 * 140 * U * A + (n + 100) * U + (2.0 ** -7 if prefill else 2.0 ** -15 if q.shape[1] > 1 else 0.0)
     return 2.0 ** -8 * want.abs() + rel * mag + 1e-30
 
 
@@ -437,3 +439,30 @@ def test_refusals_on_the_gpu():
     refuse("outside", lens=-1)
     a = flash_attn_with_kvcache_q8(q, good, q, q, torch.tensor([3, 5], device=DEV))          # int64 lengths
     assert a.shape == q.shape
+
+
+@pytest.mark.parametrize("dtype", CODES)
+@pytest.mark.parametrize("S", [2, 33, 65])
+def test_every_end_of_a_tile(S, dtype):
+    """Lengths at which the codes, the bf16 rows and the splits end at every place of a tile."""
+    print(f"[case] ends {S} {dtype}", flush=True)
+    H, Smax = 1, 256
+    lens = torch.cat((torch.arange(0, Smax - S, 5), torch.tensor([Smax - S]))).int()
+    g = torch.Generator().manual_seed(77 + S)
+    B = lens.numel()
+    q, k, v = (_rows(g, B, S, H, 128) for _ in range(3))
+    cache = _filled(B, H, Smax, dtype, g)
+    _check(q, cache, k, v, lens, True, "causal")
+    _check(q, cache, k, v, lens, False, "all")
+    _check(q, cache, None, None, lens, True, "alone")
+
+
+@pytest.mark.parametrize("S", [7, 64, 100])
+def test_one_row_with_many_splits(S):
+    """One batch row and a long cache: the most splits, whose ends fall into codes, ring and new rows."""
+    print(f"[case] splits {S}", flush=True)
+    g = torch.Generator().manual_seed(S)
+    q, k, v = (_rows(g, 1, S, 2, 128) for _ in range(3))
+    cache = _filled(1, 2, 4096, torch.float8_e4m3fn, g)
+    for n in (0, 64, 1000, 2047, 4096 - S):
+        _check(q, cache, k, v, torch.tensor([n], dtype=torch.int32), True, n)
