@@ -18,6 +18,7 @@ template <>
 struct Row8<bf16> {
   u32x4 w;
   __device__ __forceinline__ void load(const bf16* p) { w = *reinterpret_cast<const u32x4*>(p); }
+  __device__ __forceinline__ void arrive() { settle(w); }
   __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -35,6 +36,10 @@ struct Row8<float> {
   __device__ __forceinline__ void load(const float* p) {
     w[0] = reinterpret_cast<const f32x4*>(p)[0];
     w[1] = reinterpret_cast<const f32x4*>(p)[1];
+  }
+  __device__ __forceinline__ void arrive() {
+    settle(__builtin_bit_cast(u32x4, w[0]));
+    settle(__builtin_bit_cast(u32x4, w[1]));
   }
   __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
@@ -316,6 +321,9 @@ __global__ __launch_bounds__(256) void sum_kernel(SumParams P) {
       const int64_t p = (uint32_t)__builtin_amdgcn_readlane((int)pos, t + u < n ? t + u : t);
       if (on) r[u].load(dy + p * P.dy_st);
     }
+    // all at once here: a wait for the next token's row would be one for this token's stores too
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) r[u].arrive();
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (t + u >= n) break;
