@@ -375,9 +375,10 @@ int prefixlm_kvcache_fwd(const prefixlm_kvcache_args* args, void* stream);
  * Smax is a multiple of 64. Rows below len / 64 * 64 are attended from the codes, rows from there to
  * len - 1 from k_recent, v_recent, the call's new rows as given. Afterwards the blocks that the new
  * rows complete are rounded: scale = max(largest magnitude times the fp32 value of 1/448 (e4m3) or
- * 1/127 (int8), 2^-126), code = round(row / scale) to nearest, ties to even; and the new rows among the last 64 before the
- * incomplete block and those in it are written to k_recent, v_recent. So up to 64 rows can be taken
- * back by calling with a smaller len. Lengths outside [0, Smax] count as the nearest of the two. */
+ * 1/127 (int8), 2^-126), code = round(row / scale) to nearest, ties to even; and the new rows among the
+ * last 64 before the incomplete block and those in it are written to k_recent, v_recent. So up to 64
+ * rows can be taken back by calling with a smaller len. Lengths outside [0, Smax] count as the nearest
+ * of the two. The cache's tensors overlap neither each other nor q, k, v and out. */
 typedef struct prefixlm_kvcache8_args {
   const void* q;
   const void* k;                 /* new rows, or NULL (k and v together): attend the cache only */
