@@ -159,10 +159,12 @@ constexpr int kGroups = 8;        // of a thread's vectors, by their turn
 struct TopShared {
   unsigned long long cand[kCand];
   float largest[kGroups][NT];     // of each thread's values in a group
+  uint16_t list[kCand];           // groups to look at again: thread, and group << 9
   uint32_t keys[NT / 8];
   unsigned long long best[NT / 64];
-  int n;
+  int n, groups;
 };
+static_assert(NT == 1 << 9 && kGroups << 9 <= 1 << 16, "a list's entry");
 
 // The `top` largest keys of cand[0, n), in order, to put(rank, key)
 template <class Put>
@@ -209,13 +211,14 @@ __device__ __forceinline__ void finish_row(const Params& P, int64_t row, const S
 // registers and the next four on their way; four workgroups a CU. Bound by the loads where rows are
 // many (6144 of 65536 bf16 logits, 805 MB, 135 to 158 us, 5.1 to 6.0 TB/s), by about ten operations a
 // logit and the search behind the pass where all workgroups run at once (1021 rows of 50257 with
-// entropy and eight alternatives 38 us, with neither 28), and by one CU's exponentials for
-// few rows (4 rows of 65536 with five alternatives 11.3 us).
+// entropy and eight alternatives 35 us, with neither 28), and by one CU's exponentials for
+// few rows (4 rows of 65536 with five alternatives 10.1 us, without 6.4).
 //
 // TOP: after the pass the largest values of 64 sets of 8 threads are known. The k-th largest of those
-// is reached by at least k elements, so only threads whose own largest reaches it look at their
-// elements again, and only at the groups whose largest does; those that reach it, mostly few more
-// than k, are ranked against each other. Where they do not fit (rows of many equal values), or a NaN
+// is reached by at least k elements, so only the groups of a thread's vectors whose largest reaches it
+// are looked at again, one vector a thread (by the thread that holds the group, a round trip to memory
+// for each: 4 x 65536 with 20 alternatives 14.8 us, now 11.0); the elements that reach it, mostly few
+// more than k, are ranked against each other. Where they do not fit (rows of many equal values), or a NaN
 // is among them, which the maxima pass over, a walk finds the next largest k times.
 template <class T, bool ENT, bool TOP>
 __global__ __launch_bounds__(NT) void forward_kernel(Params P) {
@@ -326,7 +329,7 @@ __global__ __launch_bounds__(NT) void forward_kernel(Params P) {
     step(std::integral_constant<int, 0x4E>{});
     step(std::integral_constant<int, 0x141>{});
     if ((lane & 7) == 0) t.keys[tid >> 3] = k;
-    if (tid == 0) t.n = 0;
+    if (tid == 0) t.n = t.groups = 0;
   }
   __syncthreads();
   static_assert(NT / 8 == 64 && kMaxTop <= 64, "one set a lane, and a top-th largest of them");
@@ -343,33 +346,32 @@ __global__ __launch_bounds__(NT) void forward_kernel(Params P) {
   }
   // fewer sets with elements than `top`: every element (none of them NaN, or the walk decides)
   const float least = thr ? value_of(thr) : -INFINITY;
-  if (any && m_thread >= least) {
-    auto look = [&](float f, int64_t j) {
-      if (f >= least) {
-        const int at = atomicAdd(&t.n, 1);   // the order does not matter: they are ranked
-        if (at < kCand) t.cand[at] = key_of(f, j);
-      }
-    };
-    for (int i = 0; i < kGroups; ++i) {
-      if (!(t.largest[i][tid] >= least)) continue;
-      for (int64_t g = v0 + (int64_t)i * kUnroll * NT; g < v1; g += kGroups * kUnroll * NT) {
-        Vec<T> w[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (g + u * NT + tid < v1) w[u].load(x + 8 * (g + u * NT + tid));
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          if (g + u * NT + tid >= v1) break;
-          float m = w[u].get(0);
-#pragma unroll
-          for (int e = 1; e < 8; ++e) m = fmaxf(m, w[u].get(e));
-          if (m >= least)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) look(w[u].get(e), 8 * (g + u * NT + tid) + e);
-        }
-      }
+  auto look = [&](float f, int64_t j) {
+    if (f >= least) {
+      const int at = atomicAdd(&t.n, 1);   // the order does not matter: they are ranked
+      if (at < kCand) t.cand[at] = key_of(f, j);
     }
+  };
+  if (any && m_thread >= least) {
+    for (int i = 0; i < kGroups; ++i)
+      if (v0 + (int64_t)i * kUnroll * NT + tid < v1 && t.largest[i][tid] >= least) {
+        const int at = atomicAdd(&t.groups, 1);
+        if (at < kCand) t.list[at] = (uint16_t)(tid | i << 9);
+      }
     if (tid < n_edge) look(edge, edges.at(tid));
+  }
+  __syncthreads();
+  // a thread takes one vector of a listed group, so that all are on their way together (a group holds
+  // one of the values that are looked for at least: more groups than fit are more candidates than fit)
+  const int groups = t.groups;
+  for (int k = tid; k < kUnroll * (groups < kCand ? groups : 0); k += NT) {
+    const int of = t.list[k / kUnroll] & (NT - 1), i = t.list[k / kUnroll] >> 9;
+    for (int64_t v = v0 + ((int64_t)i * kUnroll + k % kUnroll) * NT + of; v < v1; v += kGroups * kUnroll * NT) {
+      Vec<T> w;
+      w.load(x + 8 * v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) look(w.get(e), 8 * v + e);
+    }
   }
   __syncthreads();
   const float ln_s = logf(a.s), ref = ref_of(a.m);
@@ -386,7 +388,7 @@ __global__ __launch_bounds__(NT) void forward_kernel(Params P) {
   };
   if (P.nsplit > 1 && tid >= want && tid < top) P.part_top[(row * P.nsplit + split) * top + tid] = 0;
   const int n = t.n;
-  if (n >= want && n <= kCand && a.s == a.s) {
+  if (n >= want && n <= kCand && groups < kCand && a.s == a.s) {
     sorted_top(t.cand, n, want, put);
     return;
   }

@@ -324,3 +324,20 @@ def test_refusals_on_the_gpu():
             token_logprobs(x, **bad)
     with pytest.raises(ValueError, match="bf16 or fp32"):
         token_logprobs(x.half(), t)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("equal", [3, 600, 1022, 1023, 1024, 1025, 2048])
+def test_alternatives_among_many_equal_ones(equal, dtype):
+    """The largest value at `equal` places, each in another thread's vectors: as many places as are
+    ranked at once, one more, and fewer; the lowest ids win. A row alone and a row among others."""
+    print(f"[case] equal {equal} {dtype}", flush=True)
+    V, g = 65543, torch.Generator().manual_seed(equal)
+    x = torch.randn(3, V, generator=g).clamp_(max=3.0).to(dtype)
+    turn, thread = torch.arange(2048) // 512, torch.arange(2048) % 512
+    at = (8 * (turn * 2048 + thread))[torch.randperm(2048, generator=g)[:equal]]
+    x[1, at] = 4.0
+    x[2, at] = 4.0
+    x[2, V - 1] = 5.0
+    for top in (1, 7, 64):
+        _check(x, torch.zeros(3, dtype=torch.int64), top=top, with_grad=False)
