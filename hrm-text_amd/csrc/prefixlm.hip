@@ -1374,16 +1374,20 @@ int prefixlm_timer_read(void* timer, float* total_ms, int32_t* launches) {
 static bool launchable(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffll / threads && blocks <= 0x7fffffff; }
 
 // ---- log probabilities ---------------------------------------------------------------
-// Splits of a row, where the rows alone are fewer than the CUs and long enough to pay for the second
-// launch: 512 workgroups, of at least 8192 logits each. One split against several: 8 rows of 65536 logits
-// 7.1 and 9.5 us, of 131072 10.1 and 11.2, of 262144 17.1 and 10.6; with alternatives, whose search is
-// shorter in a split, of 65536 11.9 and 11.9, of 131072 15.3 and 13.5.
+// Splits of a row, where the rows alone are far fewer than the CUs and long enough to pay for the second
+// launch: 512 workgroups, of at least 8192 logits each. One split against several: 8 rows of 98304 logits
+// 8.2 and 9.1 us, of 131072 9.8 and 9.2, of 262144 16.8 and 9.1; with five alternatives, whose search is
+// shorter in a split, of 65536 10.3 and 11.0, of 98304 12.1 and 11.6 (64 rows 12.3 and 13.7), of 131072
+// 14.2 and 11.7; with 20, 8 rows of 98304 13.0 and 14.5, of 131072 15.0 and 14.5. 64 rows of 262144 17.2
+// and 9.5, 200 rows 18.0 and 26.4. The alternatives of all splits are ranked together, each by one of 256
+// threads: with more of them than that 8 rows of 262144 with 20 took 37.2 us, now 15.5, one split 22.8.
 static int lp_nsplit(int64_t rows, int64_t V, int32_t top) {
-  if (rows < 1 || rows >= 256 || V < (top > 0 ? 98304 : 163840)) return 1;
+  if (rows < 1 || rows > 64 || V < (top > 0 && top <= 8 && rows <= 16 ? 98304 : 131072)) return 1;
   const int64_t most = V / (16 * lp::NT), want = (512 + rows - 1) / rows;
-  const int64_t fit = top > 0 ? lp::kCand / top : lp::kMaxSplits;
+  const int64_t fit = top > 0 ? 256 / top : lp::kMaxSplits;
   return (int)std::min({most, want, fit, (int64_t)lp::kMaxSplits});
 }
+static_assert(256 / lp::kMaxTop >= 1 && 256 <= lp::kCand, "a split at least, and the combine's candidates fit");
 
 static size_t lp_workspace(int64_t rows, int64_t vocab, int32_t top_k) {
   if (rows < 1 || vocab < 1 || top_k < 0) return 0;

@@ -341,3 +341,14 @@ def test_alternatives_among_many_equal_ones(equal, dtype):
     x[2, V - 1] = 5.0
     for top in (1, 7, 64):
         _check(x, torch.zeros(3, dtype=torch.int64), top=top, with_grad=False)
+
+
+@pytest.mark.parametrize("rows,V,top", [(1, 98304, 8), (16, 98307, 3), (2, 131072, 9), (64, 131073, 20), (3, 262145, 64),
+                                        (65, 131072, 2), (5, 140001, 0)])
+def test_split_rows(rows, V, top):
+    """Rows in several workgroups, with as few and as many alternatives as their join ranks."""
+    print(f"[case] split {rows} {V} {top}", flush=True)
+    x, t = _random(rows, V, torch.bfloat16, rows + top)
+    x[0, -5:] = 60.0
+    x[-1, :V // 2] = -math.inf
+    _check(x, t, top=top, with_grad=False)
