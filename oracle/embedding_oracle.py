@@ -1,6 +1,6 @@
 """CPU/fp64 oracle for the scaled embedding -- TEST INFRASTRUCTURE.
 
-Only tests may import this module, as the checker; the product path never calls it.
+Only tests may import this module; the product path never calls it.
 
 ``scale * table[ids]`` (models/lm_head.py:34-43) and the table's gradient, token by token in
 float64. Pinned by ``F.embedding`` and its autograd (tests/test_embedding_cpu.py).

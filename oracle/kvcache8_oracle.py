@@ -1,6 +1,6 @@
 """CPU/fp64 oracle for attention over an 8-bit KV cache -- TEST INFRASTRUCTURE.
 
-Only tests may import this module, as the checker; the product path never calls it.
+Only tests may import this module; the product path never calls it.
 
 ``attend`` is the definition, sequence by sequence: the rows that query i sees are the complete
 blocks' ``scale * code``, then the incomplete block's bf16 rows from the ring, then the call's new

@@ -1,6 +1,6 @@
 """CPU/fp64 oracle for token log probabilities -- TEST INFRASTRUCTURE.
 
-Only tests may import this module, as the checker; the product path never calls it.
+Only tests may import this module; the product path never calls it.
 
 Restates, row by row and from the definitions, what ``token_logprobs`` gives for logits x and a
 target t: ``x_t - lse`` with ``lse = ln sum_j e^x_j`` (the negative of the reference's cross entropy,
