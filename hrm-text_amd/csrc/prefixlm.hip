@@ -219,6 +219,10 @@ int fwd_finds_items(int64_t grid, int32_t numseqs, int32_t max_all, bool* self) 
   return rc;
 }
 
+// The forward's and backward's buffer offsets inside one segment are 32-bit byte offsets:
+// (rows + 256) rows of 16-bit elements take less than 2^31 bytes
+bool segment_fits(int64_t rows, int64_t token_stride) { return token_stride <= (((int64_t)1 << 30) - 1) / (rows + 256); }
+
 // Checks shared by forward and backward. `strides` lists (stride_t, stride_h) pairs.
 int check_common(const void* const* ptrs, int nptr, const int64_t* strides, int nstr,
                  int32_t T, int32_t H, int32_t D, int32_t total, int32_t numseqs,
@@ -248,8 +252,7 @@ int check_common(const void* const* ptrs, int nptr, const int64_t* strides, int 
                   "tensor %d strides (token %lld, head %lld) must be multiples of 8 with token "
                   "stride >= head_dim and head stride >= 0",
                   i, (long long)st, (long long)sh);
-    // buffer offsets inside one segment are 32-bit byte offsets
-    if (((int64_t)max_all + 256) * st * 2 >= (int64_t)1 << 31)
+    if (!segment_fits(max_all, st))
       return fail(PREFIXLM_ERR_INVALID, "segment of %d rows x token stride %lld exceeds 2 GiB",
                   max_all, (long long)st);
   }
@@ -1124,13 +1127,15 @@ static int64_t kv_nsplit(int64_t B, int S, int64_t H, int64_t Smax, bool one_rou
 }
 
 // The reference's prefill, an empty cache and a packed batch of new rows: the varlen forward over
-// them; with `append` the launch also writes them to the bf16 caches.
+// them; with `append` the launch also writes them to the bf16 caches. Prompts whose rows lie further
+// apart than that forward's offsets reach take the extend kernel, whose strides have 64 bits.
 static bool kv_prefills(const kvc::Params& P) {
   const int64_t S = P.S;
   const bool packed = P.B == 1 || (P.q_sb == S * P.q_ss && P.k_sb == S * P.k_ss && P.v_sb == S * P.v_ss &&
                                    P.o_sb == S * P.o_ss);
   return !P.seqlens && P.seqlen_const == 0 && P.s_new && packed && P.S <= P.Smax &&
-         (int64_t)P.B * P.S < 0x7fffffff && P.q_ss >= kvc::D && P.k_ss >= kvc::D && P.v_ss >= kvc::D && P.o_ss >= kvc::D;
+         (int64_t)P.B * P.S < 0x7fffffff && P.q_ss >= kvc::D && P.k_ss >= kvc::D && P.v_ss >= kvc::D && P.o_ss >= kvc::D &&
+         segment_fits(S, std::max(std::max(P.q_ss, P.k_ss), std::max(P.v_ss, P.o_ss)));
 }
 static int kv_prefill(const kvc::Params& P, bool append, hipStream_t stream) {
   const int B = P.B, S = P.S, H = P.H;
