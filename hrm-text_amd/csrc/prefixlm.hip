@@ -1128,12 +1128,13 @@ static int64_t kv_nsplit(int64_t B, int S, int64_t H, int64_t Smax, bool one_rou
 
 // The reference's prefill, an empty cache and a packed batch of new rows: the varlen forward over
 // them; with `append` the launch also writes them to the bf16 caches. Prompts whose rows lie further
-// apart than that forward's offsets reach take the extend kernel, whose strides have 64 bits.
+// apart than that forward's offsets reach take the extend kernel, whose strides have 64 bits, and so do
+// softmax scales that are not positive: the forward masks scores, and takes their maximum, before it scales.
 static bool kv_prefills(const kvc::Params& P) {
   const int64_t S = P.S;
   const bool packed = P.B == 1 || (P.q_sb == S * P.q_ss && P.k_sb == S * P.k_ss && P.v_sb == S * P.v_ss &&
                                    P.o_sb == S * P.o_ss);
-  return !P.seqlens && P.seqlen_const == 0 && P.s_new && packed && P.S <= P.Smax &&
+  return !P.seqlens && P.seqlen_const == 0 && P.s_new && P.scale_log2 > 0.f && packed && P.S <= P.Smax &&
          (int64_t)P.B * P.S < 0x7fffffff && P.q_ss >= kvc::D && P.k_ss >= kvc::D && P.v_ss >= kvc::D && P.o_ss >= kvc::D &&
          segment_fits(S, std::max(std::max(P.q_ss, P.k_ss), std::max(P.v_ss, P.o_ss)));
 }
