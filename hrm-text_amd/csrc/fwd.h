@@ -124,6 +124,49 @@ __device__ __forceinline__ void append_rows(const Params& P, int blk) {
   }
 }
 
+// A prompt's queries qw0 + i of a wave, for the bits i of `rows`, key by key without the matrix cores and
+// written over what is there: a 16-lane group per query. For queries whose result is not finite: in P V
+// on the matrix cores 0 * inf reaches queries that must not see the key, and the scores are summed
+// before the softmax scale, which can pass fp32's range where the scaled ones here do not.
+__device__ __forceinline__ void redo_rows(const Params& P, uint32_t rows, int qw0, int cs, int h, int L, int p) {
+  const int lane = threadIdx.x & 63, g16 = lane & 15;
+#pragma unroll 1
+  for (int i = lane >> 4; i < 32; i += 4) {
+    if (!((rows >> i) & 1)) continue;
+    const int qi = qw0 + i, kq = min(L, max(p, qi + 1));
+    float q[8], o[8];
+    const u32x4 qv = *reinterpret_cast<const u32x4*>(P.q + (int64_t)(cs + qi) * P.q_st + h * P.q_sh + 8 * g16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      q[2 * e] = bf16lo(qv[e]) * P.scale_log2;
+      q[2 * e + 1] = bf16hi(qv[e]) * P.scale_log2;
+      o[2 * e] = o[2 * e + 1] = 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int j = 0; j < kq && l == l; ++j) {   // a sum that is NaN stays so
+      const u32x4 kv = *reinterpret_cast<const u32x4*>(P.k + (int64_t)(cs + j) * P.k_st + h * P.k_sh + 8 * g16);
+      const u32x4 vv = *reinterpret_cast<const u32x4*>(P.v + (int64_t)(cs + j) * P.v_st + h * P.v_sh + 8 * g16);
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += q[2 * e] * bf16lo(kv[e]) + q[2 * e + 1] * bf16hi(kv[e]);
+      s = row16_sum(s);
+      const float mx = fmaxf(m, s), ref = mx == -INFINITY ? 0.f : mx;
+      const float alpha = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(s - ref);
+      m = mx;
+      l = l * alpha + w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[2 * e] = o[2 * e] * alpha + w * bf16lo(vv[e]);
+        o[2 * e + 1] = o[2 * e + 1] * alpha + w * bf16hi(vv[e]);
+      }
+    }
+    const float inv = 1.f / l;
+    *reinterpret_cast<bf16x8*>(P.o + (int64_t)(cs + qi) * P.o_st + h * P.o_sh + 8 * g16) =
+        cvt8(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, o[4] * inv, o[5] * inv, o[6] * inv, o[7] * inv);
+  }
+}
+
 // The (item, head) of this workgroup without a work list, for at most 64 segments: lane s reads
 // segment s, a wave scan counts the row tiles before each, and the item's segment is the first
 // whose tiles end past it. Items are in segment order, not by cost, which is as good while
@@ -437,6 +480,19 @@ __global__ __launch_bounds__(NT * KS, KS > 1 ? 2 : HD == 64 ? 4 : 3) void prefix
       }
   }
   const float inv = wave_active ? 1.f / lt : 0.f;
+  uint32_t redo = 0;   // the wave's queries that redo_rows takes again
+  if constexpr (UNIFORM) {
+    // sums past the range or NaN, outputs that are (their sum, which is finite only where they are), and
+    // scores so low that a raw one may have left the range
+    float total = 0.f;
+#pragma unroll
+    for (int t = 0; t < NDT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) total += oacc[t][r];
+    const bool sound = lt < INFINITY && fabsf(total) < INFINITY && m_run >= 200.f - 3e38f * c;
+    const uint64_t b = __builtin_amdgcn_ballot_w64(wave_active && qi < L && !sound);
+    redo = (uint32_t)b | (uint32_t)(b >> 32);   // lanes l and l + 32 hold halves of one query
+  }
   {
     char* wl = smem_all + w * (KS > 1 ? MERGE : out_wave_bytes<NDT>());   // this wave's own area
     const __amdgpu_buffer_rsrc_t orr = make_rsrc(P.o + cs * P.o_st + h * P.o_sh, rows_bytes(L, P.o_st, D));
@@ -457,6 +513,12 @@ __global__ __launch_bounds__(NT * KS, KS > 1 ? 2 : HD == 64 ? 4 : 3) void prefix
       const __amdgpu_buffer_rsrc_t lor =
           make_rsrc(P.o_lo + cs * P.lo_st + h * P.lo_sh, rows_bytes(L, P.lo_st, D, 1));
       store_lo_rows_via_lds<NDT, 2>(oacc, inv, wl, lor, qw0, (uint32_t)P.lo_st, lane);
+    }
+  }
+  if constexpr (UNIFORM) {
+    if (redo) {
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "agent");   // behind the rows' stores
+      redo_rows(P, redo, qw0, cs, h, L, p);
     }
   }
   if (!UNIFORM && wave_active && hh == 0 && qi < L) P.lse[(int64_t)h * P.T + cs + qi] = (m_run + __builtin_log2f(lt)) * kLn2;
