@@ -124,7 +124,8 @@ __device__ __forceinline__ float block_scale(uint32_t mag) {
 // a dozen (the rounding of 2 x 16 x 1021 rows 11.2 -> 9.4 us): y = 1 / s rounded
 // (one Newton step from the 1-ulp reciprocal), q = x y, and q + (x - q s) y rounds to x / s as long as
 // the residual x - q s is exact, which a scale below 2^-60 is multiplied up for. Scales and rows come
-// from bf16, so there are 128 mantissas of each: the tests take them all.
+// from bf16, so there are 128 mantissas of each: the tests take them all. By an infinite scale, whose
+// steps would end in 0 * inf, finite x give 0 and others NaN: s = y = 0.
 struct Divisor {
   float s, y, up;
   __device__ __forceinline__ explicit Divisor(float scale) {
@@ -132,6 +133,7 @@ struct Divisor {
     s = scale * up;
     const float y0 = __builtin_amdgcn_rcpf(s);
     y = __builtin_fmaf(__builtin_fmaf(-s, y0, 1.f), y0, y0);
+    if (scale == INFINITY) s = y = 0.f;
   }
   __device__ __forceinline__ float divides(float x) const {
     x *= up;
