@@ -466,14 +466,14 @@ __device__ __forceinline__ void extend_block_valu(const Params& P, int b, int h,
 // 16 staged rows is either codes or bf16 rows, and the 32 keys that a wave multiplies at a time
 // have one scale, as blocks begin at multiples of 64.
 //
-// The probabilities go into P V as two bf16 terms, each cut: that leaves less than 2^-15 of each, and on
-// average 2^-17 of the sum of p |v|, 2^-8 of what the output's rounding to bf16 does and less than the
-// rows' own rounding to 8 bits (a third term took 0.8 us of 26.6 for 4 x 16 heads x 45 queries on 2000
-// rows).
-// Bound by each wave's chain of LDS, products and exponentials, 1.7 us a tile of 64 keys and 64
-// queries (45 of them on 4051 keys of 64 pairs 33 us, with a cache in bf16 42): fewer address
-// operations change nothing.
-constexpr int kTerms = 2;
+// The probabilities, times the values' scale, go into P V as three bf16 terms, which add up to the 24 bits
+// of the fp32 value, as in kvcache.h. Two, each cut, take less (4 x 16 heads x 45 queries on 2000 rows 24.2
+// us, with three 25.5; 2 x 12 x 256 on 10500 84.3 and 94.2) but leave up to 2^-15 of each probability, all
+// towards zero, which sums that cancel show.
+// Bound by each wave's chain of LDS, products and exponentials (45 queries of 64 pairs on 2000 rows 25.5 us,
+// on 4000 35.2), and for few tiles by what a split costs once: its first loads, the join of the key groups,
+// its partials and their combine. Fewer address operations change nothing.
+constexpr int kTerms = 3;
 template <class C, int QW>
 __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
   using G = ExtGeo<QW>;
