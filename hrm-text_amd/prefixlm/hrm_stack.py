@@ -333,7 +333,10 @@ class HRMStack(nn.Module):
             return token_logprobs(logits, targets, entropy=entropy, top_k=top_k, ignore_index=ignore_index)
         logp = torch.log_softmax(logits.float(), -1)
         counted = targets != ignore_index
-        lp = torch.where(counted, logp.gather(-1, torch.where(counted, targets, 0)[..., None])[..., 0], 0.0)
+        inside = (targets >= 0) & (targets < logp.shape[-1])
+        lp = logp.gather(-1, torch.where(inside, targets, 0).long()[..., None])[..., 0]
+        # NaN, its gradient too, for a target outside the vocabulary
+        lp = torch.where(counted, lp * torch.where(inside | ~counted, 1.0, math.nan), 0.0)
         ent = -(logp.exp() * logp).sum(-1) if entropy else None
         top = torch.sort(logp, dim=-1, descending=True, stable=True) if top_k else None
         return TokenLogprobs(lp, ent, top.values[..., :top_k] if top_k else None, top.indices[..., :top_k] if top_k else None)
