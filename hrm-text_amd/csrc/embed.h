@@ -1,10 +1,12 @@
 // Scaled embedding lookup and the gradient of its table (models/lm_head.py:34-43).
 //
-//   y_i = round(s * T[id_i]),   dT_v = round(s * sum over i with id_i = v, in the order of i, of dy_i)
+//   y_i = round(s * T[id_i]),   dT_v = round(s * sum over i with id_i = v of dy_i)
 //
-// The gradient needs the tokens grouped by id: a stable radix sort of (id, i), then one pass over
-// the sorted tokens that adds the rows of each run in fp32. Stable, so every sum has one order and
-// the result is bitwise deterministic; no atomics touch floating-point data.
+// The gradient needs the tokens grouped by id: a stable sort of (id, i), then one pass over the sorted
+// tokens that adds the rows of each run in fp32, a chunk of 16 or 32 tokens by a wave, and a second one
+// that adds the sums of a run over several chunks, in order. The sort is stable, so the sums have one order
+// for the same ids and the result is bitwise deterministic; no atomics touch floating-point data. Where a
+// run meets the chunks' borders, and so the order within it, depends on the tokens that sort before it.
 #pragma once
 #include "common.h"
 

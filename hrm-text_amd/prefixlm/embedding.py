@@ -3,8 +3,8 @@
 The reference's head looks its tokens up in a table and multiplies the rows by a scale
 (models/lm_head.py:34-43). ``embedding`` does both in one pass, from a bf16 or fp32 table
 into bf16 or fp32 rows with one rounding. The backward sorts the tokens by id and adds each
-id's rows in fp32 in the tokens' order, so that the gradient is bitwise the same every time,
-and writes the whole table's gradient, zero rows included.
+id's rows in fp32, chunk by chunk of the sorted tokens, so that the gradient is bitwise the same
+every time, and writes the whole table's gradient, zero rows included.
 """
 from __future__ import annotations
 
@@ -110,8 +110,10 @@ def embedding(ids: Tensor, table: Tensor, scale: float = 1.0, *, dtype: Optional
 
     ``dtype`` (bf16 or fp32, default the table's) is the rows' type; the product is rounded once.
     An id outside the table gives a row of NaN and no gradient. ``padding_idx``: this id's rows add
-    nothing to the gradient. The table's gradient is dense, in its type, added in fp32 in the
-    tokens' order."""
+    nothing to the gradient. The table's gradient is dense, in its type. It is added in fp32: the
+    tokens are sorted by id, those of one id in their order, and each 16 or 32 sorted ones are added one
+    after another, then their sums in order. The same call gives the same bits; other ids' tokens move
+    an id's place among the sorted ones, and with it its last bits."""
     scale, dtype = float(scale), table.dtype if dtype is None else dtype
     if padding_idx is not None and not 0 <= padding_idx < table.shape[0]:
         raise ValueError(f"padding_idx must be in [0, {table.shape[0]}) (got {padding_idx})")

@@ -448,7 +448,10 @@ int prefixlm_logprob_bwd(const prefixlm_logprob_args* args, void* stream);
 /* Scaled embedding lookup (models/lm_head.py:34-43) and the gradient of its table.
  * Forward: y[i] = scale * table[ids[i]], fp32 product, one rounding; ids outside [0, vocab) give
  * NaN rows. Backward: grad[v] = scale * sum of dy[i] over the tokens with ids[i] = v, added in fp32
- * in the order of i and rounded once; the whole [vocab, cols] gradient is written, zero where no
+ * and rounded once: the tokens are sorted by id, those of one id in the order of i, and cut into chunks of
+ * 16 or 32; a chunk adds an id's rows one after another, then the chunks' sums are added in their order. So
+ * an id's last bits also depend on how many tokens sort before it; the same call gives the same bits. The
+ * whole [vocab, cols] gradient is written, zero where no
  * token is. Ids outside the table and padding_id (negative: none) have no gradient. Bitwise
  * deterministic. table and grad, and y and dy, bf16 or fp32; ids int64, or int32 with ids_int32.
  * Unit column stride, cols % 8 == 0, rows 16-byte aligned; grad contiguous; vocab < 2^27. */
