@@ -7,8 +7,9 @@
 //                           or NaN gets such a scale
 //   recent  [128, 128]      bf16: row j of the last 64 to 127 rows in slot j % 128, as given
 // A row is rounded to 8 bits once, from its bf16 value, when its block is complete, so the cache's
-// content does not depend on how many rows each call brought. The ring also lets a caller take
-// back up to 64 rows: the rows of the block that is incomplete again are still there.
+// content does not depend on how many rows each call brought. The ring also lets a caller take rows
+// back, to one block before the incomplete one of the furthest length that the cache has had: the rows of
+// the block that is incomplete again are still there. A multiple of 64 reads no ring rows.
 //
 // A call with len rows in the cache attends: rows below len / 64 * 64 from the codes, the rest
 // below len from the ring, and the call's new rows as given, so nothing reads what the call writes.

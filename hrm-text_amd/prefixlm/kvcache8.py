@@ -9,8 +9,12 @@ A row is attended in bf16 while its block of 64 is incomplete, and by the call t
 When its block is complete the block is rounded once, straight from bf16: the scale is the block's
 largest magnitude times the fp32 value of 1/448 (e4m3) or 1/127 (int8), at least 2^-126, and
 ``code = round(row / scale)``, to nearest, ties to even. So what the cache holds does not depend on how many rows each call
-brought. The last 64 to 127 rows stay in bf16 as well: a caller may take back up to 64 rows
-(rejected draft tokens) by passing a smaller length.
+brought. The last 64 to 127 rows stay in bf16 as well: a caller may take rows back (rejected draft
+tokens) by passing a smaller length. How far counts from the furthest length that the cache has had,
+taken back since or not: to ``furthest // 64 * 64 - 64`` (64 rows at least). Below that the bf16 rows have
+been overwritten, which the call cannot see; only a multiple of 64, 0 among them, needs none of them and
+may be gone back to at any time. The furthest length then counts anew, and what lies below that
+multiple is reached at multiples of 64 only.
 """
 from __future__ import annotations
 

@@ -376,8 +376,12 @@ int prefixlm_kvcache_fwd(const prefixlm_kvcache_args* args, void* stream);
  * len - 1 from k_recent, v_recent, the call's new rows as given. Afterwards the blocks that the new
  * rows complete are rounded: scale = max(largest magnitude times the fp32 value of 1/448 (e4m3) or
  * 1/127 (int8), 2^-126), code = round(row / scale) to nearest, ties to even; and the new rows among the
- * last 64 before the incomplete block and those in it are written to k_recent, v_recent. So up to 64
- * rows can be taken back by calling with a smaller len. Lengths outside [0, Smax] count as the nearest
+ * last 64 before the incomplete block and those in it are written to k_recent, v_recent. So rows can be
+ * taken back by calling with a smaller len: to max_len / 64 * 64 - 64 or more, where max_len is the furthest
+ * length that the cache has had, taken back since or not (64 rows at least; the kernels do not know max_len,
+ * and below that read bf16 rows that later ones have overwritten), or to any multiple of 64, which reads
+ * none: max_len then counts anew, and what lies below that multiple is reached at multiples of 64 only.
+ * Lengths outside [0, Smax] count as the nearest
  * of the two. The cache's tensors overlap neither each other nor q, k, v and out. */
 typedef struct prefixlm_kvcache8_args {
   const void* q;

@@ -165,3 +165,23 @@ def test_rows_taken_back_from_the_furthest_length(furthest, dtype):
         n = min(furthest - at, n)
         bring(at, _rows(g, 1, n, H, 128), _rows(g, 1, n, H, 128))
         end = at + n
+
+
+def test_back_to_a_whole_block_and_on():
+    """Far below the window, to multiples of 64: from there the window counts anew."""
+    H, Smax, dtype = 1, 512, torch.int8
+    g = torch.Generator().manual_seed(5)
+    k, v = (_rows(g, 1, Smax, H, 128) for _ in range(2))
+    k2, v2 = (_rows(g, 1, Smax, H, 128) for _ in range(2))
+    got, want = kvcache_q8(1, Smax, H, dtype=dtype), kvcache_q8(1, Smax, H, dtype=dtype)
+
+    def call(cache, at, n, k, v):
+        d = [x[:, at:at + n].to(DEV) for x in (k, k, v)]
+        return flash_attn_with_kvcache_q8(d[0], cache, d[1], d[2], torch.tensor([at], dtype=torch.int32, device=DEV), causal=True)
+
+    call(got, 0, 300, k, v)
+    call(want, 0, 128, k, v)
+    for at, n in ((128, 5), (133, 64), (197, 30), (130, 3), (133, 1)):      # 130: two blocks below 227's is 128
+        assert torch.equal(call(got, at, n, k2, v2), call(want, at, n, k2, v2)), at
+    call(want, 0, 64, k, v)
+    assert torch.equal(call(got, 64, 9, k2, v2), call(want, 64, 9, k2, v2))
