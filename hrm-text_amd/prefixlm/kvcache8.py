@@ -152,7 +152,9 @@ def flash_attn_with_kvcache_q8(q: Tensor, cache: KVCacheQ8, k: Optional[Tensor] 
     """Attention of q [B, S, H, 128] bf16 over an 8-bit cache, which takes the new rows k, v
     [B, S, H, 128] (or None: the cache only) behind its first ``cache_seqlens`` rows (an int, or int32
     [B] on the GPU, where values outside [0, Smax] count as the nearest of the two; None = 0). Rows
-    past the cache's end are dropped. ``causal``: query i sees keys j <= rows - S + i, as in
+    past the cache's end are dropped. A prompt into an empty cache (the int 0 or None) runs the training
+    forward, which rounds the probabilities to bf16; with a tensor of zeros, as in every other call, they
+    keep their fp32 bits. ``causal``: query i sees keys j <= rows - S + i, as in
     ``flash_attn_with_kvcache``. A query that sees no key gives a row of 0. Forward only: the call has
     no gradient."""
     if cache_seqlens is None:

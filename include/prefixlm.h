@@ -336,8 +336,9 @@ int prefixlm_proj_gemm_scaled(const prefixlm_proj_gemm_args* args, void* stream)
  * lk = min(Smax, len_b + S) cache keys (lk = min(Smax, len_b) without new rows), with
  * is_causal only keys j <= lk - S + i (bottom-right aligned). out: bf16 [B, S, H, D].
  * A call with cache_seqlens NULL and cache_seqlen 0 (the reference's prefill) runs the
- * varlen forward kernels over the new rows; every other call runs a split-K decode
- * kernel. All tensors have unit stride over D and element strides (batch, seq, head). */
+ * varlen forward kernel over the new rows, which rounds the probabilities to bf16, where they are
+ * packed, fit the cache and that kernel's 32-bit offsets ((S + 256) token strides below 2 GiB), and
+ * softmax_scale is positive; every other call runs a split-K decode or extend kernel. All tensors have unit stride over D and element strides (batch, seq, head). */
 typedef struct prefixlm_kvcache_args {
   const void* q;
   const void* k;                 /* new rows, or NULL (k and v together): attend the cache only */
@@ -376,7 +377,11 @@ int prefixlm_kvcache_fwd(const prefixlm_kvcache_args* args, void* stream);
  * len - 1 from k_recent, v_recent, the call's new rows as given. Afterwards the blocks that the new
  * rows complete are rounded: scale = max(largest magnitude times the fp32 value of 1/448 (e4m3) or
  * 1/127 (int8), 2^-126), code = round(row / scale) to nearest, ties to even; and the new rows among the
- * last 64 before the incomplete block and those in it are written to k_recent, v_recent. So rows can be
+ * last 64 before the incomplete block and those in it are written to k_recent, v_recent. (In a block that
+ * holds infinities or NaN their codes are e4m3's NaN, or int8 0, beside a scale that says so.) A prompt into an
+ * empty cache, given by cache_seqlen = 0 and packed, runs the training forward as in prefixlm_kvcache_fwd,
+ * which rounds the probabilities to bf16 (about 2^-9 of the sum of p |v|); every other call keeps their fp32
+ * bits. Rows can be
  * taken back by calling with a smaller len: to max_len / 64 * 64 - 64 or more, where max_len is the furthest
  * length that the cache has had, taken back since or not (64 rows at least; the kernels do not know max_len,
  * and below that read bf16 rows that later ones have overwritten), or to any multiple of 64, which reads
