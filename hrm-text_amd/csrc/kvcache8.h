@@ -471,9 +471,11 @@ __device__ __forceinline__ void extend_block_valu(const Params& P, int b, int h,
 // of the fp32 value, as in kvcache.h. Two, each cut, take less (4 x 16 heads x 45 queries on 2000 rows 24.2
 // us, with three 25.5; 2 x 12 x 256 on 10500 84.3 and 94.2) but leave up to 2^-15 of each probability, all
 // towards zero, which sums that cancel show.
-// Bound by each wave's chain of LDS, products and exponentials (45 queries of 64 pairs on 2000 rows 25.5 us,
-// on 4000 35.2), and for few tiles by what a split costs once: its first loads, the join of the key groups,
-// its partials and their combine. Fewer address operations change nothing.
+// Bound by each wave's chain of LDS, products and exponentials, and for few tiles by what a split costs
+// once: its first loads, the join of the key groups, its partials. 64 pairs x 45 queries, ten splits: on 2000
+// rows 21.8 us, on 4000 33.4, so 11.6 for each 2000 rows and 10 besides, and the combine 4.6; 24 x 100, 21
+// splits: on 5250 rows 29.7, on 10500 46.1, 16.4 for each 5250 and 13 besides, combine 6.9, append 4.9; 24 x
+// 256, ten splits: 52.9 and 86.8, 34 and 19, 8.7, 5.1. Fewer address operations change nothing.
 constexpr int kTerms = 3;
 template <class C, int QW>
 __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
@@ -531,7 +533,7 @@ __global__ __launch_bounds__(NT, 2) void extend_kernel(Params P) {
   // of a code row's, and a bf16 row the others. So no register is written on two paths, and all loads
   // of a tile are on their way together until the tile is stored (as 16 bytes on two paths, with
   // zeroed registers past k1, every 16 rows waited for those before them: 4 x 16 heads x 45 queries on
-  // 2000 rows 28.0 us, now 24.3; 16 x 16 x 32 on 2157 92.8 and 61.8).
+  // 2000 rows 28.0 us, so 24.3; 16 x 16 x 32 on 2157 92.8 and 61.8; both with two terms of P).
   // pointers that meet from two paths have to say that they are of global memory, or the loads do not know
   typedef const __attribute__((address_space(1))) char* gbytes;
   typedef const __attribute__((address_space(1))) u32x2* gu32x2;

@@ -218,8 +218,9 @@ __device__ __forceinline__ void finish_row(const Params& P, int64_t row, const S
 // is reached by at least k elements, so only the groups of a thread's vectors whose largest reaches it
 // are looked at again, one vector a thread (by the thread that holds the group, a round trip to memory
 // for each: 4 x 65536 with 20 alternatives 14.8 us, now 11.0); the elements that reach it, mostly few
-// more than k, are ranked against each other. Where they do not fit (rows of many equal values), or a NaN
-// is among them, which the maxima pass over, a walk finds the next largest k times.
+// more than k, are ranked against each other. Where they do not fit (rows of many equal values, or of fewer
+// finite logits than alternatives), or a NaN is among them, which the maxima pass over, a walk finds the next
+// largest k times (4 x 65536 with ten finite logits and 20 alternatives 164 us).
 template <class T, bool ENT, bool TOP>
 __global__ __launch_bounds__(NT) void forward_kernel(Params P) {
   __shared__ Stat s_stat[NT / 64];

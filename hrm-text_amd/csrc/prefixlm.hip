@@ -1684,9 +1684,10 @@ int prefixlm_embedding_bwd(const prefixlm_embedding_args* a, void* stream_) {
 // ---- attention over an 8-bit cache -----------------------------------------------------------
 // Splits of the keys. Several queries: as for bf16 (the tiles are the same), but above six splits no
 // more than 512 workgroups, as a second round of a few costs more than the longer splits (24 units x
-// 10569 keys of 2 rows, 100 queries, 71.8 us with 22 splits, 53.5 with 21; 60 x 4006, 90 queries 60.9
-// and 49.8; with fewer splits ragged rows want the more: 120 units x 4178 keys 94.7 with five, 110 with
-// four). One query:
+// 10569 keys, 100 queries, 67.7 us with 22 splits, 51 with 21, of ragged rows 63.8 and 47.4; 60 x 4006, 90
+// queries 63.5 and 50.7, ragged 62.9 and 53.8). Not from five splits down, where it depends on the rows: 120
+// units x 4178 keys of ragged rows took 95 with five and 110 with four in one batch, 101 and 92 in another
+// (90 queries), 66 and 58 (45). One query:
 // one split for caches of up to 1536 rows, whose keys take less time than the combine's launch (16
 // pairs x 920 of 1536 rows 8.7 us, 11.3 with three splits; 128 x 800 of 1024 9.9 and 12.8; 64 x 1800
 // of 2048 14.8, 13.2 with four), and from 192 pairs on, one for each CU nearly (256 x 12288 of 16384
@@ -1822,6 +1823,9 @@ int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* a, void* stream_) {
     return fail(PREFIXLM_ERR_INVALID, "grid too large");
   (void)hipGetLastError();
   if (prefill) {
+    // the training forward, whose probabilities are rounded to bf16 (2^-9 of each, half the output's own
+    // rounding): the extend kernel, which keeps their fp32 bits, takes twice as long (2 x 1021 rows x 16
+    // heads 84 us, so 37; 4 x 4100 x 16 1298 and 625)
     set_kernel_attrs();
     if (g_attr_err != hipSuccess)
       return fail(PREFIXLM_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(g_attr_err));
