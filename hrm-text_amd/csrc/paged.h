@@ -1,0 +1,459 @@
+// Attention over a key-value cache in pages.
+//
+// One layer's pool is [P, Hkv, ps, D] for the keys and the same for the values: P pages of ps rows (a
+// power of two from 16 to 1024), a page's rows of one head contiguous. A table [N, M] gives column c of
+// sequence n the page of its rows c ps .. c ps + ps - 1; an entry outside [0, P) is no page. refs[p] is how
+// many entries hold page p. Query head h belongs to key-value head h / G, G = Hq / Hkv.
+//
+// A call with len rows in sequence b and S new ones attends, for query i, keys j < n_i: with
+// lk = min(M ps, len + s_new), n_i = lk, or with `causal` min(lk, len + s_new - S + i + 1). Keys below
+// len come from the pages, and rows without a page are not seen; keys from len on are the call's own rows,
+// as given, so nothing reads what the call writes. New rows are stored in pages that the sequence holds
+// alone (refs 1); others are not stored.
+//
+// The G query heads of a key-value head and the S queries are the R = S G rows that share its keys: row
+// r is query r / G of head h G + r % G. Kernels:
+//   stream  : 16 RT rows a workgroup, split over the keys. Each wave walks 32 keys at a time by itself,
+//             K as it lies in memory into the matrix cores, V through LDS of its own;
+//   combine : joins the splits.
+#pragma once
+#include "common.h"
+#include "kvcache.h"
+
+namespace prefixlm {
+namespace pkv {
+
+using kvc::max_mag;
+using kvc::max_ref;
+
+constexpr int NT = 256;
+constexpr int NWAVE = NT / 64;
+constexpr int kKeys = 32;          // keys of a wave's step
+constexpr int kMaxSplits = 64;
+// floats per partial: max (log2 units), sum, whether a key was seen, unused, o[D]
+template <int D>
+constexpr int kPart = D + 4;
+
+struct Params {
+  const bf16* q;
+  const bf16* k;           // new rows (may be null)
+  const bf16* v;
+  bf16* kp;                // the layer's pages
+  bf16* vp;
+  const int32_t* refs;     // [P]
+  const int32_t* table;    // [B, M]
+  bf16* out;
+  float* part;             // [B, Hkv, R, nsplit, kPart]
+  const int32_t* seqlens;  // device [B]; null: every sequence has seqlen_const
+  int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh, table_sb;
+  int B, S, Hkv, G, P, cap, ps_log2, nsplit, causal, seqlen_const;
+  int s_new;               // rows appended by this call: S, or 0 without new k, v
+  int nrb;                 // row blocks
+  float scale_log2;
+};
+
+// Read-only data at addresses that are the same for a whole wave: through the scalar cache
+typedef const __attribute__((address_space(4))) int32_t uniform_i32;
+__device__ __forceinline__ uniform_i32* uniform(const int32_t* p) { return (uniform_i32*)(uintptr_t)p; }
+
+__device__ __forceinline__ int cache_len(const Params& P, int b) {
+  return min(max(P.seqlens ? P.seqlens[b] : P.seqlen_const, 0), P.cap);
+}
+// The keys that query i sees of a sequence of length len: [0, n)
+__device__ __forceinline__ int keys_seen(const Params& P, int len, int i) {
+  const int lk = min(P.cap, len + P.s_new);
+  return P.causal ? min(lk, len + P.s_new - P.S + i + 1) : lk;
+}
+// 1 / (sum of the weights): a row that sees no key is 0, one whose scores are all -inf NaN
+__device__ __forceinline__ float row_inv(bool seen, float sum) { return seen ? 1.f / sum : 0.f; }
+
+// D(16x16 f32) += A(16x32 bf16) B(32x16 bf16). Lane l holds A[l%16][8 (l/16) + 0..7] and
+// B[8 (l/16) + 0..7][l%16]; register r of the result is D[4 (l/16) + r][l%16].
+__device__ __forceinline__ f32x4 mfma16x16x32(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// max / sum over lanes l, l ^ 16, l ^ 32 and l ^ 48
+__device__ __forceinline__ float rows_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return halves_max(x);
+}
+__device__ __forceinline__ float rows_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return halves_sum(x);
+}
+
+// This workgroup's share of the new rows of (b, h), part `part` of `parts`, into their pages
+template <int D>
+__device__ __forceinline__ void append_share(const Params& P, int b, int h, int len, int part, int parts) {
+  constexpr int CH = D / 8;   // 16-byte chunks of a row
+  const int c = 8 * (threadIdx.x % CH), is_v = (threadIdx.x / CH) & 1;
+  for (int i = part + parts * (threadIdx.x / (2 * CH)); i < P.s_new; i += parts * (NT / (2 * CH))) {
+    const int j = len + i;
+    if (j >= P.cap) break;
+    const int page = P.table[b * P.table_sb + (j >> P.ps_log2)];
+    if ((unsigned)page >= (unsigned)P.P || P.refs[page] != 1) continue;
+    const int64_t at = ((((int64_t)page * P.Hkv + h) << P.ps_log2) + (j & ((1 << P.ps_log2) - 1))) * D + c;
+    if (is_v)
+      *reinterpret_cast<u32x4*>(P.vp + at) = *reinterpret_cast<const u32x4*>(P.v + b * P.v_sb + i * P.v_ss + h * P.v_sh + c);
+    else
+      *reinterpret_cast<u32x4*>(P.kp + at) = *reinterpret_cast<const u32x4*>(P.k + b * P.k_sb + i * P.k_ss + h * P.k_sh + c);
+  }
+}
+
+// Rows [r0, r1) over keys [k0, k1) without the matrix cores: 16 lanes a row, key by key. For splits
+// whose values hold an infinity or NaN (0 * inf in P V would reach rows that must not see the key), and
+// for scores that pass fp32's range before the softmax scale, or whose largest is about -3e38: here the
+// scale comes first.
+template <int D>
+__device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int split, int r0, int r1, int k0, int k1, int len) {
+  constexpr int E = D / 16;
+  const int g16 = threadIdx.x & 15;
+  const int R = P.S * P.G;
+  auto get = [&](const bf16* p, float* f) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = (float)p[E * g16 + e];
+  };
+#pragma unroll 1
+  for (int r = r0 + (threadIdx.x >> 4); r < r1; r += NT / 16) {
+    const int i = r / P.G, hq = h * P.G + r % P.G;
+    float q[E], o[E], x[E];
+    get(P.q + b * P.q_sb + i * P.q_ss + hq * P.q_sh, q);
+#pragma unroll
+    for (int e = 0; e < E; ++e) q[e] *= P.scale_log2, o[e] = 0.f;
+    float m = -INFINITY, l = 0.f, seen = 0.f;
+#pragma unroll 1
+    for (int j = k0; j < min(k1, keys_seen(P, len, i)); ++j) {
+      const bf16 *kr, *vr;
+      if (j < len) {
+        const int page = P.table[b * P.table_sb + (j >> P.ps_log2)];
+        if ((unsigned)page >= (unsigned)P.P) continue;
+        const int64_t at = ((((int64_t)page * P.Hkv + h) << P.ps_log2) + (j & ((1 << P.ps_log2) - 1))) * D;
+        kr = P.kp + at;
+        vr = P.vp + at;
+      } else {
+        kr = P.k + b * P.k_sb + (j - len) * P.k_ss + h * P.k_sh;
+        vr = P.v + b * P.v_sb + (j - len) * P.v_ss + h * P.v_sh;
+      }
+      seen = 1.f;
+      get(kr, x);
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += q[e] * x[e];
+      s = row16_sum(s);
+      const float mx = fmaxf(m, s), ref = max_ref(mx);
+      const float alpha = __builtin_amdgcn_exp2f(m - ref), p = __builtin_amdgcn_exp2f(s - ref);
+      m = mx;
+      l = l * alpha + p;
+      get(vr, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + p * x[e];
+    }
+    if (P.nsplit == 1) {
+      const float inv = row_inv(seen != 0.f, l);
+      bf16* dst = P.out + b * P.o_sb + i * P.o_ss + hq * P.o_sh + E * g16;
+#pragma unroll
+      for (int e = 0; e < E; ++e) dst[e] = (bf16)(o[e] * inv);
+    } else {
+      float* dst = P.part + ((((int64_t)b * P.Hkv + h) * R + r) * P.nsplit + split) * kPart<D>;
+      if (g16 == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{m, l, seen, 0.f};
+#pragma unroll
+      for (int e = 0; e < E; ++e) dst[4 + E * g16 + e] = o[e];
+    }
+  }
+}
+
+template <int D>
+struct Geo {
+  static constexpr int NS = D / 32;              // steps of the contraction over d
+  static constexpr int ND = D / 16;              // 16-column tiles of o; 16-byte loads a lane of K, and of V
+  static constexpr int CH = D / 8;               // 16-byte chunks of a row
+  static constexpr int RPL = 64 / CH;            // V rows a load
+  // V rows in LDS: 8 rows apart by 8 banks each, so that the 32 lanes of a transposing read's cycle, 8
+  // rows of 32 bytes, take all 64 banks
+  static constexpr int VS = 2 * D + 32;
+  static constexpr int OS = D + 4;               // floats of a row of o where the waves meet
+  static constexpr int AREA = kKeys * VS > 16 * OS * 4 ? kKeys * VS : 16 * OS * 4;   // bytes a wave
+};
+
+// blockIdx.x: row blocks of one (b, h, split) eight indices apart, on one XCD.
+template <int D, int RT>
+__global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
+  using G = Geo<D>;
+  constexpr int NS = G::NS, ND = G::ND, CH = G::CH, HL = ND / 2;   // HL: V loads of 16 keys
+  __shared__ __attribute__((aligned(16))) char smem[NWAVE][G::AREA];
+  __shared__ float s_m[NWAVE][16], s_l[NWAVE][16], s_seen[NWAVE][16];
+  __shared__ int s_bad;
+  const int rb = (blockIdx.x >> 3) % P.nrb;
+  const int unit = (int)((blockIdx.x >> 3) / P.nrb) * 8 + (blockIdx.x & 7);
+  if (unit >= P.B * P.Hkv * P.nsplit) return;
+  const int split = unit % P.nsplit, bh = unit / P.nsplit;
+  const int h = bh % P.Hkv, b = bh / P.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int R = P.S * P.G, r0 = rb * 16 * RT, r1 = min(R, r0 + 16 * RT);
+  const int len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
+  const int lk = min(P.cap, len + P.s_new);
+  // the splits share a sequence's own keys, in whole steps
+  const int per = ((lk + P.nsplit - 1) / P.nsplit + kKeys - 1) / kKeys * kKeys;
+  const int k0 = split * per;
+  const int k1 = min(k0 + per, keys_seen(P, len, (r1 - 1) / P.G));   // the last row sees the most
+  const int kall = keys_seen(P, len, r0 / P.G);                      // every row sees the keys below
+  if (tid == 0) s_bad = 0;
+
+  uniform_i32* const tab = uniform(P.table + b * P.table_sb);
+  const int psm = (1 << P.ps_log2) - 1;
+  const bf16* const kn = P.s_new ? P.k + b * P.k_sb + h * P.k_sh : nullptr;
+  const bf16* const vn = P.s_new ? P.v + b * P.v_sb + h * P.v_sh : nullptr;
+  char* const area = smem[w];
+
+  u32x4 kw[ND], vw[ND];
+  bool ok[2];              // the 16 keys have a page, or are new rows
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  // K: lane holds key l16 of each 16, columns 32 s + 8 g4 + 0..7; V: rows of CH lanes
+  const uint32_t koff = (uint32_t)(l16 * D + 8 * g4) * 2, voff = (uint32_t)(lane / CH * D + 8 * (lane % CH)) * 2;
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int j = j0 + 16 * hf;
+      const int page = j < len ? tab[j >> P.ps_log2] : -1;
+      const bool held = (unsigned)page < (unsigned)P.P;
+      const int64_t at = ((((int64_t)(held ? page : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
+      const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
+      ok[hf] = held;
+      if (held && j + 16 <= min(len, lk)) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) kw[hf * NS + s] = kvc::load_once(reinterpret_cast<const bf16*>(kb + koff + 64 * s));
+#pragma unroll
+        for (int u = 0; u < HL; ++u)
+          vw[hf * HL + u] = kvc::load_once(reinterpret_cast<const bf16*>(vb + voff + u * (G::RPL * D * 2)));
+      } else {
+        // the last cached rows, the new ones, none: row by row
+        {
+          const int jk = j + l16;
+          const char* p = jk < len ? (held ? kb + koff : nullptr)
+                                   : (jk < lk ? reinterpret_cast<const char*>(kn + (jk - len) * P.k_ss + 8 * g4) : nullptr);
+#pragma unroll
+          for (int s = 0; s < NS; ++s) kw[hf * NS + s] = p ? *reinterpret_cast<const u32x4*>(p + 64 * s) : zero;
+        }
+#pragma unroll
+        for (int u = 0; u < HL; ++u) {
+          const int jv = j + u * G::RPL + lane / CH;
+          const char* p = jv < len ? (held ? vb + voff + u * (G::RPL * D * 2) : nullptr)
+                                   : (jv < lk ? reinterpret_cast<const char*>(vn + (jv - len) * P.v_ss + 8 * (lane % CH)) : nullptr);
+          vw[hf * HL + u] = p ? *reinterpret_cast<const u32x4*>(p) : zero;
+        }
+      }
+    }
+  };
+
+  float m_run[RT], l_run[RT], seen[RT];
+  f32x4 oacc[RT][ND];
+  int nlim[RT];            // this lane's row sees keys below, of this split
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    m_run[t] = -INFINITY, l_run[t] = 0.f, seen[t] = 0.f;
+    nlim[t] = min(k1, keys_seen(P, len, min(r0 + 16 * t + l16, R - 1) / P.G));
+#pragma unroll
+    for (int d = 0; d < ND; ++d) oacc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  u16x2 vmag = {0, 0};
+
+  int j0 = k0 + kKeys * w;
+  if (j0 < k1) {
+    load(j0);
+    // Q^T: lane holds row l16, columns 32 s + 8 g4 + 0..7 (rows past the last: that one, not stored)
+    bf16x8 qf[RT][NS];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = min(r0 + 16 * t + l16, R - 1);
+      const bf16* qp = P.q + b * P.q_sb + (r / P.G) * P.q_ss + (h * P.G + r % P.G) * P.q_sh + 8 * g4;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qf[t][s] = *reinterpret_cast<const bf16x8*>(qp + 32 * s);
+    }
+    const char* const vt = area + (4 * g4 + (l16 >> 2)) * G::VS + 8 * (l16 & 3);
+    for (; j0 < k1; j0 += kKeys * NWAVE) {
+      f32x4 s[RT][2];
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          s[t][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int n = 0; n < NS; ++n) s[t][hf] = mfma16x16x32(__builtin_bit_cast(bf16x8, kw[hf * NS + n]), qf[t][n], s[t][hf]);
+        }
+#pragma unroll
+      for (int u = 0; u < ND; ++u) {
+        vmag = max_mag(vmag, vw[u]);
+        *reinterpret_cast<u32x4*>(area + (u * G::RPL + lane / CH) * G::VS + 16 * (lane % CH)) = vw[u];
+      }
+      // a page that is missing hides cached keys only
+      const bool ok0 = ok[0], ok1 = ok[1];
+      if (j0 + kKeys * NWAVE < k1) load(j0 + kKeys * NWAVE);
+      bf16x8 pt[RT][3];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[t][hf][r] *= P.scale_log2;   // before the mask: the scale may have any sign
+        if (j0 + kKeys > min(kall, k1) || !ok0 || !ok1) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int j = j0 + 16 * hf + 4 * g4 + r;
+              const bool sees = j < nlim[t] && ((hf ? ok1 : ok0) || j >= len);
+              seen[t] = sees ? 1.f : seen[t];
+              s[t][hf][r] = sees ? s[t][hf][r] : -INFINITY;
+            }
+        } else {
+          seen[t] = 1.f;
+        }
+        float mx = s[t][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[t][e >> 2][e & 3]);
+        mx = rows_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m_run[t]) != 0) {
+          const float m_new = fmaxf(m_run[t], mx);
+          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[t] - m_new);
+          m_run[t] = m_new;
+          l_run[t] *= alpha;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) oacc[t][d] *= alpha;
+        }
+        const float m_use = max_ref(m_run[t]);
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(s[t][i >> 2][i & 3] - m_use);
+          l_run[t] += e[i];
+        }
+        // the probabilities go into P V as three bf16 terms, which add up to their fp32 bits
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+          u32x4 x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[i] = pack_hi(__builtin_bit_cast(uint32_t, e[2 * i]), __builtin_bit_cast(uint32_t, e[2 * i + 1]));
+          pt[t][n] = __builtin_bit_cast(bf16x8, x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)   // exact
+            e[i] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, e[i]) & 0xffff0000u);
+        }
+      }
+      // V^T: lane holds column 16 d + l16 of keys 4 g4 + 0..3 and 16 + 4 g4 + 0..3, as s has them
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const u32x2 x0 = lds_read_tr(vt, 32 * d), x1 = lds_read_tr(vt, 16 * G::VS + 32 * d);
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{x0[0], x0[1], x1[0], x1[1]});
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int n = 0; n < 3; ++n) oacc[t][d] = mfma16x16x32(vf, pt[t][n], oacc[t][d]);
+      }
+    }
+  }
+
+  __syncthreads();   // s_bad is cleared
+  bool bad = vmag[0] >= 0x7f80 || vmag[1] >= 0x7f80;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    l_run[t] = rows_sum(l_run[t]);
+    // a score past the range upwards leaves NaN; one past it downwards (raw below -3.4e38) only counts
+    // where every key that the row sees here scores about as low
+    bad |= seen[t] != 0.f && (l_run[t] != l_run[t] || m_run[t] < 200.f - 3e38f * fabsf(P.scale_log2));
+    seen[t] = rows_max(seen[t]);
+  }
+  if (bad) s_bad = 1;
+  // the waves' results meet, 16 rows at a time
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    if (t) __syncthreads();
+    float* o = reinterpret_cast<float*>(area) + l16 * G::OS + 4 * g4;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(o + 16 * d) = oacc[t][d];
+    if (g4 == 0) s_m[w][l16] = m_run[t], s_l[w][l16] = l_run[t], s_seen[w][l16] = seen[t];
+    __syncthreads();
+    if (s_bad) break;
+    constexpr int E = D / 16;
+    const int row = tid >> 4, r = r0 + 16 * t + row;
+    if (r >= r1) continue;
+    float M = s_m[0][row], L = 0.f, any = 0.f, x[E];
+#pragma unroll
+    for (int g = 1; g < NWAVE; ++g) M = fmaxf(M, s_m[g][row]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = 0.f;
+#pragma unroll
+    for (int g = 0; g < NWAVE; ++g) {
+      const float wgt = s_m[g][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[g][row] - M);
+      L += wgt * s_l[g][row];
+      any = fmaxf(any, s_seen[g][row]);
+      const float* src = reinterpret_cast<const float*>(smem[g]) + row * G::OS + E * l16;
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(src + e);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[e + c] += wgt * y[c];
+      }
+    }
+    if (P.nsplit == 1) {
+      const float inv = row_inv(any != 0.f, L);
+      bf16* dst = P.out + b * P.o_sb + (r / P.G) * P.o_ss + (h * P.G + r % P.G) * P.o_sh + E * l16;
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        *reinterpret_cast<bf16x4*>(dst + e) = cvt4(x[e] * inv, x[e + 1] * inv, x[e + 2] * inv, x[e + 3] * inv);
+    } else {
+      float* dst = P.part + ((((int64_t)b * P.Hkv + h) * R + r) * P.nsplit + split) * kPart<D>;
+      if (l16 == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{M, L, any, 0.f};
+#pragma unroll
+      for (int e = 0; e < E; e += 4) *reinterpret_cast<f32x4*>(dst + 4 + E * l16 + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+    }
+  }
+  if (s_bad) walk_rows<D>(P, b, h, split, r0, r1, k0, k1, len);
+  append_share<D>(P, b, h, len, rb * P.nsplit + split, P.nrb * P.nsplit);
+}
+
+// One wave per (b, h, r): lane s weighs split s, then D / 4 lanes a split add their four columns.
+template <int D>
+__global__ __launch_bounds__(256) void combine_kernel(Params P) {
+  constexpr int L4 = D / 4, NG = 64 / L4;
+  const int R = P.S * P.G;
+  const int64_t u = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 6;
+  const int lane = threadIdx.x & 63, col = lane % L4, grp = lane / L4;
+  if (u >= (int64_t)P.B * P.Hkv * R) return;
+  const float* src = P.part + u * P.nsplit * kPart<D>;
+  const int n = P.nsplit;   // at most 64
+  f32x4 head = {-INFINITY, 0.f, 0.f, 0.f};
+  if (lane < n) head = *reinterpret_cast<const f32x4*>(src + lane * kPart<D>);
+  const float M = wave_max(head[0]);
+  const float wgt = head[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(head[0] - M);
+  float L = wgt * head[1];
+  const bool seen = __builtin_amdgcn_ballot_w64(head[2] != 0.f) != 0;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = grp; s0 < n + grp; s0 += 8 * NG) {
+    // eight loads in flight; past the last split its partial again, not added (it may be inf)
+    f32x4 o[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] = *reinterpret_cast<const f32x4*>(src + min(s0 + NG * x, n - 1) * kPart<D> + 4 + 4 * col);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int at = s0 + NG * x;
+      const f32x4 y = acc + __shfl(wgt, at & 63) * o[x];
+      acc = at < n ? y : acc;
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) L += __shfl_xor(L, m);
+#pragma unroll
+  for (int m = L4; m < 64; m <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], m);
+  const float inv = row_inv(seen, L);
+  const int r = (int)(u % R), bh = (int)(u / R), h = bh % P.Hkv, b = bh / P.Hkv;
+  if (grp == 0)
+    *reinterpret_cast<bf16x4*>(P.out + b * P.o_sb + (r / P.G) * P.o_ss + (h * P.G + r % P.G) * P.o_sh + 4 * col) =
+        cvt4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+}
+
+}  // namespace pkv
+}  // namespace prefixlm

@@ -27,6 +27,8 @@
 #include "gemm.h"
 #include "logprob.h"
 #include "embed.h"
+#include "paged.h"
+#include "pages.h"
 
 using namespace prefixlm;
 
@@ -1847,6 +1849,328 @@ int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* a, void* stream_) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "8-bit kv-cache launch: %s", hipGetErrorString(e));
   return PREFIXLM_OK;
+}
+
+}  // extern "C"
+
+// ---- a cache in pages ------------------------------------------------------------------------
+static int pool_check(const prefixlm_page_pool& p, bool contents) {
+  if (p.head_dim != 64 && p.head_dim != 128) return fail(PREFIXLM_ERR_INVALID, "head_dim must be 64 or 128 (got %d)", p.head_dim);
+  if (p.page_size < 16 || p.page_size > 1024 || (p.page_size & (p.page_size - 1)))
+    return fail(PREFIXLM_ERR_INVALID, "page_size must be a power of two from 16 to 1024 (got %d)", p.page_size);
+  if (p.layers < 1 || p.layers > 32767 || p.num_pages < 1 || p.num_kv_heads < 1 || p.batch < 1 || p.columns < 1)
+    return fail(PREFIXLM_ERR_INVALID, "layers=%d (to 32767) num_pages=%d num_kv_heads=%d batch=%d columns=%d must be >= 1",
+                p.layers, p.num_pages, p.num_kv_heads, p.batch, p.columns);
+  if ((int64_t)p.columns * p.page_size > (1 << 30))
+    return fail(PREFIXLM_ERR_INVALID, "columns=%d x page_size=%d exceeds 2^30 rows", p.columns, p.page_size);
+  if ((int64_t)p.num_kv_heads * p.page_size * p.head_dim > (1 << 30))
+    return fail(PREFIXLM_ERR_INVALID, "a page of %d heads x %d x %d exceeds 2^30 elements", p.num_kv_heads, p.page_size, p.head_dim);
+  if (contents && (!p.k_pages || !p.v_pages || !aligned16(p.k_pages) || !aligned16(p.v_pages)))
+    return fail(PREFIXLM_ERR_INVALID, "k_pages or v_pages is null or not 16-byte aligned");
+  return PREFIXLM_OK;
+}
+static int table_check(const prefixlm_page_pool& p) {
+  if (!p.refs || !p.page_table || (uintptr_t)p.refs % 4 || (uintptr_t)p.page_table % 4)
+    return fail(PREFIXLM_ERR_INVALID, "refs or page_table is null or not 4-byte aligned");
+  if (p.table_stride < p.columns)
+    return fail(PREFIXLM_ERR_INVALID, "table_stride=%lld is below columns=%d", (long long)p.table_stride, p.columns);
+  return PREFIXLM_OK;
+}
+static int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
+
+// Rows that share a key-value head's keys, and the row blocks and key splits of their kernel.
+static int pg_rt(int64_t R) { return R <= 16 ? 1 : 2; }
+static int64_t pg_nrb(int64_t R) { return (R + 16 * pg_rt(R) - 1) / (16 * pg_rt(R)); }
+static int64_t pg_nsplit(int64_t B, int64_t Hkv, int64_t R, int64_t cap) {
+  const int64_t units = B * Hkv * pg_nrb(R), most = (cap + 4 * pkv::kKeys - 1) / (4 * pkv::kKeys);
+  return std::max<int64_t>(1, std::min({(768 + units - 1) / units, most, (int64_t)pkv::kMaxSplits}));
+}
+
+template <int D>
+static void pg_launch(const pkv::Params& P, int64_t nblk, hipStream_t stream) {
+  const int64_t R = (int64_t)P.S * P.G;
+  if (pg_rt(R) == 1)
+    hipLaunchKernelGGL((pkv::stream_kernel<D, 1>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
+  else
+    hipLaunchKernelGGL((pkv::stream_kernel<D, 2>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
+  if (P.nsplit > 1)
+    hipLaunchKernelGGL((pkv::combine_kernel<D>), dim3((unsigned)((P.B * P.Hkv * R + 3) / 4)), dim3(256), 0, stream, P);
+}
+
+extern "C" {
+
+size_t prefixlm_paged_workspace_size(int32_t batch, int32_t seqlen_q, int32_t num_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, int32_t page_size, int32_t columns) {
+  if (batch < 1 || seqlen_q < 1 || num_heads < 1 || num_kv_heads < 1 || num_heads % num_kv_heads || head_dim < 1 ||
+      page_size < 1 || columns < 1)
+    return 0;
+  const int64_t R = (int64_t)seqlen_q * (num_heads / num_kv_heads);
+  const int64_t n = pg_nsplit(batch, num_kv_heads, R, (int64_t)columns * page_size);
+  return n == 1 ? 0 : align_up(sizeof(float) * (size_t)batch * num_kv_heads * R * n * (head_dim + 4));
+}
+
+int prefixlm_paged_fwd(const prefixlm_paged_args* a, void* stream_) {
+  if (!a) return fail(PREFIXLM_ERR_INVALID, "args is null");
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  const prefixlm_page_pool& pool = a->pool;
+  int rc = pool_check(pool, true);
+  if (!rc) rc = table_check(pool);
+  if (rc) return rc;
+  const int S = a->seqlen_q, cap = pool.columns * pool.page_size;
+  if (S < 1 || S > 0x7fffffff - cap) return fail(PREFIXLM_ERR_INVALID, "seqlen_q=%d must be >= 1 and below 2^31 - %d", S, cap);
+  if (a->num_heads < 1 || a->num_heads % pool.num_kv_heads)
+    return fail(PREFIXLM_ERR_INVALID, "num_heads=%d must be a multiple of num_kv_heads=%d", a->num_heads, pool.num_kv_heads);
+  if (a->layer < 0 || a->layer >= pool.layers)
+    return fail(PREFIXLM_ERR_INVALID, "layer=%d outside [0, %d)", a->layer, pool.layers);
+  const bool has_new = a->k != nullptr;
+  if ((a->k == nullptr) != (a->v == nullptr)) return fail(PREFIXLM_ERR_INVALID, "k and v must be given together");
+  const void* ptrs[] = {a->q, a->out, a->k, a->v};
+  for (int i = 0; i < (has_new ? 4 : 2); ++i)
+    if (!ptrs[i] || !aligned16(ptrs[i]))
+      return fail(PREFIXLM_ERR_INVALID, "tensor pointer %d is null or not 16-byte aligned", i);
+  const int64_t st[] = {a->q_stride_b, a->q_stride_s, a->q_stride_h, a->out_stride_b, a->out_stride_s, a->out_stride_h,
+                        a->k_stride_b, a->k_stride_s, a->k_stride_h, a->v_stride_b,   a->v_stride_s,   a->v_stride_h};
+  for (int i = 0; i < (has_new ? 12 : 6); ++i)
+    if (st[i] < 0 || st[i] % 8)
+      return fail(PREFIXLM_ERR_INVALID, "stride %d (%lld) must be a non-negative multiple of 8", i, (long long)st[i]);
+  if (!a->cache_seqlens && (a->cache_seqlen < 0 || a->cache_seqlen > cap))
+    return fail(PREFIXLM_ERR_INVALID, "cache_seqlen=%d outside [0, %d]", a->cache_seqlen, cap);
+  const size_t need = prefixlm_paged_workspace_size(pool.batch, S, a->num_heads, pool.num_kv_heads, pool.head_dim,
+                                                    pool.page_size, pool.columns);
+  if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
+    return fail(PREFIXLM_ERR_INVALID, "workspace of %zu bytes is null, unaligned or below %zu", a->workspace_bytes, need);
+
+  pkv::Params P{};
+  const int64_t layer = (int64_t)pool.num_pages * pool.num_kv_heads * pool.page_size * pool.head_dim * a->layer;
+  P.q = static_cast<const bf16*>(a->q);
+  P.k = static_cast<const bf16*>(a->k);
+  P.v = static_cast<const bf16*>(a->v);
+  P.kp = static_cast<bf16*>(pool.k_pages) + layer;
+  P.vp = static_cast<bf16*>(pool.v_pages) + layer;
+  P.refs = pool.refs;
+  P.table = pool.page_table;
+  P.out = static_cast<bf16*>(a->out);
+  P.part = static_cast<float*>(a->workspace);
+  P.seqlens = a->cache_seqlens;
+  P.q_sb = a->q_stride_b; P.q_ss = a->q_stride_s; P.q_sh = a->q_stride_h;
+  P.k_sb = a->k_stride_b; P.k_ss = a->k_stride_s; P.k_sh = a->k_stride_h;
+  P.v_sb = a->v_stride_b; P.v_ss = a->v_stride_s; P.v_sh = a->v_stride_h;
+  P.o_sb = a->out_stride_b; P.o_ss = a->out_stride_s; P.o_sh = a->out_stride_h;
+  P.table_sb = pool.table_stride;
+  P.B = pool.batch; P.S = S; P.Hkv = pool.num_kv_heads; P.G = a->num_heads / pool.num_kv_heads;
+  P.P = pool.num_pages; P.cap = cap; P.ps_log2 = log2_of(pool.page_size);
+  P.causal = a->is_causal ? 1 : 0;
+  P.seqlen_const = a->cache_seqlen;
+  P.s_new = has_new ? S : 0;
+  P.scale_log2 = a->softmax_scale * kLog2e;
+  const int64_t R = (int64_t)S * P.G;
+  if (R > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "seqlen_q=%d x %d heads of a group is too large", S, P.G);
+  P.nsplit = (int)pg_nsplit(P.B, P.Hkv, R, cap);
+  P.nrb = (int)pg_nrb(R);
+  const int64_t units = (int64_t)P.B * P.Hkv * P.nsplit;
+  if (units > 0x7fffffff || P.nrb > 0x7fffffff / ((units + 7) / 8 * 8) || !launchable((units + 7) / 8 * 8 * P.nrb, pkv::NT) ||
+      !launchable(((int64_t)P.B * P.Hkv * R + 3) / 4, 256))
+    return fail(PREFIXLM_ERR_INVALID, "grid too large");
+  const int64_t nblk = (units + 7) / 8 * 8 * P.nrb;
+  (void)hipGetLastError();
+  if (pool.head_dim == 128)
+    pg_launch<128>(P, nblk, stream);
+  else
+    pg_launch<64>(P, nblk, stream);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "paged kv-cache launch: %s", hipGetErrorString(e));
+  return PREFIXLM_OK;
+}
+
+}  // extern "C"
+
+// Workspace of reserve: free pages, three words a page, copies; of compact: moves, targets
+static size_t pages_free_words(const prefixlm_page_pool& p) {
+  return (size_t)std::min<int64_t>(p.num_pages, (int64_t)p.batch * p.columns);
+}
+static int pages_check(const prefixlm_pages_args* a, bool contents, bool workspace) {
+  if (!a) return fail(PREFIXLM_ERR_INVALID, "args is null");
+  int rc = pool_check(a->pool, contents);
+  if (!rc) rc = table_check(a->pool);
+  if (rc) return rc;
+  if (workspace) {
+    const size_t need = prefixlm_pages_workspace_size(&a->pool);
+    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need)
+      return fail(PREFIXLM_ERR_INVALID, "workspace of %zu bytes is null, unaligned or below %zu", a->workspace_bytes, need);
+    if (!a->result || (uintptr_t)a->result % 4) return fail(PREFIXLM_ERR_INVALID, "result is null or not 4-byte aligned");
+  }
+  return PREFIXLM_OK;
+}
+static int pages_end(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "%s launch: %s", what, hipGetErrorString(e));
+  return PREFIXLM_OK;
+}
+// What all copies of a pool share. by_head: pairs bring rows, else whole pages move.
+static pages::CopyParams pages_copy(const prefixlm_page_pool& to, const prefixlm_page_pool& from, bool by_head) {
+  pages::CopyParams C{};
+  const int64_t page = (int64_t)to.num_kv_heads * to.page_size * to.head_dim;
+  C.from[0] = static_cast<const bf16*>(from.k_pages);
+  C.from[1] = static_cast<const bf16*>(from.v_pages);
+  C.to[0] = static_cast<bf16*>(to.k_pages);
+  C.to[1] = static_cast<bf16*>(to.v_pages);
+  C.from_layer = page * from.num_pages;
+  C.to_layer = page * to.num_pages;
+  C.P_from = from.num_pages;
+  C.P_to = to.num_pages;
+  C.heads = by_head ? to.num_kv_heads : 1;
+  C.head_elems = (int)(page / C.heads);
+  C.row_elems = to.head_dim;
+  C.rows = by_head;
+  C.pieces = (C.head_elems + 2047) / 2048;
+  return C;
+}
+// Workgroups of a copy of up to n pairs: eight for each CU over all layers, or what there is to do
+static int pages_copy_grid(const pages::CopyParams& C, int64_t n, int layers, dim3* grid) {
+  const int64_t most = (int64_t)C.heads * C.pieces;   // waves of a pair
+  if (n > 0x7fffffff / most) return fail(PREFIXLM_ERR_INVALID, "too many pages to copy in one call");
+  int cus = 0;
+  const int rc = persistent_grid(&cus);
+  if (rc) return rc;
+  const int64_t x = std::min<int64_t>((n * most + 3) / 4, (8 * (int64_t)cus + 2 * layers - 1) / (2 * layers));
+  *grid = dim3((unsigned)(std::max<int64_t>(1, x) + C.n_remap), (unsigned)(2 * layers));
+  return PREFIXLM_OK;
+}
+
+extern "C" {
+
+size_t prefixlm_pages_workspace_size(const prefixlm_page_pool* p) {
+  if (!p || p->num_pages < 1 || p->batch < 1 || p->columns < 1) return 0;
+  const size_t reserve = pages_free_words(*p) + 3 * (size_t)p->num_pages + 1 + 3 * (size_t)p->batch;
+  const size_t compact = 1 + 2 * (size_t)p->num_pages;
+  return align_up(sizeof(int32_t) * std::max(reserve, compact));
+}
+
+int prefixlm_pages_reserve(const prefixlm_pages_args* a, void* stream_) {
+  const int rc = pages_check(a, true, true);
+  if (rc) return rc;
+  const prefixlm_page_pool& p = a->pool;
+  if (p.batch > pages::kMaxSeqs) return fail(PREFIXLM_ERR_INVALID, "batch=%d exceeds %d", p.batch, pages::kMaxSeqs);
+  if ((int64_t)p.batch * p.columns > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "a table of %d x %d is too large", p.batch, p.columns);
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  pages::ReserveParams P{};
+  P.refs = p.refs;
+  P.table = p.page_table;
+  P.seqlens = a->rows;
+  P.new_rows = a->new_rows;
+  P.short_ = a->result;
+  P.free_list = static_cast<int32_t*>(a->workspace);
+  P.was = P.free_list + pages_free_words(p);
+  P.copies = P.was + 3 * (size_t)p.num_pages;
+  P.table_sb = p.table_stride;
+  P.N = p.batch; P.M = p.columns; P.P = p.num_pages; P.ps_log2 = log2_of(p.page_size);
+  P.seqlen_const = a->row_const;
+  P.new_const = a->new_row_const;
+  pages::CopyParams C = pages_copy(p, p, true);
+  C.src = P.copies + 1;
+  C.count = P.copies;
+  dim3 grid;
+  const int rc2 = pages_copy_grid(C, p.batch, p.layers, &grid);   // a sequence's first column alone has rows to be copied
+  if (rc2) return rc2;
+  (void)hipGetLastError();
+  hipLaunchKernelGGL(pages::reserve_kernel, dim3(1), dim3(pages::NTH), 0, stream, P);
+  hipLaunchKernelGGL(pages::copy_kernel, grid, dim3(256), 0, stream, C);
+  return pages_end("page reserve");
+}
+
+int prefixlm_pages_fork(const prefixlm_pages_args* a, void* stream_) {
+  const int rc = pages_check(a, false, false);
+  if (rc) return rc;
+  const prefixlm_page_pool& p = a->pool;
+  if (p.batch > pages::kMaxSeqs) return fail(PREFIXLM_ERR_INVALID, "batch=%d exceeds %d", p.batch, pages::kMaxSeqs);
+  if (!a->src || (uintptr_t)a->src % 4) return fail(PREFIXLM_ERR_INVALID, "src is null or not 4-byte aligned");
+  pages::ForkParams P{};
+  P.refs = p.refs;
+  P.table = p.page_table;
+  P.parents = a->src;
+  P.table_sb = p.table_stride;
+  P.N = p.batch; P.M = p.columns; P.P = p.num_pages;
+  // 64 KB of LDS
+  P.TC = std::min(p.batch <= 1024 ? 16 : p.batch <= 2048 ? 8 : p.batch <= 4096 ? 4 : 2, p.columns);
+  (void)hipGetLastError();
+  hipLaunchKernelGGL(pages::fork_kernel, dim3((unsigned)((p.columns + P.TC - 1) / P.TC)), dim3(pages::NTH),
+                     sizeof(int32_t) * P.N * P.TC, reinterpret_cast<hipStream_t>(stream_), P);
+  return pages_end("page fork");
+}
+
+int prefixlm_pages_free(const prefixlm_pages_args* a, void* stream_) {
+  const int rc = pages_check(a, false, false);
+  if (rc) return rc;
+  const prefixlm_page_pool& p = a->pool;
+  pages::FreeParams P{};
+  P.refs = p.refs;
+  P.table = p.page_table;
+  P.keep = a->rows;
+  P.keep_const = a->row_const;
+  P.table_sb = p.table_stride;
+  P.N = p.batch; P.M = p.columns; P.P = p.num_pages; P.ps_log2 = log2_of(p.page_size);
+  const int64_t nblk = ((int64_t)P.N * P.M + 255) / 256;
+  if (!launchable(nblk, 256)) return fail(PREFIXLM_ERR_INVALID, "a table of %d x %d is too large", P.N, P.M);
+  (void)hipGetLastError();
+  hipLaunchKernelGGL(pages::free_kernel, dim3((unsigned)nblk), dim3(256), 0, reinterpret_cast<hipStream_t>(stream_), P);
+  return pages_end("page free");
+}
+
+int prefixlm_pages_compact(const prefixlm_pages_args* a, void* stream_) {
+  const int rc = pages_check(a, true, true);
+  if (rc) return rc;
+  const prefixlm_page_pool& p = a->pool;
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  pages::CompactParams P{};
+  P.refs = p.refs;
+  P.table = p.page_table;
+  P.used = a->result;
+  P.moves = static_cast<int32_t*>(a->workspace);
+  P.to = P.moves + 1 + p.num_pages;
+  P.table_sb = p.table_stride;
+  P.N = p.batch; P.M = p.columns; P.P = p.num_pages;
+  pages::CopyParams C = pages_copy(p, p, false);
+  // the moves' targets come first, then as many sources; how many, the kernel before this one knows
+  C.dst = P.moves + 1;
+  C.src = nullptr;
+  C.count = P.moves;
+  C.table = p.page_table;
+  C.to_page = P.to;
+  C.used = a->result;
+  C.table_sb = p.table_stride;
+  C.N = p.batch; C.M = p.columns;
+  C.n_remap = (int)std::min<int64_t>(64, ((int64_t)C.N * C.M + 1023) / 1024);
+  dim3 grid;
+  const int rc2 = pages_copy_grid(C, p.num_pages / 2, p.layers, &grid);
+  if (rc2) return rc2;
+  (void)hipGetLastError();
+  hipLaunchKernelGGL(pages::compact_kernel, dim3(1), dim3(pages::NTH), 0, stream, P);
+  hipLaunchKernelGGL(pages::copy_kernel, grid, dim3(256), 0, stream, C);
+  return pages_end("page compact");
+}
+
+int prefixlm_pages_copy(const prefixlm_pages_args* a, void* stream_) {
+  if (!a) return fail(PREFIXLM_ERR_INVALID, "args is null");
+  const prefixlm_page_pool &to = a->pool, &from = a->from ? *a->from : a->pool;
+  int rc = pool_check(to, true);
+  if (!rc) rc = pool_check(from, true);
+  if (rc) return rc;
+  if (to.layers != from.layers || to.num_kv_heads != from.num_kv_heads || to.page_size != from.page_size || to.head_dim != from.head_dim)
+    return fail(PREFIXLM_ERR_INVALID, "the pools' layers, heads, page_size or head_dim differ");
+  if (a->n < 0 || a->n > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "n=%lld is negative or too large", (long long)a->n);
+  if (a->n == 0) return PREFIXLM_OK;
+  if (!a->src || !a->dst || (uintptr_t)a->src % 4 || (uintptr_t)a->dst % 4)
+    return fail(PREFIXLM_ERR_INVALID, "src or dst is null or not 4-byte aligned");
+  pages::CopyParams C = pages_copy(to, from, false);
+  C.src = a->src;
+  C.dst = a->dst;
+  C.n = (int)a->n;
+  dim3 grid;
+  rc = pages_copy_grid(C, a->n, to.layers, &grid);
+  if (rc) return rc;
+  (void)hipGetLastError();
+  hipLaunchKernelGGL(pages::copy_kernel, grid, dim3(256), 0, reinterpret_cast<hipStream_t>(stream_), C);
+  return pages_end("page copy");
 }
 
 }  // extern "C"

@@ -8,6 +8,8 @@ from .plan import build_plan, plan_ds_blocks, plan_inputs, plan_size
 from .layer import fused_attention_layer
 from .kvcache import flash_attn_with_kvcache
 from .kvcache8 import KVCacheQ8, flash_attn_with_kvcache_q8, kvcache_q8
+from .paged import (PagedKVCache, flash_attn_with_paged_kvcache, paged_kvcache, paged_kvcache_compact, paged_kvcache_copy,
+                    paged_kvcache_fork, paged_kvcache_free, paged_kvcache_reserve)
 from .norm_mlp import rms_norm, swiglu
 from .embedding import embedding
 from .logprob import TokenLogprobs, token_logprobs
@@ -19,10 +21,18 @@ __all__ = [
     "flash_attn_varlen_prefixlm",
     "flash_attn_with_kvcache",
     "flash_attn_with_kvcache_q8",
+    "flash_attn_with_paged_kvcache",
     "fused_attention_layer",
     "FlashAttnVarlenPrefixLM",
     "KVCacheQ8",
     "kvcache_q8",
+    "PagedKVCache",
+    "paged_kvcache",
+    "paged_kvcache_compact",
+    "paged_kvcache_copy",
+    "paged_kvcache_fork",
+    "paged_kvcache_free",
+    "paged_kvcache_reserve",
     "TokenLogprobs",
     "token_logprobs",
     "useful_entries",

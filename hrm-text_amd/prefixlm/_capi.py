@@ -160,6 +160,35 @@ class Kvcache8Args(ctypes.Structure):
     ]
 
 
+class PagePool(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", c_vp), ("v_pages", c_vp), ("refs", c_vp), ("page_table", c_vp), ("table_stride", c_i64),
+        ("layers", c_i32), ("num_pages", c_i32), ("num_kv_heads", c_i32), ("page_size", c_i32), ("head_dim", c_i32),
+        ("batch", c_i32), ("columns", c_i32),
+    ]
+
+
+class PagedArgs(ctypes.Structure):
+    _fields_ = [
+        ("pool", PagePool), ("q", c_vp), ("k", c_vp), ("v", c_vp), ("out", c_vp),
+        ("q_stride_b", c_i64), ("q_stride_s", c_i64), ("q_stride_h", c_i64),
+        ("k_stride_b", c_i64), ("k_stride_s", c_i64), ("k_stride_h", c_i64),
+        ("v_stride_b", c_i64), ("v_stride_s", c_i64), ("v_stride_h", c_i64),
+        ("out_stride_b", c_i64), ("out_stride_s", c_i64), ("out_stride_h", c_i64),
+        ("cache_seqlens", c_vp), ("cache_seqlen", c_i32), ("layer", c_i32), ("seqlen_q", c_i32), ("num_heads", c_i32),
+        ("is_causal", c_i32), ("softmax_scale", c_f32),
+        ("workspace", c_vp), ("workspace_bytes", c_sz),
+    ]
+
+
+class PagesArgs(ctypes.Structure):
+    _fields_ = [
+        ("pool", PagePool), ("from_", ctypes.POINTER(PagePool)), ("rows", c_vp), ("new_rows", c_vp), ("src", c_vp),
+        ("dst", c_vp), ("row_const", c_i32), ("new_row_const", c_i32), ("n", c_i64), ("result", c_vp),
+        ("workspace", c_vp), ("workspace_bytes", c_sz),
+    ]
+
+
 class LogprobArgs(ctypes.Structure):
     _fields_ = [
         ("x", c_vp), ("targets", c_vp), ("logprob", c_vp), ("entropy", c_vp), ("stats", c_vp),
@@ -206,6 +235,14 @@ SIGNATURES = {
     "prefixlm_kvcache_fwd": (ctypes.c_int, [ctypes.POINTER(KvcacheArgs), c_vp]),
     "prefixlm_kvcache8_workspace_size": (c_sz, [c_i32, c_i32, c_i32, c_i32]),
     "prefixlm_kvcache8_fwd": (ctypes.c_int, [ctypes.POINTER(Kvcache8Args), c_vp]),
+    "prefixlm_paged_workspace_size": (c_sz, [c_i32] * 7),
+    "prefixlm_paged_fwd": (ctypes.c_int, [ctypes.POINTER(PagedArgs), c_vp]),
+    "prefixlm_pages_workspace_size": (c_sz, [ctypes.POINTER(PagePool)]),
+    "prefixlm_pages_reserve": (ctypes.c_int, [ctypes.POINTER(PagesArgs), c_vp]),
+    "prefixlm_pages_fork": (ctypes.c_int, [ctypes.POINTER(PagesArgs), c_vp]),
+    "prefixlm_pages_free": (ctypes.c_int, [ctypes.POINTER(PagesArgs), c_vp]),
+    "prefixlm_pages_compact": (ctypes.c_int, [ctypes.POINTER(PagesArgs), c_vp]),
+    "prefixlm_pages_copy": (ctypes.c_int, [ctypes.POINTER(PagesArgs), c_vp]),
     "prefixlm_logprob_workspace_size": (c_sz, [c_i64, c_i64, c_i32]),
     "prefixlm_logprob_fwd": (ctypes.c_int, [ctypes.POINTER(LogprobArgs), c_vp]),
     "prefixlm_logprob_bwd": (ctypes.c_int, [ctypes.POINTER(LogprobArgs), c_vp]),

@@ -419,6 +419,86 @@ typedef struct prefixlm_kvcache8_args {
 size_t prefixlm_kvcache8_workspace_size(int32_t batch, int32_t seqlen_q, int32_t num_heads, int32_t max_seqlen_cache);
 int prefixlm_kvcache8_fwd(const prefixlm_kvcache8_args* args, void* stream);
 
+/* A key-value cache in pages. k_pages, v_pages: bf16 [layers, num_pages, num_kv_heads, page_size, head_dim],
+ * contiguous, 16-byte aligned; page_size a power of two from 16 to 1024, head_dim 64 or 128. page_table: int32
+ * [batch, columns], rows table_stride elements apart (>= columns): column c of a sequence is the page of its
+ * rows c * page_size and on; an entry outside [0, num_pages) is no page. refs: int32 [num_pages], how many
+ * entries hold a page; 0: it is free. columns * page_size at most 2^30. */
+typedef struct prefixlm_page_pool {
+  void* k_pages;
+  void* v_pages;
+  int32_t* refs;
+  int32_t* page_table;
+  int64_t table_stride;
+  int32_t layers, num_pages, num_kv_heads, page_size, head_dim;
+  int32_t batch, columns;
+} prefixlm_page_pool;
+
+/* Attention of q [B, S, num_heads, head_dim] over a layer's pages (B = pool.batch; num_heads a multiple of
+ * num_kv_heads: query head h reads key-value head h / (num_heads / num_kv_heads)). k, v [B, S,
+ * num_kv_heads, head_dim] (or both NULL) are rows cache_seqlens[b] .. + S - 1 of their sequences: attended as given,
+ * and stored in pages that refs counts once; those at columns * page_size and beyond are dropped. Cached rows
+ * without a page are not seen. Lengths outside [0, columns * page_size] count as the nearest of the two.
+ * is_causal: query i sees keys j <= rows - S + i. A query that sees no key gives 0. Unit stride over
+ * head_dim; other strides multiples of 8; pointers 16-byte aligned. */
+typedef struct prefixlm_paged_args {
+  prefixlm_page_pool pool;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;                     /* [B, S, num_heads, head_dim] */
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  int64_t out_stride_b, out_stride_s, out_stride_h;
+  const int32_t* cache_seqlens;  /* device int32 [B], or NULL */
+  int32_t cache_seqlen;          /* used when cache_seqlens is NULL */
+  int32_t layer;
+  int32_t seqlen_q;              /* S */
+  int32_t num_heads;
+  int32_t is_causal;
+  float softmax_scale;
+  void* workspace;               /* >= prefixlm_paged_workspace_size(...) bytes */
+  size_t workspace_bytes;
+} prefixlm_paged_args;
+size_t prefixlm_paged_workspace_size(int32_t batch, int32_t seqlen_q, int32_t num_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, int32_t page_size, int32_t columns);
+int prefixlm_paged_fwd(const prefixlm_paged_args* args, void* stream);
+
+/* The pages themselves. Nothing here waits for the host; a call whose inputs are the same ends the same.
+ * reserve: each sequence gets pages of its own for rows rows[b] .. rows[b] + new_rows[b] - 1. Those columns
+ *   that lack a page, or whose page other entries hold too, get the lowest free pages in the order of sequences
+ *   and columns; of a page whose holders all ask for it in this call, the first keeps it. A page that others
+ *   hold is left behind, with the rows before rows[b] copied from it, in every layer. result[b]: how many of
+ *   the columns are left without a page of their own (0 while free pages last). batch at most 8192.
+ * fork: sequence b's row of the table becomes sequence src[b]'s, all at once; src[b] outside [0, batch) leaves it.
+ * free: sequence b gives up the pages from row rows[b] on (those whose first row is not below it).
+ * compact: the pages in use, U, move to numbers below U: the i-th used one from U on to the i-th free one
+ *   below it, in every layer. result[0] = U.
+ * copy: pages src[i] of `from` (NULL: of the pool itself) to pages dst[i], in every layer, i < n; pairs with a
+ *   page outside its pool are skipped. The pages of dst differ from each other and from src where the pools
+ *   are the same; else what they hold afterwards is not defined. Pools of the same layers, heads, page_size and
+ *   head_dim. refs and tables stay. */
+typedef struct prefixlm_pages_args {
+  prefixlm_page_pool pool;
+  const prefixlm_page_pool* from;  /* copy only; its refs and table are not read */
+  const int32_t* rows;           /* device [batch], or NULL: row_const. reserve, free */
+  const int32_t* new_rows;       /* device [batch], or NULL: new_row_const. reserve */
+  const int32_t* src;            /* device: fork [batch], copy [n] */
+  const int32_t* dst;            /* device: copy [n] */
+  int32_t row_const, new_row_const;
+  int64_t n;
+  int32_t* result;               /* device: reserve [batch], compact [1] */
+  void* workspace;               /* >= prefixlm_pages_workspace_size(&pool) bytes, 16-byte aligned. reserve, compact */
+  size_t workspace_bytes;
+} prefixlm_pages_args;
+size_t prefixlm_pages_workspace_size(const prefixlm_page_pool* pool);
+int prefixlm_pages_reserve(const prefixlm_pages_args* args, void* stream);
+int prefixlm_pages_fork(const prefixlm_pages_args* args, void* stream);
+int prefixlm_pages_free(const prefixlm_pages_args* args, void* stream);
+int prefixlm_pages_compact(const prefixlm_pages_args* args, void* stream);
+int prefixlm_pages_copy(const prefixlm_pages_args* args, void* stream);
+
 /* Log probabilities of given tokens from logits, with the entropy and the top alternatives (the
  * cross entropy of models/lm_head.py:52 is -logprob), and the gradient of the logits. x: bf16 or
  * fp32 [rows, vocab], unit stride over the vocabulary, any row stride, aligned to its element.
