@@ -13,6 +13,7 @@
 //
 // The G query heads of a key-value head and the S queries are the R = S G rows that share its keys: row
 // r is query r / G of head h G + r % G. Kernels:
+//   decode  : up to four rows, split over the keys, without the matrix cores;
 //   stream  : 16 RT rows a workgroup, split over the keys. Each wave walks 32 keys at a time by itself,
 //             K as it lies in memory into the matrix cores, V through LDS of its own;
 //   combine : joins the splits.
@@ -83,11 +84,11 @@ __device__ __forceinline__ float rows_sum(float x) {
 }
 
 // This workgroup's share of the new rows of (b, h), part `part` of `parts`, into their pages
-template <int D>
+template <int D, int NTH = NT>
 __device__ __forceinline__ void append_share(const Params& P, int b, int h, int len, int part, int parts) {
   constexpr int CH = D / 8;   // 16-byte chunks of a row
   const int c = 8 * (threadIdx.x % CH), is_v = (threadIdx.x / CH) & 1;
-  for (int i = part + parts * (threadIdx.x / (2 * CH)); i < P.s_new; i += parts * (NT / (2 * CH))) {
+  for (int i = part + parts * (threadIdx.x / (2 * CH)); i < P.s_new; i += parts * (NTH / (2 * CH))) {
     const int j = len + i;
     if (j >= P.cap) break;
     const int page = P.table[b * P.table_sb + (j >> P.ps_log2)];
@@ -162,17 +163,242 @@ __device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int spl
   }
 }
 
+// ---- few rows ---------------------------------------------------------------------------------
+// Sum over the D / 8 lanes that hold a key row
+template <int D>
+__device__ __forceinline__ float lanes_sum(float x) {
+  x += dpp_f<0xB1>(x);                 // quad_perm [1,0,3,2]
+  x += dpp_f<0x4E>(x);                 // quad_perm [2,3,0,1]
+  x += dpp_f<0x141>(x);                // row_half_mirror
+  if (D == 128) x += dpp_f<0x140>(x);  // row_mirror
+  return x;
+}
+
+// NR rows (R of them real) of one (b, h, split): blockIdx.x = (b Hkv + h) nsplit + split. Each wave walks 16
+// NH keys at a time by itself; D / 8 lanes hold a key row, 16 bytes each, and take its products with all
+// rows.
+template <int D, int NR, int NTH>
+__global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
+  constexpr int NWAVE = NTH / 64, CH = D / 8, RPL = 64 / CH, NH = D == 128 ? 1 : 2, U = 16 / RPL;
+  constexpr int kStep = 16 * NH * NWAVE;     // keys of a workgroup's step
+  __shared__ float s_m[NWAVE][NR], s_l[NWAVE][NR], s_seen[NWAVE][NR];
+  __shared__ f32x4 s_o[NWAVE][NR][D / 4];
+  const int split = blockIdx.x % P.nsplit, bh = blockIdx.x / P.nsplit;
+  const int h = bh % P.Hkv, b = bh / P.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, c8 = 8 * (lane % CH), grp = lane / CH;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int R = P.S * P.G;
+  const int len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
+  const int lk = min(P.cap, len + P.s_new);
+  const int per = ((lk + P.nsplit - 1) / P.nsplit + kStep - 1) / kStep * kStep;
+  const int k0 = split * per;
+  const int k1 = min(k0 + per, keys_seen(P, len, P.S - 1));     // the last row sees the most
+  const int kall = min(min(k1, len), keys_seen(P, len, 0));     // cached keys below are seen by every row
+
+  uniform_i32* const tab = uniform(P.table + b * P.table_sb);
+  const int psm = (1 << P.ps_log2) - 1;
+  const bf16* const kn = P.s_new ? P.k + b * P.k_sb + h * P.k_sh + c8 : nullptr;
+  const bf16* const vn = P.s_new ? P.v + b * P.v_sb + h * P.v_sh + c8 : nullptr;
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  u32x4 kw[NH][U], vw[NH][U];
+  int page[NH];                 // of the 16 keys to load next
+  bool ok[NH];                  // the cached ones among the 16 keys have a page
+  auto look = [&](int j0) {
+#pragma unroll
+    for (int hf = 0; hf < NH; ++hf) page[hf] = j0 + 16 * hf < len ? tab[(j0 + 16 * hf) >> P.ps_log2] : -1;
+  };
+  const uint32_t off = (uint32_t)(grp * D + c8) * 2;
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int hf = 0; hf < NH; ++hf) {
+      const int j = j0 + 16 * hf;
+      ok[hf] = (unsigned)page[hf] < (unsigned)P.P;
+      const int64_t at = ((((int64_t)(ok[hf] ? page[hf] : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
+      const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
+      if (ok[hf] && j + 16 <= len) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          kw[hf][u] = kvc::load_once(reinterpret_cast<const bf16*>(kb + off + u * (RPL * D * 2)));
+          vw[hf][u] = kvc::load_once(reinterpret_cast<const bf16*>(vb + off + u * (RPL * D * 2)));
+        }
+      } else {
+        // the last cached rows, the new ones, none: row by row
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int jr = j + u * RPL + grp;
+          kw[hf][u] = vw[hf][u] = zero;
+          if (jr < len ? ok[hf] : jr < lk) {
+            kw[hf][u] = *reinterpret_cast<const u32x4*>(jr < len ? kb + off + u * (RPL * D * 2) : reinterpret_cast<const char*>(kn + (jr - len) * P.k_ss));
+            vw[hf][u] = *reinterpret_cast<const u32x4*>(jr < len ? vb + off + u * (RPL * D * 2) : reinterpret_cast<const char*>(vn + (jr - len) * P.v_ss));
+          }
+        }
+      }
+    }
+  };
+  int j0 = k0 + 16 * NH * w;
+  if (j0 < k1) {
+    look(j0);
+    load(j0);
+    look(j0 + kStep);
+  }
+  float q[NR][8], o[NR][8], m[NR], l[NR], seen[NR];
+  int nlim[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int rr = min(r, R - 1);
+    const u32x4 x = *reinterpret_cast<const u32x4*>(P.q + b * P.q_sb + (rr / P.G) * P.q_ss + (h * P.G + rr % P.G) * P.q_sh + c8);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[r][2 * e] = bf16lo(x[e]) * P.scale_log2, q[r][2 * e + 1] = bf16hi(x[e]) * P.scale_log2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[r][e] = 0.f;
+    m[r] = -INFINITY, l[r] = 0.f, seen[r] = 0.f;
+    nlim[r] = min(k1, keys_seen(P, len, rr / P.G));
+  }
+  for (; j0 < k1; j0 += kStep) {
+    float s[NR][NH][U];
+#pragma unroll
+    for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[2 * e] = bf16lo(kw[hf][u][e]), x[2 * e + 1] = bf16hi(kw[hf][u][e]);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          float d = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d += q[r][e] * x[e];
+          s[r][hf][u] = lanes_sum<D>(d);
+        }
+      }
+    bool full = j0 + 16 * NH <= kall;
+#pragma unroll
+    for (int hf = 0; hf < NH; ++hf) full = full && ok[hf];
+    uint32_t hides = 0;          // bit (r, hf, u): the row does not see this lane's key
+    if (!full) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int j = j0 + 16 * hf + u * RPL + grp;
+            const bool sees = j < nlim[r] && (ok[hf] || j >= len);
+            seen[r] = sees ? 1.f : seen[r];
+            s[r][hf][u] = sees ? s[r][hf][u] : -INFINITY;
+            hides |= (sees ? 0u : 1u) << ((r * NH + hf) * U + u);
+          }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      if (full) seen[r] = 1.f;
+      float mx = m[r];
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[r][hf][u]);
+      const float ref = max_ref(mx), alpha = __builtin_amdgcn_exp2f(m[r] - ref);   // m = -inf at first: 0
+      m[r] = mx;
+      l[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[r][e] *= alpha;
+#pragma unroll
+      for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          s[r][hf][u] = __builtin_amdgcn_exp2f(s[r][hf][u] - ref);
+          l[r] += s[r][hf][u];
+        }
+    }
+#pragma unroll
+    for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[2 * e] = bf16lo(vw[hf][u][e]), x[2 * e + 1] = bf16hi(vw[hf][u][e]);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          // a value that the row does not see may be infinite
+          if (!full && (hides >> ((r * NH + hf) * U + u) & 1)) continue;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[r][e] += s[r][hf][u] * x[e];
+        }
+      }
+    if (j0 + kStep < k1) {
+      load(j0 + kStep);
+      look(j0 + 2 * kStep);
+    }
+  }
+  // the wave's groups, then the waves
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    float M = m[r];
+#pragma unroll
+    for (int x = CH; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
+    const float a = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[r] - M);
+    l[r] *= a;
+#pragma unroll
+    for (int x = CH; x < 64; x <<= 1) {
+      l[r] += __shfl_xor(l[r], x);
+      seen[r] = fmaxf(seen[r], __shfl_xor(seen[r], x));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      o[r][e] *= a;
+#pragma unroll
+      for (int x = CH; x < 64; x <<= 1) o[r][e] += __shfl_xor(o[r][e], x);
+    }
+    if (lane < CH) {
+      if (lane == 0) s_m[w][r] = M, s_l[w][r] = l[r], s_seen[w][r] = seen[r];
+      s_o[w][r][2 * lane] = f32x4{o[r][0], o[r][1], o[r][2], o[r][3]};
+      s_o[w][r][2 * lane + 1] = f32x4{o[r][4], o[r][5], o[r][6], o[r][7]};
+    }
+  }
+  __syncthreads();
+  if (tid < NR * (D / 4)) {
+    const int r = tid / (D / 4), c = tid % (D / 4);
+    if (r < R) {
+      float M = s_m[0][r], L = 0.f, any = 0.f;
+#pragma unroll
+      for (int g = 1; g < NWAVE; ++g) M = fmaxf(M, s_m[g][r]);
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < NWAVE; ++g) {
+        const float wgt = s_m[g][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[g][r] - M);
+        L += wgt * s_l[g][r];
+        any = fmaxf(any, s_seen[g][r]);
+        acc += wgt * s_o[g][r][c];
+      }
+      if (P.nsplit == 1) {
+        const float inv = row_inv(any != 0.f, L);
+        *reinterpret_cast<bf16x4*>(P.out + b * P.o_sb + (r / P.G) * P.o_ss + (h * P.G + r % P.G) * P.o_sh + 4 * c) =
+            cvt4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      } else {
+        float* dst = P.part + (((int64_t)bh * R + r) * P.nsplit + split) * kPart<D>;
+        if (c == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{M, L, any, 0.f};
+        *reinterpret_cast<f32x4*>(dst + 4 + 4 * c) = acc;
+      }
+    }
+  }
+  append_share<D, NTH>(P, b, h, len, split, P.nsplit);
+}
+
+// ---- more of them -------------------------------------------------------------------------------
 template <int D>
 struct Geo {
   static constexpr int NS = D / 32;              // steps of the contraction over d
-  static constexpr int ND = D / 16;              // 16-column tiles of o; 16-byte loads a lane of K, and of V
+  static constexpr int ND = D / 16;              // 16-column tiles of o; 16-byte loads a lane of 32 keys
   static constexpr int CH = D / 8;               // 16-byte chunks of a row
-  static constexpr int RPL = 64 / CH;            // V rows a load
+  static constexpr int RPL = 64 / CH;            // rows a load
   // V rows in LDS: 8 rows apart by 8 banks each, so that the 32 lanes of a transposing read's cycle, 8
   // rows of 32 bytes, take all 64 banks
   static constexpr int VS = 2 * D + 32;
+  // K rows in LDS: 4 banks apart, so that 16 rows' 16 bytes at one column take all 64
+  static constexpr int KS = 2 * D + 16;
   static constexpr int OS = D + 4;               // floats of a row of o where the waves meet
-  static constexpr int AREA = kKeys * VS > 16 * OS * 4 ? kKeys * VS : 16 * OS * 4;   // bytes a wave
+  static constexpr int AREA = kKeys * (VS + KS); // bytes a wave
+  static_assert(AREA >= 16 * OS * 4, "16 rows of o fit");
 };
 
 // blockIdx.x: row blocks of one (b, h, split) eight indices apart, on one XCD.
@@ -202,15 +428,14 @@ __global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
 
   uniform_i32* const tab = uniform(P.table + b * P.table_sb);
   const int psm = (1 << P.ps_log2) - 1;
-  const bf16* const kn = P.s_new ? P.k + b * P.k_sb + h * P.k_sh : nullptr;
-  const bf16* const vn = P.s_new ? P.v + b * P.v_sb + h * P.v_sh : nullptr;
+  const bf16* const kn = P.s_new ? P.k + b * P.k_sb + h * P.k_sh + 8 * (lane % CH) : nullptr;
+  const bf16* const vn = P.s_new ? P.v + b * P.v_sb + h * P.v_sh + 8 * (lane % CH) : nullptr;
   char* const area = smem[w];
 
   u32x4 kw[ND], vw[ND];
   bool ok[2];              // the 16 keys have a page, or are new rows
   const u32x4 zero = {0u, 0u, 0u, 0u};
-  // K: lane holds key l16 of each 16, columns 32 s + 8 g4 + 0..7; V: rows of CH lanes
-  const uint32_t koff = (uint32_t)(l16 * D + 8 * g4) * 2, voff = (uint32_t)(lane / CH * D + 8 * (lane % CH)) * 2;
+  const uint32_t off = (uint32_t)(lane / CH * D + 8 * (lane % CH)) * 2;
   auto load = [&](int j0) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -220,27 +445,24 @@ __global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
       const int64_t at = ((((int64_t)(held ? page : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
       const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
       ok[hf] = held;
-      if (held && j + 16 <= min(len, lk)) {
-#pragma unroll
-        for (int s = 0; s < NS; ++s) kw[hf * NS + s] = kvc::load_once(reinterpret_cast<const bf16*>(kb + koff + 64 * s));
-#pragma unroll
-        for (int u = 0; u < HL; ++u)
-          vw[hf * HL + u] = kvc::load_once(reinterpret_cast<const bf16*>(vb + voff + u * (G::RPL * D * 2)));
-      } else {
-        // the last cached rows, the new ones, none: row by row
-        {
-          const int jk = j + l16;
-          const char* p = jk < len ? (held ? kb + koff : nullptr)
-                                   : (jk < lk ? reinterpret_cast<const char*>(kn + (jk - len) * P.k_ss + 8 * g4) : nullptr);
-#pragma unroll
-          for (int s = 0; s < NS; ++s) kw[hf * NS + s] = p ? *reinterpret_cast<const u32x4*>(p + 64 * s) : zero;
-        }
+      if (held && j + 16 <= len) {
 #pragma unroll
         for (int u = 0; u < HL; ++u) {
-          const int jv = j + u * G::RPL + lane / CH;
-          const char* p = jv < len ? (held ? vb + voff + u * (G::RPL * D * 2) : nullptr)
-                                   : (jv < lk ? reinterpret_cast<const char*>(vn + (jv - len) * P.v_ss + 8 * (lane % CH)) : nullptr);
-          vw[hf * HL + u] = p ? *reinterpret_cast<const u32x4*>(p) : zero;
+          kw[hf * HL + u] = kvc::load_once(reinterpret_cast<const bf16*>(kb + off + u * (G::RPL * D * 2)));
+          vw[hf * HL + u] = kvc::load_once(reinterpret_cast<const bf16*>(vb + off + u * (G::RPL * D * 2)));
+        }
+      } else {
+        // the last cached rows, the new ones, none: row by row
+#pragma unroll
+        for (int u = 0; u < HL; ++u) {
+          const int jr = j + u * G::RPL + lane / CH;
+          kw[hf * HL + u] = vw[hf * HL + u] = zero;
+          if (jr < len ? held : jr < lk) {
+            kw[hf * HL + u] = *reinterpret_cast<const u32x4*>(
+                jr < len ? kb + off + u * (G::RPL * D * 2) : reinterpret_cast<const char*>(kn + (jr - len) * P.k_ss));
+            vw[hf * HL + u] = *reinterpret_cast<const u32x4*>(
+                jr < len ? vb + off + u * (G::RPL * D * 2) : reinterpret_cast<const char*>(vn + (jr - len) * P.v_ss));
+          }
         }
       }
     }
@@ -270,25 +492,30 @@ __global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) qf[t][s] = *reinterpret_cast<const bf16x8*>(qp + 32 * s);
     }
-    const char* const vt = area + (4 * g4 + (l16 >> 2)) * G::VS + 8 * (l16 & 3);
+    char* const karea = area + kKeys * G::VS;
+    const char *const vt = area + (4 * g4 + (l16 >> 2)) * G::VS + 8 * (l16 & 3), *const kt = karea + l16 * G::KS + 16 * g4;
+    const int row = lane / CH, c16 = 16 * (lane % CH);
     for (; j0 < k1; j0 += kKeys * NWAVE) {
-      f32x4 s[RT][2];
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          s[t][hf] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int n = 0; n < NS; ++n) s[t][hf] = mfma16x16x32(__builtin_bit_cast(bf16x8, kw[hf * NS + n]), qf[t][n], s[t][hf]);
-        }
+      for (int u = 0; u < ND; ++u) *reinterpret_cast<u32x4*>(karea + (u * G::RPL + row) * G::KS + c16) = kw[u];
 #pragma unroll
       for (int u = 0; u < ND; ++u) {
         vmag = max_mag(vmag, vw[u]);
-        *reinterpret_cast<u32x4*>(area + (u * G::RPL + lane / CH) * G::VS + 16 * (lane % CH)) = vw[u];
+        *reinterpret_cast<u32x4*>(area + (u * G::RPL + row) * G::VS + c16) = vw[u];
       }
       // a page that is missing hides cached keys only
       const bool ok0 = ok[0], ok1 = ok[1];
       if (j0 + kKeys * NWAVE < k1) load(j0 + kKeys * NWAVE);
+      // K: lane holds key l16 of 16, columns 32 n + 8 g4 + 0..7
+      f32x4 s[RT][2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + 16 * hf * G::KS + 64 * n);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) s[t][hf] = mfma16x16x32(kf, qf[t][n], n ? s[t][hf] : f32x4{0.f, 0.f, 0.f, 0.f});
+        }
       bf16x8 pt[RT][3];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {

@@ -1879,8 +1879,8 @@ static int table_check(const prefixlm_page_pool& p) {
 static int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 // Rows that share a key-value head's keys, and the row blocks and key splits of their kernel.
-static int pg_rt(int64_t R) { return R <= 16 ? 1 : 2; }
-static int64_t pg_nrb(int64_t R) { return (R + 16 * pg_rt(R) - 1) / (16 * pg_rt(R)); }
+static int pg_rt(int64_t R) { return R <= 4 ? 0 : R <= 16 ? 1 : 2; }
+static int64_t pg_nrb(int64_t R) { return pg_rt(R) ? (R + 16 * pg_rt(R) - 1) / (16 * pg_rt(R)) : 1; }
 static int64_t pg_nsplit(int64_t B, int64_t Hkv, int64_t R, int64_t cap) {
   const int64_t units = B * Hkv * pg_nrb(R), most = (cap + 4 * pkv::kKeys - 1) / (4 * pkv::kKeys);
   return std::max<int64_t>(1, std::min({(768 + units - 1) / units, most, (int64_t)pkv::kMaxSplits}));
@@ -1889,7 +1889,13 @@ static int64_t pg_nsplit(int64_t B, int64_t Hkv, int64_t R, int64_t cap) {
 template <int D>
 static void pg_launch(const pkv::Params& P, int64_t nblk, hipStream_t stream) {
   const int64_t R = (int64_t)P.S * P.G;
-  if (pg_rt(R) == 1)
+  if (R == 1)
+    hipLaunchKernelGGL((pkv::decode_kernel<D, 1, pkv::NT>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
+  else if (R == 2)
+    hipLaunchKernelGGL((pkv::decode_kernel<D, 2, pkv::NT>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
+  else if (pg_rt(R) == 0)
+    hipLaunchKernelGGL((pkv::decode_kernel<D, 4, pkv::NT>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
+  else if (pg_rt(R) == 1)
     hipLaunchKernelGGL((pkv::stream_kernel<D, 1>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
   else
     hipLaunchKernelGGL((pkv::stream_kernel<D, 2>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
@@ -1971,7 +1977,7 @@ int prefixlm_paged_fwd(const prefixlm_paged_args* a, void* stream_) {
   if (units > 0x7fffffff || P.nrb > 0x7fffffff / ((units + 7) / 8 * 8) || !launchable((units + 7) / 8 * 8 * P.nrb, pkv::NT) ||
       !launchable(((int64_t)P.B * P.Hkv * R + 3) / 4, 256))
     return fail(PREFIXLM_ERR_INVALID, "grid too large");
-  const int64_t nblk = (units + 7) / 8 * 8 * P.nrb;
+  const int64_t nblk = pg_rt(R) ? (units + 7) / 8 * 8 * P.nrb : units;
   (void)hipGetLastError();
   if (pool.head_dim == 128)
     pg_launch<128>(P, nblk, stream);

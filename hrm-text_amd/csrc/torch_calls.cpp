@@ -65,6 +65,14 @@ struct Lib {
   decltype(&prefixlm_kvcache_fwd) kv_fwd;
   decltype(&prefixlm_kvcache8_workspace_size) kv8_ws;
   decltype(&prefixlm_kvcache8_fwd) kv8_fwd;
+  decltype(&prefixlm_paged_workspace_size) paged_ws;
+  decltype(&prefixlm_paged_fwd) paged_fwd;
+  decltype(&prefixlm_pages_workspace_size) pages_ws;
+  decltype(&prefixlm_pages_reserve) pages_reserve;
+  decltype(&prefixlm_pages_fork) pages_fork;
+  decltype(&prefixlm_pages_free) pages_free;
+  decltype(&prefixlm_pages_compact) pages_compact;
+  decltype(&prefixlm_pages_copy) pages_copy;
   decltype(&prefixlm_logprob_workspace_size) lp_ws;
   decltype(&prefixlm_logprob_fwd) lp_fwd;
   decltype(&prefixlm_logprob_bwd) lp_bwd;
@@ -1087,6 +1095,285 @@ PyObject* py_kvcache_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- a cache in pages --------------------------------------------------------------------
+// The bytes that x's elements lie in
+struct Span {
+  const char *lo, *hi;
+  explicit Span(const Tensor& x) : lo(static_cast<const char*>(x.const_data_ptr())) {
+    int64_t n = 1;
+    for (int64_t d = 0; d < x.dim(); ++d) n += (x.size(d) - 1) * x.stride(d);
+    hi = lo + n * x.element_size();
+  }
+  bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+bool apart(std::initializer_list<std::reference_wrapper<const Tensor>> own, std::initializer_list<std::reference_wrapper<const Tensor>> others) {
+  for (auto i = own.begin(); i != own.end(); ++i) {
+    const Span s(*i);
+    for (auto j = own.begin(); j != i; ++j)
+      if (s.meets(Span(*j))) return false;
+    for (const Tensor& x : others)
+      if (x.defined() && s.meets(Span(x))) return false;
+  }
+  return true;
+}
+bool page_array(const Tensor& x) {
+  if (x.scalar_type() != at::kBFloat16 || x.dim() != 5 || x.numel() == 0 || !x.is_contiguous() || !aligned(x, 16) || wants_grad(x))
+    return false;
+  for (int64_t d = 0; d < 5; ++d)
+    if (x.size(d) > INT32_MAX) return false;
+  return true;
+}
+bool page_counts(const Tensor& refs, const Tensor& table) {
+  return refs.scalar_type() == at::kInt && refs.dim() == 1 && refs.numel() > 0 && refs.numel() <= INT32_MAX && refs.is_contiguous() &&
+         table.scalar_type() == at::kInt && table.dim() == 2 && table.numel() > 0 && table.size(0) <= INT32_MAX &&
+         table.size(1) <= INT32_MAX && table.device() == refs.device() && (table.size(1) == 1 || table.stride(1) == 1) &&
+         (table.size(0) == 1 || table.stride(0) >= table.size(1));
+}
+// k_pages, v_pages, refs, page_table; what the C entry checks itself is left to it, once it takes the whole cache
+struct Pages {
+  Tensor k, v, refs, table;
+  prefixlm_page_pool pool{};
+  bool parse(PyObject* const* a) {
+    if (!get_tensor(a[0], &k) || !get_tensor(a[1], &v) || !get_tensor(a[2], &refs) || !get_tensor(a[3], &table)) return false;
+    if (!page_array(k) || !page_array(v) || k.sizes() != v.sizes() || k.device() != v.device() || !page_counts(refs, table) ||
+        refs.device() != k.device() || refs.numel() != k.size(1))
+      return false;
+    const int64_t ps = k.size(3), D = k.size(4);
+    if (ps < 16 || ps > 1024 || (ps & (ps - 1)) || (D != 64 && D != 128)) return false;
+    fill(k.sizes());
+    pool.k_pages = k.data_ptr();
+    pool.v_pages = v.data_ptr();
+    return true;
+  }
+  bool parse_counts(PyObject* const* a, int64_t page_size) {
+    if (!get_tensor(a[0], &refs) || !get_tensor(a[1], &table) || !page_counts(refs, table)) return false;
+    fill({1, refs.numel(), 1, page_size, 64});
+    return true;
+  }
+  void fill(at::IntArrayRef s) {
+    pool.layers = (int32_t)s[0];
+    pool.num_pages = (int32_t)s[1];
+    pool.num_kv_heads = (int32_t)s[2];
+    pool.page_size = (int32_t)s[3];
+    pool.head_dim = (int32_t)s[4];
+    pool.batch = (int32_t)table.size(0);
+    pool.columns = (int32_t)table.size(1);
+    pool.table_stride = table.size(0) > 1 ? table.stride(0) : table.size(1);
+    pool.refs = refs.data_ptr<int32_t>();
+    pool.page_table = table.data_ptr<int32_t>();
+  }
+  void wrote_counts() const {
+    refs.unsafeGetTensorImpl()->bump_version();
+    table.unsafeGetTensorImpl()->bump_version();
+  }
+  void wrote_rows() const {
+    k.unsafeGetTensorImpl()->bump_version();
+    v.unsafeGetTensorImpl()->bump_version();
+  }
+};
+// An int, or int32 [n] on the cache's device
+struct RowCounts {
+  Tensor t;
+  int64_t c = 0;
+  bool parse(PyObject* o, const Tensor& like, int64_t n) {
+    if (PyLong_CheckExact(o)) {
+      int over = 0;
+      c = PyLong_AsLongLongAndOverflow(o, &over);
+      c = over ? (over > 0 ? INT32_MAX : -1) : std::max<int64_t>(-1, std::min<int64_t>(c, INT32_MAX));
+      return true;
+    }
+    return get_tensor(o, &t) && meta(t, like) && t.numel() == n;
+  }
+  const int32_t* data() const { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
+};
+
+// q, the cache's four tensors, k, v, cache_seqlens (int or tensor), softmax_scale (float or None), causal, layer
+PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v;
+  Pages c;
+  RowCounts lens;
+  Scalar layer;
+  bool causal;
+  double scale;
+  if (!ready(n, 11) || c10::InferenceMode::is_enabled() || !get_tensor(a[0], &q) || !c.parse(a + 1)) return none();
+  const bool has_new = a[5] != Py_None;
+  if (has_new != (a[6] != Py_None) || (has_new && (!get_tensor(a[5], &k) || !get_tensor(a[6], &v)))) return none();
+  for (const Tensor* t : {&q, &k, &v})
+    if (t->defined() && (!cache_layout(*t) || t->device() != c.k.device() || t->numel() == 0 || wants_grad(*t))) return none();
+  const int64_t B = q.size(0), S = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = c.k.size(2);
+  const int64_t cap = c.table.size(1) * c.k.size(3);
+  if (B != c.table.size(0) || D != c.k.size(4) || Hq % Hkv || S > INT32_MAX || Hq > INT32_MAX || cap > INT32_MAX) return none();
+  if (has_new && (k.sizes() != at::IntArrayRef({B, S, Hkv, D}) || v.sizes() != k.sizes())) return none();
+  if (!apart({c.k, c.v, c.refs, c.table}, {q, k, v})) return none();
+  if (!lens.parse(a[7], q, B) || (!lens.t.defined() && (lens.c < 0 || lens.c > cap))) return none();
+  if (a[8] == Py_None)
+    scale = 1.0 / std::sqrt((double)D);
+  else if (!get_double(a[8], &scale))
+    return none();
+  if (!get_bool(a[9], &causal) || !PyLong_CheckExact(a[10]) || !get_scalar(a[10], &layer) || layer.v < 0 || layer.v >= c.k.size(0))
+    return none();
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const Recorded call("prefixlm::paged_kvcache_attn", {q, c.k, c.v});
+    const c10::DeviceGuard guard(q.device());
+    out = empty_like_on(q, {B, S, Hq, D}, at::kBFloat16);
+    prefixlm_paged_args p{};
+    p.pool = c.pool;
+    p.workspace_bytes = lib.paged_ws(c.pool.batch, (int32_t)S, (int32_t)Hq, (int32_t)Hkv, (int32_t)D, c.pool.page_size, c.pool.columns);
+    Tensor ws;
+    if (p.workspace_bytes) {
+      ws = empty_like_on(q, {(int64_t)p.workspace_bytes}, at::kByte);
+      p.workspace = ws.data_ptr();
+    }
+    p.q = q.const_data_ptr();
+    p.out = out.data_ptr();
+    p.q_stride_b = q.stride(0), p.q_stride_s = q.stride(1), p.q_stride_h = q.stride(2);
+    if (has_new) {
+      p.k = k.const_data_ptr();
+      p.v = v.const_data_ptr();
+      p.k_stride_b = k.stride(0), p.k_stride_s = k.stride(1), p.k_stride_h = k.stride(2);
+      p.v_stride_b = v.stride(0), p.v_stride_s = v.stride(1), p.v_stride_h = v.stride(2);
+    }
+    p.out_stride_b = S * Hq * D, p.out_stride_s = Hq * D, p.out_stride_h = D;
+    p.cache_seqlens = lens.data();
+    p.cache_seqlen = (int32_t)lens.c;
+    p.layer = (int32_t)layer.v;
+    p.seqlen_q = (int32_t)S;
+    p.num_heads = (int32_t)Hq;
+    p.is_causal = i32(causal);
+    p.softmax_scale = (float)scale;
+    check(lib.paged_fwd(&p, stream_of(q)), "prefixlm_paged_fwd");
+    c.wrote_rows();
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// A call on the pages of c, with a workspace if it takes one
+void pages_call(const char* op, const char* name, decltype(lib.pages_fork) fn, const Pages& c, prefixlm_pages_args& p, bool workspace) {
+  const Tensor& on = c.k.defined() ? c.k : c.refs;
+  const Recorded call(op, {on});
+  const c10::DeviceGuard guard(on.device());
+  p.pool = c.pool;
+  Tensor ws;
+  if (workspace) {
+    p.workspace_bytes = lib.pages_ws(&c.pool);
+    ws = empty_like_on(on, {(int64_t)p.workspace_bytes}, at::kByte);
+    p.workspace = ws.data_ptr();
+  }
+  check(fn(&p, stream_of(on)), name);
+}
+// the cache's four tensors, cache_seqlens, new_rows (ints or tensors)
+PyObject* py_pages_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c;
+  RowCounts lens, more;
+  if (!ready(n, 6) || c10::InferenceMode::is_enabled() || !c.parse(a) || c.pool.batch > 8192 || !lens.parse(a[4], c.k, c.pool.batch) ||
+      !more.parse(a[5], c.k, c.pool.batch) || !apart({c.k, c.v, c.refs, c.table}, {}))
+    return none();
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty_like_on(c.refs, {c.pool.batch}, at::kInt);
+    prefixlm_pages_args p{};
+    p.rows = lens.data(), p.row_const = (int32_t)lens.c;
+    p.new_rows = more.data(), p.new_row_const = (int32_t)more.c;
+    p.result = out.data_ptr<int32_t>();
+    pages_call("prefixlm::paged_kvcache_reserve", "prefixlm_pages_reserve", lib.pages_reserve, c, p, true);
+    c.wrote_rows();
+    c.wrote_counts();
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+// refs, page_table, parents; True if done
+PyObject* py_pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c;
+  Tensor parents;
+  if (!ready(n, 3) || c10::InferenceMode::is_enabled() || !c.parse_counts(a, 16) || c.pool.batch > 8192 || !get_tensor(a[2], &parents) ||
+      !meta(parents, c.refs) || parents.numel() != c.pool.batch || !apart({c.refs, c.table}, {}))
+    return none();
+  {
+    pybind11::gil_scoped_release no_gil;
+    prefixlm_pages_args p{};
+    p.src = parents.const_data_ptr<int32_t>();
+    pages_call("prefixlm::paged_kvcache_fork", "prefixlm_pages_fork", lib.pages_fork, c, p, false);
+    c.wrote_counts();
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+// refs, page_table, page_size, keep_rows (int or tensor); True if done
+PyObject* py_pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c;
+  Scalar ps;
+  RowCounts keep;
+  if (!ready(n, 4) || c10::InferenceMode::is_enabled() || !PyLong_CheckExact(a[2]) || !get_scalar(a[2], &ps) || ps.v < 16 || ps.v > 1024 ||
+      !c.parse_counts(a, ps.v) || !keep.parse(a[3], c.refs, c.pool.batch) || !apart({c.refs, c.table}, {}))
+    return none();
+  {
+    pybind11::gil_scoped_release no_gil;
+    prefixlm_pages_args p{};
+    p.rows = keep.data(), p.row_const = (int32_t)keep.c;
+    pages_call("prefixlm::paged_kvcache_free", "prefixlm_pages_free", lib.pages_free, c, p, false);
+    c.wrote_counts();
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+// the cache's four tensors
+PyObject* py_pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c;
+  if (!ready(n, 4) || c10::InferenceMode::is_enabled() || !c.parse(a) || !apart({c.k, c.v, c.refs, c.table}, {})) return none();
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = empty_like_on(c.refs, {1}, at::kInt);
+    prefixlm_pages_args p{};
+    p.result = out.data_ptr<int32_t>();
+    pages_call("prefixlm::paged_kvcache_compact", "prefixlm_pages_compact", lib.pages_compact, c, p, true);
+    c.wrote_rows();
+    c.wrote_counts();
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+// the cache's four tensors, the source's (or four None), src, dst; True if done
+PyObject* py_pages_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c, from;
+  Tensor src, dst;
+  if (!ready(n, 10) || c10::InferenceMode::is_enabled() || !c.parse(a)) return none();
+  const bool other = a[4] != Py_None;
+  if (other) {
+    if (!from.parse(a + 4) || from.k.device() != c.k.device() || !apart({c.k, c.v, from.k, from.v}, {})) return none();
+    for (int d : {0, 2, 3, 4})
+      if (from.k.size(d) != c.k.size(d)) return none();
+  } else if (!apart({c.k, c.v}, {})) {
+    return none();
+  }
+  if (!get_tensor(a[8], &src) || !get_tensor(a[9], &dst) || !meta(src, c.k) || !meta(dst, c.k) || src.dim() != 1 ||
+      src.sizes() != dst.sizes() || src.numel() == 0)
+    return none();
+  {
+    pybind11::gil_scoped_release no_gil;
+    prefixlm_pages_args p{};
+    p.from = other ? &from.pool : nullptr;
+    p.src = src.const_data_ptr<int32_t>();
+    p.dst = dst.const_data_ptr<int32_t>();
+    p.n = src.numel();
+    pages_call("prefixlm::paged_kvcache_copy", "prefixlm_pages_copy", lib.pages_copy, c, p, false);
+    c.wrote_rows();
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // logits, targets (tensor or None), entropy, top_k, ignore_index -> (logprob, entropy, top_logprobs,
 // top_ids), None where not asked for
 PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -1365,6 +1652,12 @@ PyMethodDef methods[] = {
     {"layer", FAST(py_layer), nullptr},
     {"kvcache", FAST(py_kvcache), nullptr},
     {"kvcache_q8", FAST(py_kvcache_q8), nullptr},
+    {"paged", FAST(py_paged), nullptr},
+    {"pages_reserve", FAST(py_pages_reserve), nullptr},
+    {"pages_fork", FAST(py_pages_fork), nullptr},
+    {"pages_free", FAST(py_pages_free), nullptr},
+    {"pages_compact", FAST(py_pages_compact), nullptr},
+    {"pages_copy", FAST(py_pages_copy), nullptr},
     {"token_logprobs", FAST(py_token_logprobs), nullptr},
     {"embedding", FAST(py_embedding), nullptr},
     {"swiglu", FAST(py_swiglu), nullptr},

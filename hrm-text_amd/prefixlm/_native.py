@@ -26,7 +26,9 @@ _ENTRY_POINTS = ("prefixlm_fwd", "prefixlm_bwd", "prefixlm_fwd_q_amax_count", "p
                  "prefixlm_rope", "prefixlm_swiglu_fwd", "prefixlm_swiglu_bwd", "prefixlm_rmsnorm_fwd",
                  "prefixlm_rmsnorm_bwd", "prefixlm_add_rmsnorm", "prefixlm_proj_gemm", "prefixlm_proj_gemm_scaled",
                  "prefixlm_kvcache_workspace_size", "prefixlm_kvcache_fwd", "prefixlm_kvcache8_workspace_size",
-                 "prefixlm_kvcache8_fwd", "prefixlm_logprob_workspace_size", "prefixlm_logprob_fwd",
+                 "prefixlm_kvcache8_fwd", "prefixlm_paged_workspace_size", "prefixlm_paged_fwd",
+                 "prefixlm_pages_workspace_size", "prefixlm_pages_reserve", "prefixlm_pages_fork", "prefixlm_pages_free",
+                 "prefixlm_pages_compact", "prefixlm_pages_copy", "prefixlm_logprob_workspace_size", "prefixlm_logprob_fwd",
                  "prefixlm_logprob_bwd", "prefixlm_embedding_workspace_size", "prefixlm_embedding_fwd",
                  "prefixlm_embedding_bwd", "prefixlm_last_error")
 

@@ -32,7 +32,7 @@ from torch import Tensor
 from . import _capi
 from .kvcache import _check4
 from .kvcache8 import _span
-from .op import _ptr, _stream
+from .op import _native_calls, _ptr, _stream
 
 __all__ = ["PagedKVCache", "paged_kvcache", "flash_attn_with_paged_kvcache", "paged_kvcache_reserve", "paged_kvcache_fork",
            "paged_kvcache_free", "paged_kvcache_compact", "paged_kvcache_copy", "paged_kvcache_attn"]
@@ -187,9 +187,16 @@ def flash_attn_with_paged_kvcache(q: Tensor, cache: PagedKVCache, k: Optional[Te
     without a page are not seen. ``causal``: query i sees keys j <= rows - S + i, as in
     ``flash_attn_with_kvcache``. A query that sees no key gives a row of 0. Forward only: the call has
     no gradient."""
+    if cache_seqlens is None:
+        cache_seqlens = 0
+    native = _native_calls()
+    if native is not None:
+        out = native.paged(q, *cache, k, v, cache_seqlens, softmax_scale, causal, layer)
+        if out is not None:
+            return out
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(q.shape[-1])
-    lens, n = (cache_seqlens, 0) if isinstance(cache_seqlens, Tensor) else (None, int(cache_seqlens or 0))
+    lens, n = (cache_seqlens, 0) if isinstance(cache_seqlens, Tensor) else (None, int(cache_seqlens))
     return paged_kvcache_attn(q, k, v, *cache, lens, n, int(layer), bool(causal), float(softmax_scale))
 
 
@@ -234,6 +241,13 @@ def paged_kvcache_reserve(cache: PagedKVCache, cache_seqlens: Union[int, Tensor,
     shared page is left, its rows below ``cache_seqlens`` are copied, in every layer. Returns int32 [batch]:
     how many columns are left without a page of their own, 0 as long as pages last; new rows in these are not stored
     by ``flash_attn_with_paged_kvcache``. At most 8192 sequences."""
+    if cache_seqlens is None:
+        cache_seqlens = 0
+    native = _native_calls()
+    if native is not None:
+        short = native.pages_reserve(*cache, cache_seqlens, new_rows)
+        if short is not None:
+            return short
     lens, n = _rows(cache_seqlens, cache.page_table.shape[0], cache.page_table.device, "cache_seqlens")
     new, m = _rows(new_rows, cache.page_table.shape[0], cache.page_table.device, "new_rows")
     return _reserve(*cache, lens, n, new, m)
@@ -262,7 +276,9 @@ def paged_kvcache_fork(cache: PagedKVCache, parents: Tensor) -> None:
     each sequence a page of its own before it takes new rows. At most 8192 sequences."""
     if not isinstance(parents, Tensor):
         raise ValueError(f"parents must be int32 [{cache.page_table.shape[0]}] (got {type(parents).__name__})")
-    _fork(cache.refs, cache.page_table, parents)
+    native = _native_calls()
+    if native is None or native.pages_fork(cache.refs, cache.page_table, parents) is None:
+        _fork(cache.refs, cache.page_table, parents)
 
 
 @torch.library.custom_op("prefixlm::paged_kvcache_free", mutates_args=("refs", "page_table"))
@@ -286,8 +302,12 @@ def paged_kvcache_free(cache: PagedKVCache, keep_rows: Union[int, Tensor] = 0) -
     """Each sequence keeps the pages of its first ``keep_rows`` rows (an int, or int32 [batch] on the GPU) and
     gives up the others: 0 for a sequence that ended, its length to give up what draft tokens took, any
     number from columns * page_size on for one that keeps everything. A page that no one holds any more is free."""
+    page_size = cache.k_pages.shape[3]
+    native = _native_calls()
+    if native is not None and native.pages_free(cache.refs, cache.page_table, page_size, keep_rows) is not None:
+        return
     keep, n = _rows(keep_rows, cache.page_table.shape[0], cache.page_table.device, "keep_rows")
-    _free(cache.refs, cache.page_table, cache.k_pages.shape[3], keep, n)
+    _free(cache.refs, cache.page_table, page_size, keep, n)
 
 
 @torch.library.custom_op("prefixlm::paged_kvcache_compact", mutates_args=("k_pages", "v_pages", "refs", "page_table"))
@@ -310,7 +330,9 @@ def paged_kvcache_compact(cache: PagedKVCache) -> Tensor:
     """Moves the pages in use, U of them, to numbers below U, in every layer, and the table with them: the i-th used
     page from U on goes to the i-th free one below U. Returns U, int32 [1]: a pool of U pages holds it all
     (``paged_kvcache_copy``)."""
-    return _compact(*cache)
+    native = _native_calls()
+    used = native.pages_compact(*cache) if native is not None else None
+    return _compact(*cache) if used is None else used
 
 
 @torch.library.custom_op("prefixlm::paged_kvcache_copy", mutates_args=("k_pages", "v_pages"))
@@ -349,4 +371,7 @@ def paged_kvcache_copy(cache: PagedKVCache, src: Tensor, dst: Tensor, source: Op
     layer; src and dst are int32 [n] on the GPU. Pairs with a page outside its pool are skipped. The pages of dst
     differ from each other, and within one pool from those of src: else what they hold afterwards is not
     defined. Tables and refs stay as they are."""
+    native = _native_calls()
+    if native is not None and native.pages_copy(*cache, *((None,) * 4 if source is None else source), src, dst) is not None:
+        return
     _copy(cache.k_pages, cache.v_pages, *((source.k_pages, source.v_pages) if source is not None else (None, None)), src, dst)
