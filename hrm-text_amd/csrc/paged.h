@@ -14,8 +14,9 @@
 // The G query heads of a key-value head and the S queries are the R = S G rows that share its keys: row
 // r is query r / G of head h G + r % G. Kernels:
 //   decode  : up to four rows, split over the keys, without the matrix cores;
-//   stream  : 16 RT rows a workgroup, split over the keys. Each wave walks 32 keys at a time by itself,
-//             K as it lies in memory into the matrix cores, V through LDS of its own;
+//   stream  : up to 16 RT rows. Each wave walks 32 keys at a time by itself, through LDS of its own into the
+//             matrix cores;
+//   tile    : more rows: 64 or 128 a workgroup, which share tiles of the keys in LDS;
 //   combine : joins the splits.
 #pragma once
 #include "common.h"
@@ -637,6 +638,319 @@ __global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
     }
   }
   if (s_bad) walk_rows<D>(P, b, h, split, r0, r1, k0, k1, len);
+  append_share<D>(P, b, h, len, rb * P.nsplit + split, P.nrb * P.nsplit);
+}
+
+// ---- many rows -----------------------------------------------------------------------------------
+// Workgroup = 32 QW rows of (b, h, split): QW waves along the rows and KW = 4 / QW along the keys, as the
+// contiguous cache's extend kernel: a staged tile of 32 KW keys serves all of them, S^T = K Q^T with the
+// row as the lane column, V^T from transposing reads.
+template <int D, int QW>
+struct TileGeo {
+  static constexpr int KW = 4 / QW;
+  static constexpr int TK = 32 * KW;                     // keys a tile
+  static constexpr int CH = D / 8, RPP = NT / CH;        // 16-byte chunks of a row; rows that all threads load at once
+  static constexpr int NP = TK / RPP;
+  static constexpr int NDT = D / 32;
+  // rows 12 banks apart modulo 64 times an odd number, four rows 48: see RS in common.h
+  static constexpr int RSD = 2 * D + 48;
+  static constexpr int TILE = TK * RSD, BUF = 2 * TILE;  // K tile, V tile; two of them
+  static constexpr int OUT = 32 * (2 * D + 16);          // a wave's output rows
+  static constexpr int MERGE = 64 * 16 * NDT * 4 + 3 * 64 * 4;   // a wave's O, max, sum, seen
+  static constexpr int LDS_BYTES = 2 * BUF;
+  static_assert((4 - QW) * MERGE <= LDS_BYTES && QW * OUT <= LDS_BYTES, "epilogue areas fit");
+};
+
+template <int D, int QW>
+__global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
+  using G = TileGeo<D, QW>;
+  constexpr int KW = G::KW, TK = G::TK, NP = G::NP, NDT = G::NDT, NS = D / 16, CH = G::CH, RSD = G::RSD;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ int s_bad, s_hole;   // a value row or score is not finite; a tile had rows without a page
+  const int rb = (blockIdx.x >> 3) % P.nrb;
+  const int unit = (int)((blockIdx.x >> 3) / P.nrb) * 8 + (blockIdx.x & 7);
+  if (unit >= P.B * P.Hkv * P.nsplit) return;
+  const int split = unit % P.nsplit, bh = unit / P.nsplit;
+  const int h = bh % P.Hkv, b = bh / P.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qw = w % QW, kw = w / QW;
+  const int R = P.S * P.G, r0 = rb * 32 * QW, r1 = min(R, r0 + 32 * QW);
+  const int len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
+  const int lk = min(P.cap, len + P.s_new);
+  const int per = ((lk + P.nsplit - 1) / P.nsplit + TK - 1) / TK * TK;
+  const int k0 = split * per;
+  const int k1 = min(k0 + per, keys_seen(P, len, (r1 - 1) / P.G));
+  const int kall = keys_seen(P, len, r0 / P.G);                  // every row of the block sees the keys below
+  const int row = min(r0 + 32 * qw + l32, R - 1);                // this lane's (past the last: that one, not stored)
+  const int ri = row / P.G, rh = h * P.G + row % P.G;
+  const bool active = r0 + 32 * qw < R;
+  const int kq = min(k1, keys_seen(P, len, ri));
+  const int kend_w = active ? min(k1, keys_seen(P, len, (min(R, r0 + 32 * qw + 32) - 1) / P.G)) : 0;
+
+  uniform_i32* const tab = uniform(P.table + b * P.table_sb);
+  const int psm = (1 << P.ps_log2) - 1;
+  // staging: thread = chunk sch of rows srow + RPP n; V rows in permuted order
+  const int srow = tid / CH, sch = tid % CH, vrow = perm_row(srow);
+  const int g16 = __builtin_amdgcn_readfirstlane(srow & ~15);    // this wave's 16 keys of a pass
+  const bf16* const kn = P.s_new ? P.k + b * P.k_sb + h * P.k_sh + 8 * sch : nullptr;
+  const bf16* const vn = P.s_new ? P.v + b * P.v_sb + h * P.v_sh + 8 * sch : nullptr;
+  const uint32_t koff = (uint32_t)((srow & 15) * D + 8 * sch) * 2, voff = (uint32_t)((vrow & 15) * D + 8 * sch) * 2;
+  u32x4 ks[NP], vs[NP];
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  int page[NP];                 // of this wave's keys of the tile to load next
+  auto look = [&](int t0) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const int j = t0 + G::RPP * n + g16;
+      page[n] = j < len ? tab[j >> P.ps_log2] : -1;
+    }
+  };
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      const int j = t0 + G::RPP * n + g16;
+      const bool held = (unsigned)page[n] < (unsigned)P.P;
+      const int64_t at = ((((int64_t)(held ? page[n] : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
+      const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
+      if (held && j + 16 <= len) {
+        ks[n] = *reinterpret_cast<const u32x4*>(kb + koff);
+        vs[n] = *reinterpret_cast<const u32x4*>(vb + voff);
+      } else {
+        // the last cached rows, the new ones, none: row by row
+        if (j < min(len, k1) && !held) s_hole = 1;
+        const int jk = j + (srow & 15), jv = j + (vrow & 15);
+        ks[n] = vs[n] = zero;
+        if (jk < len ? held : jk < k1)
+          ks[n] = *reinterpret_cast<const u32x4*>(jk < len ? kb + koff : reinterpret_cast<const char*>(kn + (jk - len) * P.k_ss));
+        if (jv < len ? held : jv < k1)
+          vs[n] = *reinterpret_cast<const u32x4*>(jv < len ? vb + voff : reinterpret_cast<const char*>(vn + (jv - len) * P.v_ss));
+      }
+    }
+  };
+  u16x2 vmag = {0, 0};
+  auto store = [&](int buf) {
+    char* base = smem + buf * G::BUF + srow * RSD + sch * 16;
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      *reinterpret_cast<u32x4*>(base + G::RPP * n * RSD) = ks[n];
+      *reinterpret_cast<u32x4*>(base + G::TILE + G::RPP * n * RSD) = vs[n];
+      vmag = max_mag(vmag, vs[n]);
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.f, seen = 0.f;
+  f32x16 oacc[NDT];
+#pragma unroll
+  for (int t = 0; t < NDT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) oacc[t][r] = 0.f;
+  if (tid == 0) s_bad = 0, s_hole = 0;
+  __syncthreads();
+
+  if (k0 < k1) {
+    const int nt = (k1 - k0 + TK - 1) / TK;
+    look(k0);
+    load(k0);
+    look(k0 + TK);
+    // Q^T fragments: lane holds its row, columns 16 s + 8 hh + 0..7
+    bf16x8 qf[NS];
+    {
+      const bf16* qp = P.q + b * P.q_sb + ri * P.q_ss + rh * P.q_sh + 8 * hh;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 16 * s);
+    }
+    store(0);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) settle(__builtin_bit_cast(u32x4, qf[s]));
+    __syncthreads();
+    const float c = P.scale_log2;
+    for (int t = 0; t < nt; ++t) {
+      const int buf = t & 1;
+      if (t + 1 < nt) {
+        load(k0 + (t + 1) * TK);
+        look(k0 + (t + 2) * TK);
+      }
+      const int kk = k0 + t * TK + 32 * kw;   // first key of this wave's 32
+      if (kk < kend_w) {
+        const char* kt = smem + buf * G::BUF + (32 * kw + l32) * RSD + hh * 16;
+        const char* vt = smem + buf * G::BUF + G::TILE + 32 * kw * RSD + xt_lane_off<RSD>(lane);
+        f32x16 sacc;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sacc[r] = 0.f;
+        bf16x8 ka[NS];
+        ka[0] = *reinterpret_cast<const bf16x8*>(kt);
+        ka[1] = *reinterpret_cast<const bf16x8*>(kt + 32);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {   // operands two steps ahead
+          if (s + 2 < NS) ka[s + 2] = *reinterpret_cast<const bf16x8*>(kt + 32 * (s + 2));
+          sched_fence();
+          sacc = mfma32x32x16(ka[s], qf[s], sacc);
+          sched_fence();
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sacc[r] *= c;   // before the mask: the scale may have any sign
+        const bool hole = s_hole != 0;
+        if (kk + 32 > min(kall, k1) || hole) {
+          // key kk + 8 (r / 4) + 4 hh + r % 4 is seen iff it is below kq, and cached ones have a page
+          bool ok[2];
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int j = kk + 16 * g;
+            ok[g] = !hole || j >= len || (unsigned)tab[j >> P.ps_log2] < (unsigned)P.P;
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = kk + 8 * (r >> 2) + 4 * hh + (r & 3);
+            const bool sees = j < kq && (ok[r >> 3] || j >= len);
+            seen = sees ? 1.f : seen;
+            sacc[r] = sees ? sacc[r] : -INFINITY;
+          }
+        } else {
+          seen = 1.f;
+        }
+        float mx = sacc[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sacc[r]);
+        mx = halves_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m_run) != 0) {
+          const float m_new = fmaxf(m_run, mx);
+          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+          m_run = m_new;
+          l_run *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) oacc[dt][r] *= alpha;
+        }
+        const float m_use = max_ref(m_run);
+        u32x4 xt[2 * NDT];
+        xt[0] = lds_read_xt<RSD>(vt, 0, 0);
+        xt[1] = lds_read_xt<RSD>(vt, 0, 1);
+        // 16 keys at a time: P's three bf16 terms, which add up to its fp32 bits, times V
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float e[8], ps = 0.f;
+          bf16x8 pt[3];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(sacc[8 * half + i] - m_use);
+            ps += e[i];
+          }
+          l_run += ps;
+#pragma unroll
+          for (int n = 0; n < 3; ++n) {
+            u32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              x[i] = pack_hi(__builtin_bit_cast(uint32_t, e[2 * i]), __builtin_bit_cast(uint32_t, e[2 * i + 1]));
+            pt[n] = __builtin_bit_cast(bf16x8, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)   // exact
+              e[i] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, e[i]) & 0xffff0000u);
+          }
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) {
+            const int x = NDT * half + dt;
+            if (x + 2 < 2 * NDT) xt[x + 2] = lds_read_xt<RSD>(vt, (x + 2) / NDT, (x + 2) % NDT);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[x]), pt[n], oacc[dt]);
+          }
+        }
+      }
+      if (t + 1 < nt) store(buf ^ 1);
+      __syncthreads();
+    }
+  }
+  l_run = halves_sum(l_run);
+  // a score past the range upwards leaves NaN; one past it downwards (raw below -3.4e38) only counts
+  // where every key that the row sees here scores about as low
+  if (vmag[0] >= 0x7f80 || vmag[1] >= 0x7f80 || (seen != 0.f && (l_run != l_run || m_run < 200.f - 3e38f * fabsf(P.scale_log2))))
+    s_bad = 1;
+  seen = halves_max(seen);
+  // the KW waves of 32 rows: waves kw > 0 hand theirs to wave kw = 0
+  if (KW > 1) {
+    if (kw > 0) {
+      float* area = reinterpret_cast<float*>(smem + (w - QW) * G::MERGE);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          *reinterpret_cast<f32x4*>(area + ((4 * dt + m) * 64 + lane) * 4) =
+              f32x4{oacc[dt][4 * m], oacc[dt][4 * m + 1], oacc[dt][4 * m + 2], oacc[dt][4 * m + 3]};
+      area += 64 * 16 * NDT;
+      area[lane] = m_run;
+      area[64 + lane] = l_run;
+      area[128 + lane] = seen;
+    }
+    __syncthreads();
+    if (kw == 0) {
+      float mo[KW], M = m_run;
+#pragma unroll
+      for (int g = 1; g < KW; ++g) {
+        mo[g] = reinterpret_cast<const float*>(smem + (g * QW + qw - QW) * G::MERGE)[64 * 16 * NDT + lane];
+        M = fmaxf(M, mo[g]);
+      }
+      mo[0] = m_run;
+      m_run = M;
+      float L = 0.f;
+#pragma unroll
+      for (int g = 0; g < KW; ++g) {
+        const float* area = reinterpret_cast<const float*>(smem + (g * QW + qw - QW) * G::MERGE);
+        const float wgt = mo[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mo[g] - M);
+        L += wgt * (g == 0 ? l_run : area[64 * 16 * NDT + 64 + lane]);
+        if (g) seen = fmaxf(seen, area[64 * 16 * NDT + 128 + lane]);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            if (g == 0) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) oacc[dt][4 * m + e] *= wgt;
+            } else {
+              const f32x4 x = *reinterpret_cast<const f32x4*>(area + ((4 * dt + m) * 64 + lane) * 4);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) oacc[dt][4 * m + e] += wgt * x[e];
+            }
+          }
+      }
+      l_run = L;
+    }
+  }
+  __syncthreads();
+  if (s_bad) {
+    walk_rows<D>(P, b, h, split, r0, r1, k0, k1, len);
+  } else if (kw == 0 && active) {
+    if (P.nsplit == 1) {
+      // whole rows through LDS
+      constexpr int ORS = 2 * D + 16;
+      const float inv = row_inv(seen != 0.f, l_run);
+      char* wl = smem + qw * G::OUT;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          *reinterpret_cast<bf16x4*>(wl + l32 * ORS + (32 * dt + 8 * m + 4 * hh) * 2) =
+              cvt4(oacc[dt][4 * m] * inv, oacc[dt][4 * m + 1] * inv, oacc[dt][4 * m + 2] * inv,
+                   oacc[dt][4 * m + 3] * inv);
+#pragma unroll
+      for (int n = 0; n < 32 / (64 / CH); ++n) {
+        const int rr = lane / CH + (64 / CH) * n, r = r0 + 32 * qw + rr;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(wl + rr * ORS + (lane % CH) * 16);
+        if (r < R)
+          *reinterpret_cast<u32x4*>(P.out + b * P.o_sb + (r / P.G) * P.o_ss + (h * P.G + r % P.G) * P.o_sh + 8 * (lane % CH)) = v;
+      }
+    } else if (r0 + 32 * qw + l32 < R) {
+      float* dst = P.part + (((int64_t)bh * R + row) * P.nsplit + split) * kPart<D>;
+      if (hh == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{m_run, l_run, seen, 0.f};
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          *reinterpret_cast<f32x4*>(dst + 4 + 32 * dt + 8 * m + 4 * hh) =
+              f32x4{oacc[dt][4 * m], oacc[dt][4 * m + 1], oacc[dt][4 * m + 2], oacc[dt][4 * m + 3]};
+    }
+  }
   append_share<D>(P, b, h, len, rb * P.nsplit + split, P.nrb * P.nsplit);
 }
 

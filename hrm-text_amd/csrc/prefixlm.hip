@@ -1878,29 +1878,58 @@ static int table_check(const prefixlm_page_pool& p) {
 }
 static int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
-// Rows that share a key-value head's keys, and the row blocks and key splits of their kernel.
-static int pg_rt(int64_t R) { return R <= 4 ? 0 : R <= 16 ? 1 : 2; }
-static int64_t pg_nrb(int64_t R) { return pg_rt(R) ? (R + 16 * pg_rt(R) - 1) / (16 * pg_rt(R)) : 1; }
+// R rows share a key-value head's keys: how they are cut into blocks, and the keys into splits.
+static int pg_rows(int64_t R) { return R <= 4 ? 4 : R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }   // of a block
+static int64_t pg_nrb(int64_t R) { return (R + pg_rows(R) - 1) / pg_rows(R); }
 static int64_t pg_nsplit(int64_t B, int64_t Hkv, int64_t R, int64_t cap) {
   const int64_t units = B * Hkv * pg_nrb(R), most = (cap + 4 * pkv::kKeys - 1) / (4 * pkv::kKeys);
-  return std::max<int64_t>(1, std::min({(768 + units - 1) / units, most, (int64_t)pkv::kMaxSplits}));
+  return std::max<int64_t>(1, std::min({((R > 4 ? 512 : 768) + units - 1) / units, most, (int64_t)pkv::kMaxSplits}));
 }
 
 template <int D>
 static void pg_launch(const pkv::Params& P, int64_t nblk, hipStream_t stream) {
   const int64_t R = (int64_t)P.S * P.G;
-  if (R == 1)
-    hipLaunchKernelGGL((pkv::decode_kernel<D, 1, pkv::NT>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
-  else if (R == 2)
-    hipLaunchKernelGGL((pkv::decode_kernel<D, 2, pkv::NT>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
-  else if (pg_rt(R) == 0)
-    hipLaunchKernelGGL((pkv::decode_kernel<D, 4, pkv::NT>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
-  else if (pg_rt(R) == 1)
-    hipLaunchKernelGGL((pkv::stream_kernel<D, 1>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
-  else
-    hipLaunchKernelGGL((pkv::stream_kernel<D, 2>), dim3((unsigned)nblk), dim3(pkv::NT), 0, stream, P);
+  const dim3 g((unsigned)nblk), n(pkv::NT);
+  switch (pg_rows(R)) {
+    case 4:
+      if (R == 1)
+        hipLaunchKernelGGL((pkv::decode_kernel<D, 1, pkv::NT>), g, n, 0, stream, P);
+      else if (R == 2)
+        hipLaunchKernelGGL((pkv::decode_kernel<D, 2, pkv::NT>), g, n, 0, stream, P);
+      else
+        hipLaunchKernelGGL((pkv::decode_kernel<D, 4, pkv::NT>), g, n, 0, stream, P);
+      break;
+    case 16:
+      hipLaunchKernelGGL((pkv::stream_kernel<D, 1>), g, n, 0, stream, P);
+      break;
+    case 32:
+      hipLaunchKernelGGL((pkv::stream_kernel<D, 2>), g, n, 0, stream, P);
+      break;
+    case 64:
+      hipLaunchKernelGGL((pkv::tile_kernel<D, 2>), g, n, (pkv::TileGeo<D, 2>::LDS_BYTES), stream, P);
+      break;
+    default:
+      hipLaunchKernelGGL((pkv::tile_kernel<D, 4>), g, n, (pkv::TileGeo<D, 4>::LDS_BYTES), stream, P);
+  }
   if (P.nsplit > 1)
     hipLaunchKernelGGL((pkv::combine_kernel<D>), dim3((unsigned)((P.B * P.Hkv * R + 3) / 4)), dim3(256), 0, stream, P);
+}
+static_assert(pkv::TileGeo<128, 4>::LDS_BYTES <= 65536 && pkv::TileGeo<64, 2>::LDS_BYTES <= 65536, "within the default limit");
+// The one tile whose LDS is above the default limit, allowed once per device
+static int pg_allow_lds() {
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = -1;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "hipGetDevice: %s", hipGetErrorString(e));
+  if (dev < 0 || dev >= 64) return fail(PREFIXLM_ERR_INVALID, "device %d >= 64", dev);
+  std::lock_guard<std::mutex> g(mu);
+  if (done[dev]) return PREFIXLM_OK;
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&pkv::tile_kernel<128, 2>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          (pkv::TileGeo<128, 2>::LDS_BYTES));
+  if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
+  done[dev] = true;
+  return PREFIXLM_OK;
 }
 
 extern "C" {
@@ -1977,7 +2006,9 @@ int prefixlm_paged_fwd(const prefixlm_paged_args* a, void* stream_) {
   if (units > 0x7fffffff || P.nrb > 0x7fffffff / ((units + 7) / 8 * 8) || !launchable((units + 7) / 8 * 8 * P.nrb, pkv::NT) ||
       !launchable(((int64_t)P.B * P.Hkv * R + 3) / 4, 256))
     return fail(PREFIXLM_ERR_INVALID, "grid too large");
-  const int64_t nblk = pg_rt(R) ? (units + 7) / 8 * 8 * P.nrb : units;
+  const int64_t nblk = pg_rows(R) > 4 ? (units + 7) / 8 * 8 * P.nrb : units;
+  rc = pg_allow_lds();
+  if (rc) return rc;
   (void)hipGetLastError();
   if (pool.head_dim == 128)
     pg_launch<128>(P, nblk, stream);
