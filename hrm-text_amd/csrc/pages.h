@@ -25,54 +25,71 @@ __device__ __forceinline__ void arrive() {
   __syncthreads();
 }
 
-// Sum of x over the threads before this one, and over all (NTH threads). s: 17 ints
+// Sum of x over the lanes up to this one
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
+  return x;
+}
+// Sum of x over the threads before this one, and over all (NTH threads). s: 16 ints
 __device__ __forceinline__ int scan(int x, int* s, int* total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int y = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int z = __shfl_up(y, d);
-    if (lane >= d) y += z;
-  }
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, y = wave_scan(x);
   __syncthreads();   // s may be in use
   if (lane == 63) s[w] = y;
   __syncthreads();
-  if (threadIdx.x < 64) {
-    int v = lane < NTH / 64 ? s[lane] : 0;
+  int before = 0, all = 0;
 #pragma unroll
-    for (int d = 1; d < NTH / 64; d <<= 1) {
-      const int z = __shfl_up(v, d);
-      if (lane >= d) v += z;
-    }
-    if (lane < NTH / 64) s[lane] = v;
+  for (int i = 0; i < NTH / 64; ++i) {
+    before += i < w ? s[i] : 0;
+    all += s[i];
   }
-  __syncthreads();
-  *total = s[NTH / 64 - 1];
-  return y - x + (w ? s[w - 1] : 0);
+  *total = all;
+  return y - x + before;
 }
 
-// The numbers p of [p0, P) for which pick(p, refs[p]), in order, 16384 at a time, into list[0, n): ends after
-// the first 16384 that bring the count to `want`. Returns the count, which may pass `cap` numbers: those are
-// counted, not written.
-constexpr int kPer = 16;           // of one thread
-template <class Pick>
-__device__ __forceinline__ int list_pages(const int32_t* refs, int P, int want, int cap, int32_t* list, int* s, Pick pick) {
-  int n = 0;
-  for (int base = 0; base < P && n < want; base += NTH * kPer) {
-    const int p0 = base + kPer * (int)threadIdx.x;
-    int32_t x[kPer];
+// 16 counts a thread, 16384 pages the workgroup: from page `base` on, 0 past the end
+constexpr int kPer = 16, kLook = NTH * kPer;
+__device__ __forceinline__ void look(const int32_t* refs, int P, int base, int32_t (&x)[kPer]) {
+  typedef int32_t i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+  const int p0 = base + kPer * (int)threadIdx.x;
+  if (p0 + kPer <= P) {
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+      const i32x4 y = *reinterpret_cast<const i32x4*>(refs + p0 + i);
+      x[i] = y[0], x[i + 1] = y[1], x[i + 2] = y[2], x[i + 3] = y[3];
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = p0 + i < P ? refs[p0 + i] : 0;
-    uint32_t mask = 0;
+  }
+}
+// Bit i: pick(p, x[i]) for the page p = base + 16 thread + i
+template <class Pick>
+__device__ __forceinline__ uint32_t picked(int P, int base, const int32_t (&x)[kPer], Pick pick) {
+  const int p0 = base + kPer * (int)threadIdx.x;
+  uint32_t mask = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) mask |= (p0 + i < P && pick(p0 + i, x[i]) ? 1u : 0u) << i;
+  for (int i = 0; i < kPer; ++i) mask |= (p0 + i < P && pick(p0 + i, x[i]) ? 1u : 0u) << i;
+  return mask;
+}
+// The pages for which pick(p, refs[p]), in order, 16384 at a time (the first of them given in x), by put_one(rank, p):
+// ends after the first 16384 that bring the count to `want`. Returns the count.
+template <class Pick, class Put>
+__device__ __forceinline__ int list_pages(const int32_t* refs, int P, int want, int32_t (&x)[kPer], int* s, Pick pick, Put put_one) {
+  int n = 0;
+  for (int base = 0; base < P && n < want; base += kLook) {
+    if (base) look(refs, P, base, x);
+    uint32_t mask = picked(P, base, x, pick);
     int total;
     int at = n + scan(__popc(mask), s, &total);
     while (mask) {
       const int i = __ffs(mask) - 1;
       mask &= mask - 1;
-      if (at < cap) put(list + at, p0 + i);
-      ++at;
+      put_one(at++, base + kPer * (int)threadIdx.x + i);
     }
     n += total;
   }
@@ -106,11 +123,18 @@ __device__ __forceinline__ void columns(const ReserveParams& P, int n, int* c0, 
 
 // One workgroup. The columns of all sequences, in order, are its items. An item needs a page if it has
 // none, or one that others hold too: unless all who hold it ask here and it is the first of them. The k-th
-// that needs one gets the k-th lowest free page.
+// that needs one gets the k-th lowest free page. Bound by the chain of dependent loads and barriers: lengths,
+// entries, their counts, and the scan of the free pages meanwhile. Up to 1024 items keep what they know in
+// registers and meet in a table in LDS; more go through the workspace, round after round.
+constexpr int kSlots = 2 * NTH;    // of the table
 __global__ __launch_bounds__(NTH) void reserve_kernel(ReserveParams P) {
   __shared__ int s_off[kMaxSeqs + 1];   // items before sequence n
-  __shared__ int s_scan[NTH / 64 + 1], s_copies;
+  __shared__ int s_scan[NTH / 64], s_copies;
+  __shared__ int s_page[kSlots], s_asks[kSlots], s_first[kSlots], s_free[NTH];
   const int tid = threadIdx.x;
+  int32_t refs[kPer];
+  look(P.refs, P.P, 0, refs);
+  for (int i = tid; i < kSlots; i += NTH) s_page[i] = -1, s_asks[i] = 0, s_first[i] = 0x7fffffff;
   if (tid == 0) s_copies = 0;
   int W = 0;
   for (int base = 0; base < P.N; base += NTH) {
@@ -126,7 +150,7 @@ __global__ __launch_bounds__(NTH) void reserve_kernel(ReserveParams P) {
     W += total;
   }
   if (tid == 0) s_off[P.N] = W;
-  arrive();
+  __syncthreads();
   // item -> its sequence, column, entry
   auto item = [&](int it, int* n, int* c, int32_t** e, int* rest) {
     int lo = 0, hi = P.N;
@@ -141,57 +165,79 @@ __global__ __launch_bounds__(NTH) void reserve_kernel(ReserveParams P) {
     *e = P.table + lo * P.table_sb + *c;
     *rest = *c == c0 ? len & ((1 << P.ps_log2) - 1) : 0;
   };
-  int n, c, rest;
-  int32_t* e;
-  for (int it = tid; it < W; it += NTH) {
-    item(it, &n, &c, &e, &rest);
-    const int p = *e;
-    if ((unsigned)p >= (unsigned)P.P) continue;
-    put(P.was + 3 * (int64_t)p, P.refs[p]);
-    put(P.was + 3 * (int64_t)p + 1, 0);
-    put(P.was + 3 * (int64_t)p + 2, 0x7fffffff);
-  }
-  arrive();
-  for (int it = tid; it < W; it += NTH) {
-    item(it, &n, &c, &e, &rest);
-    const int p = *e;
-    if ((unsigned)p >= (unsigned)P.P) continue;
-    add(P.was + 3 * (int64_t)p + 1, 1);
-    lower(P.was + 3 * (int64_t)p + 2, it);
-  }
-  const int nfree = W ? list_pages(P.refs, P.P, W, W, P.free_list, s_scan, [](int, int32_t r) { return r == 0; }) : 0;
-  arrive();
-  int needed = 0;
-  for (int base = 0; base < W; base += NTH) {
-    const int it = base + tid;
-    bool needs = false, leaves = false;
+  int n = 0, c, rest = 0;
+  int32_t* e = nullptr;
+  auto grant = [&](int to, int p, bool leaves) {
+    put(e, to);
+    put(P.refs + to, 1);
+    if (!leaves) return;
+    add(P.refs + p, -1);
+    if (!rest) return;
+    int32_t* q = P.copies + 1 + 3 * atomicAdd(&s_copies, 1);
+    q[0] = p, q[1] = to, q[2] = rest;
+  };
+  auto is_free = [](int, int32_t r) { return r == 0; };
+  int needed = 0, nfree = 0;
+  if (W <= NTH) {
     int p = -1;
-    if (it < W) {
-      item(it, &n, &c, &e, &rest);
+    if (tid < W) {
+      item(tid, &n, &c, &e, &rest);
       p = *e;
-      if ((unsigned)p < (unsigned)P.P) {
-        const int32_t* was = P.was + 3 * (int64_t)p;
-        const int holders = fresh(was);
-        leaves = holders > 1 && !(fresh(was + 1) == holders && fresh(was + 2) == it);
-        needs = leaves;
-      } else {
-        needs = true;
-      }
     }
-    int total;
-    const int rank = needed + scan(needs ? 1 : 0, s_scan, &total);
-    needed += total;
-    if (needs && rank < nfree) {
-      const int to = fresh(P.free_list + rank);
-      put(e, to);
-      put(P.refs + to, 1);
-      if (leaves) {
-        add(P.refs + p, -1);
-        if (rest) {
-          int32_t* q = P.copies + 1 + 3 * atomicAdd(&s_copies, 1);
-          q[0] = p, q[1] = to, q[2] = rest;
+    if (W) nfree = list_pages(P.refs, P.P, W, refs, s_scan, is_free, [&](int k, int page) { if (k < NTH) s_free[k] = page; });
+    const bool held = (unsigned)p < (unsigned)P.P;
+    const int holders = tid < W && held ? P.refs[p] : 0;
+    int at = (int)(((uint32_t)p * 2654435761u) >> 21);   // of 2048 slots, which at most half are taken
+    if (holders > 1) {
+      for (;; at = (at + 1) & (kSlots - 1)) {
+        const int old = atomicCAS(&s_page[at], -1, p);
+        if (old == -1 || old == p) break;
+      }
+      atomicAdd(&s_asks[at], 1);
+      atomicMin(&s_first[at], tid);
+    }
+    __syncthreads();
+    const bool leaves = holders > 1 && !(s_asks[at] == holders && s_first[at] == tid);
+    const bool needs = tid < W && (!held || leaves);
+    const int rank = scan(needs ? 1 : 0, s_scan, &needed);
+    if (needs && rank < nfree) grant(s_free[rank], p, leaves);
+  } else {
+    for (int it = tid; it < W; it += NTH) {
+      item(it, &n, &c, &e, &rest);
+      const int p = *e;
+      if ((unsigned)p >= (unsigned)P.P) continue;
+      put(P.was + 3 * (int64_t)p, P.refs[p]);
+      put(P.was + 3 * (int64_t)p + 1, 0);
+      put(P.was + 3 * (int64_t)p + 2, 0x7fffffff);
+    }
+    arrive();
+    for (int it = tid; it < W; it += NTH) {
+      item(it, &n, &c, &e, &rest);
+      const int p = *e;
+      if ((unsigned)p >= (unsigned)P.P) continue;
+      add(P.was + 3 * (int64_t)p + 1, 1);
+      lower(P.was + 3 * (int64_t)p + 2, it);
+    }
+    nfree = list_pages(P.refs, P.P, W, refs, s_scan, is_free, [&](int k, int page) { if (k < W) put(P.free_list + k, page); });
+    arrive();
+    for (int base = 0; base < W; base += NTH) {
+      const int it = base + tid;
+      bool needs = false, leaves = false;
+      int p = -1;
+      if (it < W) {
+        item(it, &n, &c, &e, &rest);
+        p = *e;
+        needs = (unsigned)p >= (unsigned)P.P;
+        if (!needs) {
+          const int32_t* was = P.was + 3 * (int64_t)p;
+          const int holders = fresh(was), asks = fresh(was + 1), first = fresh(was + 2);
+          needs = leaves = holders > 1 && !(asks == holders && first == it);
         }
       }
+      int total;
+      const int rank = needed + scan(needs ? 1 : 0, s_scan, &total);
+      needed += total;
+      if (needs && rank < nfree) grant(fresh(P.free_list + rank), p, leaves);
     }
   }
   arrive();
@@ -203,6 +249,7 @@ __global__ __launch_bounds__(NTH) void reserve_kernel(ReserveParams P) {
       if ((unsigned)p >= (unsigned)P.P || fresh(P.refs + p) > 1) add(P.short_ + n, 1);
     }
 }
+static_assert(kSlots == 2048, "the slot is 11 bits");
 
 // ---- fork -----------------------------------------------------------------------------------
 struct ForkParams {
@@ -263,24 +310,63 @@ struct CompactParams {
   int64_t table_sb;
   int N, M, P;
 };
-// One workgroup. U pages are in use: the i-th of them from U on moves to the i-th free one below U.
+// One workgroup. U pages are in use: the i-th of them from U on moves to the i-th free one below U. Pools of up to
+// 16384 pages stay in registers between the two looks at their counts; the free ones meet the others in LDS.
 __global__ __launch_bounds__(NTH) void compact_kernel(CompactParams P) {
-  __shared__ int s_scan[NTH / 64 + 1];
+  __shared__ int s_scan[NTH / 64];
+  __shared__ uint16_t s_hole[kLook / 2];
   const int tid = threadIdx.x;
-  int mine = 0, U;
-  for (int p = tid; p < P.P; p += NTH) mine += P.refs[p] > 0;
-  (void)scan(mine, s_scan, &U);
   int32_t* const list = P.moves + 1;
+  int32_t x[kPer];
+  look(P.refs, P.P, 0, x);
+  int mine = 0, U, half;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) mine += x[i] > 0;
+  for (int p = kLook + tid; p < P.P; p += NTH) mine += P.refs[p] > 0;
+  (void)scan(mine, s_scan, &U);
   // free below U, then used above: as many of one as of the other, and in this order by number
-  const int n = list_pages(P.refs, P.P, 0x7fffffff, 2 * P.P, list, s_scan, [U](int p, int32_t r) { return (p < U) != (r > 0); });
-  for (int p = U + tid; p < P.P; p += NTH) put(P.to + p, p);
-  arrive();
-  const int half = n >> 1;
-  for (int i = tid; i < half; i += NTH) {
-    const int dst = fresh(list + i), src = fresh(list + half + i);
-    put(P.to + src, dst);
-    P.refs[dst] = P.refs[src];
-    P.refs[src] = 0;
+  auto pick = [U](int p, int32_t r) { return (p < U) != (r > 0); };
+  if (P.P <= kLook) {
+    const uint32_t mask = picked(P.P, 0, x, pick);
+    int total;
+    const int at0 = scan(__popc(mask), s_scan, &total);
+    half = total >> 1;
+    int at = at0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int p = kPer * tid + i;
+      if ((mask >> i & 1) && p < U) s_hole[at++] = (uint16_t)p;
+    }
+    __syncthreads();
+    at = at0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int p = kPer * tid + i;
+      if (p >= U && p < P.P) {
+        int dst = p;
+        if (mask >> i & 1) {
+          dst = s_hole[at - half];
+          list[at - half] = dst;
+          list[at++] = p;
+          P.refs[dst] = x[i];
+          P.refs[p] = 0;
+        }
+        P.to[p] = dst;
+      } else {
+        at += mask >> i & 1;
+      }
+    }
+  } else {
+    const int n = list_pages(P.refs, P.P, 0x7fffffff, x, s_scan, pick, [&](int k, int p) { put(list + k, p); });
+    half = n >> 1;
+    for (int p = U + tid; p < P.P; p += NTH) put(P.to + p, p);
+    arrive();
+    for (int i = tid; i < half; i += NTH) {
+      const int dst = fresh(list + i), src = fresh(list + half + i);
+      put(P.to + src, dst);
+      P.refs[dst] = P.refs[src];
+      P.refs[src] = 0;
+    }
   }
   if (tid == 0) {
     P.moves[0] = half;
@@ -305,8 +391,10 @@ struct CopyParams {
   int64_t table_sb;
   int N, M, n_remap;        // workgroups that do so, before the others
 };
-// A wave has 4 KB of one head of one pair's page: four loads of 16 bytes a lane on their way
-// together. blockIdx.y: layer and keys or values. heads = 1: a page's heads as one.
+typedef const __attribute__((address_space(4))) int32_t uniform_i32;   // through the scalar cache
+// A wave has 4 KB of one head of one pair's page at a time, four loads of 16 bytes a lane, and loads the next before
+// it stores these. blockIdx.y: layer and keys or values. heads = 1: a page's heads as one. Bound by memory (1.26
+// GB in and out 247 us, 5.1 TB/s); little by its chain of count, pair, load and store.
 __global__ __launch_bounds__(256) void copy_kernel(CopyParams P) {
   int blk = blockIdx.x;
   if (blk < P.n_remap) {
@@ -323,34 +411,53 @@ __global__ __launch_bounds__(256) void copy_kernel(CopyParams P) {
   const int lane = threadIdx.x & 63;
   const uint32_t w = (uint32_t)__builtin_amdgcn_readfirstlane(blk * 4 + (threadIdx.x >> 6));
   const uint32_t nw = 4 * (gridDim.x - P.n_remap);
-  const int n = P.count ? *P.count : P.n, kv = blockIdx.y & 1;
+  const int n = P.count ? *(uniform_i32*)(uintptr_t)P.count : P.n, kv = blockIdx.y & 1;
   const int64_t layer = blockIdx.y >> 1;
   const bf16* from = P.from[kv] + layer * P.from_layer;
   bf16* to = P.to[kv] + layer * P.to_layer;
-  const uint32_t per = (uint32_t)P.heads * P.pieces;   // of a pair; n per < 2^31
-  for (uint32_t u = w; u < n * per; u += nw) {
-    const uint32_t pair = u / per, x = u - pair * per, head = x / P.pieces, piece = x - head * P.pieces;
+  uniform_i32 *const src = (uniform_i32*)(uintptr_t)P.src, *const dst = (uniform_i32*)(uintptr_t)P.dst;
+  const uint32_t per = (uint32_t)P.heads * P.pieces, total = n * per;   // n per < 2^31
+  struct Piece {
+    bf16* d;
+    int elems;               // of the head from this piece on; 0: nothing
+    u32x4 v[4];
+  };
+  auto load = [&](uint32_t u, Piece& x) {
+    x.elems = 0;
+    if (u >= total) return;
+    const uint32_t pair = u / per, y = u - pair * per, head = y / P.pieces, piece = y - head * P.pieces;
     int a, b, elems = P.head_elems;
     if (P.rows) {
-      a = P.src[3 * pair], b = P.src[3 * pair + 1];
-      elems = P.src[3 * pair + 2] * P.row_elems;
+      a = src[3 * pair], b = src[3 * pair + 1];
+      elems = src[3 * pair + 2] * P.row_elems;
     } else {
-      a = P.src ? P.src[pair] : P.dst[n + pair], b = P.dst[pair];
+      b = dst[pair], a = P.src ? src[pair] : dst[n + pair];
     }
-    if ((unsigned)a >= (unsigned)P.P_from || (unsigned)b >= (unsigned)P.P_to) continue;
-    const bf16* s = from + ((int64_t)a * P.heads + head) * P.head_elems;
-    bf16* d = to + ((int64_t)b * P.heads + head) * P.head_elems;
-    u32x4 v[4];
+    if ((unsigned)a >= (unsigned)P.P_from || (unsigned)b >= (unsigned)P.P_to) return;
+    const bf16* s = from + ((int64_t)a * P.heads + head) * P.head_elems + piece * 2048;
+    x.d = to + ((int64_t)b * P.heads + head) * P.head_elems + piece * 2048;
+    x.elems = elems - (int)piece * 2048;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = piece * 2048 + 8 * (64 * i + lane);
-      if (at < elems) v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(s + at));
+      const int at = 8 * (64 * i + lane);
+      if (at < x.elems) x.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(s + at));
     }
+  };
+  auto store = [&](const Piece& x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = piece * 2048 + 8 * (64 * i + lane);
-      if (at < elems) __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4*>(d + at));
+      const int at = 8 * (64 * i + lane);
+      if (at < x.elems) __builtin_nontemporal_store(x.v[i], reinterpret_cast<u32x4*>(x.d + at));
     }
+  };
+  // total < 2^31 and a step is below 2^17: no overflow
+  Piece x, y;
+  load(w, x);
+  for (uint32_t u = w; u < total; u += 2 * nw) {
+    load(u + nw, y);
+    store(x);
+    load(u + 2 * nw, x);
+    store(y);
   }
 }
 
