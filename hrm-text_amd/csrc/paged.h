@@ -13,11 +13,14 @@
 //
 // The G query heads of a key-value head and the S queries are the R = S G rows that share its keys: row
 // r is query r / G of head h G + r % G. Kernels:
-//   decode  : up to four rows, split over the keys, without the matrix cores;
-//   stream  : up to 16 RT rows. Each wave walks 32 keys at a time by itself, through LDS of its own into the
+//   decode  : one row, without the matrix cores;
+//   stream  : up to 16 rows. Each wave walks 32 keys at a time by itself, through LDS of its own into the
 //             matrix cores;
 //   tile    : more rows: 64 or 128 a workgroup, which share tiles of the keys in LDS;
-//   combine : joins the splits.
+//   combine : joins the pieces of a unit.
+//
+// A unit is a block of rows of one (sequence, key-value head); its keys are tiles. Where units are few, each is cut
+// into pieces, as many as its sequence's tiles are worth, so that sequences of any lengths end together (Sched).
 #pragma once
 #include "common.h"
 #include "kvcache.h"
@@ -31,7 +34,7 @@ using kvc::max_ref;
 constexpr int NT = 256;
 constexpr int NWAVE = NT / 64;
 constexpr int kKeys = 32;          // keys of a wave's step
-constexpr int kMaxSplits = 64;
+constexpr int kMaxShared = 256;    // sequences of a call whose units are cut
 // floats per partial: max (log2 units), sum, whether a key was seen, unused, o[D]
 template <int D>
 constexpr int kPart = D + 4;
@@ -45,12 +48,14 @@ struct Params {
   const int32_t* refs;     // [P]
   const int32_t* table;    // [B, M]
   bf16* out;
-  float* part;             // [B, Hkv, R, nsplit, kPart]
+  float* part;             // [workgroups, rows of a block, kPart]: a piece's result, where it is not the whole unit's
+  int32_t* pre;            // [B + 1]: workgroups before each sequence, from the first one for the combine
   const int32_t* seqlens;  // device [B]; null: every sequence has seqlen_const
   int64_t q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh, table_sb;
-  int B, S, Hkv, G, P, cap, ps_log2, nsplit, causal, seqlen_const;
+  int B, S, Hkv, G, P, cap, ps_log2, causal, seqlen_const;
   int s_new;               // rows appended by this call: S, or 0 without new k, v
   int nrb;                 // row blocks
+  int nwg;                 // workgroups that the units share; 0: one for each unit
   float scale_log2;
 };
 
@@ -84,12 +89,144 @@ __device__ __forceinline__ float rows_sum(float x) {
   return halves_sum(x);
 }
 
+// ---- which workgroup takes what --------------------------------------------------------------------
+// Workgroup = tiles [first, first + count) of TS keys, piece `piece` of the `pieces` of unit (b, h, rb). With
+// P.nwg the units of a sequence of t tiles are cut into n(t) = ceil(t / c) pieces each, c the smallest length, of
+// those that a few bisections try, at which all pieces together are at most P.nwg: the pieces are then of nearly
+// the same length, whatever the sequences' are, and all in flight at once. Each wave finds c by itself, lane i
+// holding sequences i, i + 64, ...
+template <int RB, int TS>
+struct Sched {
+  int b, h, rb, len, first, count, piece, pieces, wg;
+
+  __device__ __forceinline__ static int tiles(const Params& P, int len, int rb) {
+    const int n = keys_seen(P, len, (min(P.S * P.G, (rb + 1) * RB) - 1) / P.G);   // the last row sees the most
+    return max(1, (max(n, 0) + TS - 1) / TS);
+  }
+  __device__ __forceinline__ bool begin(const Params& P) {
+    const int lane = threadIdx.x & 63;
+    piece = first = 0;
+    pieces = 1;
+    if (P.nwg == 0) {
+      // row blocks of one (b, h) eight indices apart, on one XCD
+      rb = (int)((blockIdx.x >> 3) % P.nrb);
+      const int u = (int)((blockIdx.x >> 3) / P.nrb) * 8 + (blockIdx.x & 7);
+      if (u >= P.B * P.Hkv) return false;
+      wg = 0;
+      h = u % P.Hkv;
+      b = u / P.Hkv;
+      len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
+      count = tiles(P, len, rb);
+      return true;
+    }
+    constexpr int NB = kMaxShared / 64;
+    int lens[NB], t[NB], sum = 0;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const int i = lane + 64 * k;
+      lens[k] = i < P.B ? cache_len(P, i) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      t[k] = lane + 64 * k < P.B ? tiles(P, lens[k], P.nrb - 1) : 0;
+      sum += t[k];
+    }
+    const int units = P.Hkv * P.nrb, most = P.nwg / units;      // pieces of all sequences' units of one head and block
+    const float total = (float)__builtin_amdgcn_readlane(wave_scan(sum), 63);
+    auto cut = [&](float inv, int (&n)[NB]) {                   // the pieces of each sequence; their sum
+      int s = 0;
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        n[k] = (int)__builtin_ceilf((float)t[k] * inv);         // 0 for no sequence
+        s += n[k];
+      }
+      return __builtin_amdgcn_readlane(wave_scan(s), 63);
+    };
+    // a sequence has at most t / c + 1 pieces: a length that is long enough, and one that none below could be
+    int n[NB], lower[NB];
+    float c1 = fmaxf(1.f, 1.001f * total / (float)max(1, most - P.B)), c0 = fmaxf(1.f, total / (float)most);
+    if (most <= P.B || cut(1.f / c1, n) > most) {
+      // rounding, or hardly more workgroups than units: one piece each
+#pragma unroll
+      for (int k = 0; k < NB; ++k) n[k] = t[k] ? 1 : 0;
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < 5; ++i) {
+        const float c = i ? 0.5f * (c0 + c1) : c0;
+        if (cut(1.f / c, lower) > most) {
+          c0 = c;
+        } else {
+          c1 = c;
+#pragma unroll
+          for (int k = 0; k < NB; ++k) n[k] = lower[k];
+          if (i == 0) break;
+        }
+      }
+    }
+    // the workgroups before each sequence
+    wg = (int)blockIdx.x;
+    int base = 0;
+    b = -1;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      if (64 * k >= P.B) break;
+      const int upto = base + units * wave_scan(n[k]);
+      if (wg == 0 && threadIdx.x < 64 && lane + 64 * k < P.B) P.pre[lane + 64 * k + 1] = upto;
+      const int end = __builtin_amdgcn_readlane(upto, 63);
+      if (b < 0 && wg < end) {
+        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= wg));
+        b = 64 * k + at;
+        len = __builtin_amdgcn_readlane(lens[k], at);
+        pieces = __builtin_amdgcn_readlane(n[k], at);
+        piece = wg - (__builtin_amdgcn_readlane(upto, at) - units * pieces);
+      }
+      base = end;
+    }
+    if (wg == 0 && threadIdx.x == 0) P.pre[0] = 0;
+    if (b < 0) return false;
+    const int u = piece / pieces;
+    piece -= u * pieces;
+    h = u / P.nrb;
+    rb = u - h * P.nrb;
+    // the pieces that there are no tiles for are empty
+    const int all = tiles(P, len, rb), per = (all + pieces - 1) / pieces;
+    first = min(all, piece * per);
+    count = min(all - first, per);
+    return true;
+  }
+  // The compiler does not see that all of it is the same for a whole wave
+  __device__ __forceinline__ void settle() {
+    for (int* x : {&b, &h, &rb, &len, &first, &count, &piece, &pieces, &wg}) *x = __builtin_amdgcn_readfirstlane(*x);
+  }
+  // where row r0 of the piece's result goes, if it is not the unit's
+  template <int D>
+  __device__ __forceinline__ float* partial(const Params& P) const {
+    return pieces == 1 ? nullptr : P.part + (int64_t)wg * RB * kPart<D>;
+  }
+};
+
+// 16 bytes a lane of 16 rows of a page, off a uniform base; ONCE: kept out of the caches
+template <int D>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rows(const bf16* p) { return make_rsrc(p, 16 * D * 2); }
+template <bool ONCE>
+__device__ __forceinline__ u32x4 page_chunk(__amdgpu_buffer_rsrc_t rows, uint32_t off) {
+  return __builtin_amdgcn_raw_buffer_load_b128(rows, (int)off, 0, ONCE ? 2 : 0);
+}
+// 16 bytes of a row of a sequence: `cached`, or `at` elements into the new rows `fresh`; 0 if it is not there, where
+// q is read instead.
+__device__ __forceinline__ u32x4 row_chunk(const Params& P, bool there, bool old, const char* cached, const bf16* fresh, int64_t at) {
+  const char* p = old ? cached : reinterpret_cast<const char*>(fresh + at);
+  const u32x4 x = *reinterpret_cast<const u32x4*>(there ? p : reinterpret_cast<const char*>(P.q));
+  const uint32_t keep = there ? ~0u : 0u;
+  return u32x4{x[0] & keep, x[1] & keep, x[2] & keep, x[3] & keep};
+}
+
 // This workgroup's share of the new rows of (b, h), part `part` of `parts`, into their pages
-template <int D, int NTH = NT>
+template <int D>
 __device__ __forceinline__ void append_share(const Params& P, int b, int h, int len, int part, int parts) {
   constexpr int CH = D / 8;   // 16-byte chunks of a row
   const int c = 8 * (threadIdx.x % CH), is_v = (threadIdx.x / CH) & 1;
-  for (int i = part + parts * (threadIdx.x / (2 * CH)); i < P.s_new; i += parts * (NTH / (2 * CH))) {
+  for (int i = part + parts * (threadIdx.x / (2 * CH)); i < P.s_new; i += parts * (NT / (2 * CH))) {
     const int j = len + i;
     if (j >= P.cap) break;
     const int page = P.table[b * P.table_sb + (j >> P.ps_log2)];
@@ -102,15 +239,14 @@ __device__ __forceinline__ void append_share(const Params& P, int b, int h, int 
   }
 }
 
-// Rows [r0, r1) over keys [k0, k1) without the matrix cores: 16 lanes a row, key by key. For splits
+// Rows [r0, r1) over keys [k0, k1) without the matrix cores: 16 lanes a row, key by key. For pieces
 // whose values hold an infinity or NaN (0 * inf in P V would reach rows that must not see the key), and
 // for scores that pass fp32's range before the softmax scale, or whose largest is about -3e38: here the
 // scale comes first.
 template <int D>
-__device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int split, int r0, int r1, int k0, int k1, int len) {
+__device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int r0, int r1, int k0, int k1, int len, float* part) {
   constexpr int E = D / 16;
   const int g16 = threadIdx.x & 15;
-  const int R = P.S * P.G;
   auto get = [&](const bf16* p, float* f) {
 #pragma unroll
     for (int e = 0; e < E; ++e) f[e] = (float)p[E * g16 + e];
@@ -150,13 +286,13 @@ __device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int spl
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + p * x[e];
     }
-    if (P.nsplit == 1) {
+    if (!part) {
       const float inv = row_inv(seen != 0.f, l);
       bf16* dst = P.out + b * P.o_sb + i * P.o_ss + hq * P.o_sh + E * g16;
 #pragma unroll
       for (int e = 0; e < E; ++e) dst[e] = (bf16)(o[e] * inv);
     } else {
-      float* dst = P.part + ((((int64_t)b * P.Hkv + h) * R + r) * P.nsplit + split) * kPart<D>;
+      float* dst = part + (r - r0) * kPart<D>;
       if (g16 == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{m, l, seen, 0.f};
 #pragma unroll
       for (int e = 0; e < E; ++e) dst[4 + E * g16 + e] = o[e];
@@ -164,7 +300,7 @@ __device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int spl
   }
 }
 
-// ---- few rows ---------------------------------------------------------------------------------
+// ---- one row ----------------------------------------------------------------------------------
 // Sum over the D / 8 lanes that hold a key row
 template <int D>
 __device__ __forceinline__ float lanes_sum(float x) {
@@ -175,32 +311,30 @@ __device__ __forceinline__ float lanes_sum(float x) {
   return x;
 }
 
-// NR rows (R of them real) of one (b, h, split): blockIdx.x = (b Hkv + h) nsplit + split. Each wave walks 16
-// NH keys at a time by itself; D / 8 lanes hold a key row, 16 bytes each, and take its products with all
-// rows.
-template <int D, int NR, int NTH>
-__global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
-  constexpr int NWAVE = NTH / 64, CH = D / 8, RPL = 64 / CH, NH = D == 128 ? 1 : 2, U = 16 / RPL;
-  constexpr int kStep = 16 * NH * NWAVE;     // keys of a workgroup's step
-  __shared__ float s_m[NWAVE][NR], s_l[NWAVE][NR], s_seen[NWAVE][NR];
-  __shared__ f32x4 s_o[NWAVE][NR][D / 4];
-  const int split = blockIdx.x % P.nsplit, bh = blockIdx.x / P.nsplit;
-  const int h = bh % P.Hkv, b = bh / P.Hkv;
+// R = 1. Each wave walks 16 NH keys at a time by itself; D / 8 lanes hold a key row, 16 bytes each. Bound by memory
+// where there is much to read (64 x 16 heads on 2150-3993 rows, 1.6 GB: 257 us, 6.2 TB/s; 3 x 12 on 16000-29000 65 us,
+// 5.6), by the chain of length, page, keys, joining where there is little (16 heads on 900 rows 9.8 us with the
+// combine). The matrix cores (stream) are as fast on the former and 0.6 to 1.2 us slower on the latter.
+template <int D>
+__global__ __launch_bounds__(NT) void decode_kernel(Params P) {
+  constexpr int CH = D / 8, RPL = 64 / CH, NH = D == 128 ? 1 : 2, U = 16 / RPL;
+  constexpr int kStep = 16 * NH * NWAVE;     // keys of a workgroup's step, a tile
+  __shared__ float s_m[NWAVE], s_l[NWAVE], s_seen[NWAVE];
+  __shared__ f32x4 s_o[NWAVE][D / 4];
+  Sched<1, kStep> sc;
+  if (!sc.begin(P)) return;
+  sc.settle();
+  const int b = sc.b, h = sc.h, len = sc.len;
   const int tid = threadIdx.x, lane = tid & 63, c8 = 8 * (lane % CH), grp = lane / CH;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int R = P.S * P.G;
-  const int len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
   const int lk = min(P.cap, len + P.s_new);
-  const int per = ((lk + P.nsplit - 1) / P.nsplit + kStep - 1) / kStep * kStep;
-  const int k0 = split * per;
-  const int k1 = min(k0 + per, keys_seen(P, len, P.S - 1));     // the last row sees the most
-  const int kall = min(min(k1, len), keys_seen(P, len, 0));     // cached keys below are seen by every row
+  const int k0 = sc.first * kStep;
+  const int k1 = min(k0 + sc.count * kStep, lk);
+  const int kold = min(k1, len);               // keys below are cached
 
   uniform_i32* const tab = uniform(P.table + b * P.table_sb);
   const int psm = (1 << P.ps_log2) - 1;
-  const bf16* const kn = P.s_new ? P.k + b * P.k_sb + h * P.k_sh + c8 : nullptr;
-  const bf16* const vn = P.s_new ? P.v + b * P.v_sb + h * P.v_sh + c8 : nullptr;
-  const u32x4 zero = {0u, 0u, 0u, 0u};
+  const bf16 *const kn = P.k + b * P.k_sb + h * P.k_sh, *const vn = P.v + b * P.v_sb + h * P.v_sh;
   u32x4 kw[NH][U], vw[NH][U];
   int page[NH];                 // of the 16 keys to load next
   bool ok[NH];                  // the cached ones among the 16 keys have a page
@@ -215,23 +349,22 @@ __global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
       const int j = j0 + 16 * hf;
       ok[hf] = (unsigned)page[hf] < (unsigned)P.P;
       const int64_t at = ((((int64_t)(ok[hf] ? page[hf] : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
-      const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
       if (ok[hf] && j + 16 <= len) {
+        const __amdgpu_buffer_rsrc_t kr = page_rows<D>(P.kp + at), vr = page_rows<D>(P.vp + at);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          kw[hf][u] = kvc::load_once(reinterpret_cast<const bf16*>(kb + off + u * (RPL * D * 2)));
-          vw[hf][u] = kvc::load_once(reinterpret_cast<const bf16*>(vb + off + u * (RPL * D * 2)));
+          kw[hf][u] = page_chunk<true>(kr, off + u * (RPL * D * 2));
+          vw[hf][u] = page_chunk<true>(vr, off + u * (RPL * D * 2));
         }
       } else {
-        // the last cached rows, the new ones, none: row by row
+        // the last cached rows, the new one, none: row by row
+        const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int jr = j + u * RPL + grp;
-          kw[hf][u] = vw[hf][u] = zero;
-          if (jr < len ? ok[hf] : jr < lk) {
-            kw[hf][u] = *reinterpret_cast<const u32x4*>(jr < len ? kb + off + u * (RPL * D * 2) : reinterpret_cast<const char*>(kn + (jr - len) * P.k_ss));
-            vw[hf][u] = *reinterpret_cast<const u32x4*>(jr < len ? vb + off + u * (RPL * D * 2) : reinterpret_cast<const char*>(vn + (jr - len) * P.v_ss));
-          }
+          const bool old = jr < len, there = old ? ok[hf] : jr < lk;
+          kw[hf][u] = row_chunk(P, there, old, kb + off + u * (RPL * D * 2), kn, (jr - len) * P.k_ss + c8);
+          vw[hf][u] = row_chunk(P, there, old, vb + off + u * (RPL * D * 2), vn, (jr - len) * P.v_ss + c8);
         }
       }
     }
@@ -242,88 +375,62 @@ __global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
     load(j0);
     look(j0 + kStep);
   }
-  float q[NR][8], o[NR][8], m[NR], l[NR], seen[NR];
-  int nlim[NR];
+  float q[8], o[8], m = -INFINITY, l = 0.f, seen = 0.f;
+  {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(P.q + b * P.q_sb + h * P.q_sh + c8);
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    const int rr = min(r, R - 1);
-    const u32x4 x = *reinterpret_cast<const u32x4*>(P.q + b * P.q_sb + (rr / P.G) * P.q_ss + (h * P.G + rr % P.G) * P.q_sh + c8);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) q[r][2 * e] = bf16lo(x[e]) * P.scale_log2, q[r][2 * e + 1] = bf16hi(x[e]) * P.scale_log2;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[r][e] = 0.f;
-    m[r] = -INFINITY, l[r] = 0.f, seen[r] = 0.f;
-    nlim[r] = min(k1, keys_seen(P, len, rr / P.G));
+    for (int e = 0; e < 4; ++e) q[2 * e] = bf16lo(x[e]) * P.scale_log2, q[2 * e + 1] = bf16hi(x[e]) * P.scale_log2;
   }
-  for (; j0 < k1; j0 += kStep) {
-    float s[NR][NH][U];
 #pragma unroll
-    for (int hf = 0; hf < NH; ++hf)
+  for (int e = 0; e < 8; ++e) o[e] = 0.f;
+  for (; j0 < k1; j0 += kStep) {
+    float s[NH][U];
+    bool full = j0 + 16 * NH <= kold;
+#pragma unroll
+    for (int hf = 0; hf < NH; ++hf) {
+      full = full && ok[hf];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float x[8];
+        float d = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[2 * e] = bf16lo(kw[hf][u][e]), x[2 * e + 1] = bf16hi(kw[hf][u][e]);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          float d = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d += q[r][e] * x[e];
-          s[r][hf][u] = lanes_sum<D>(d);
-        }
+        for (int e = 0; e < 4; ++e) d += q[2 * e] * bf16lo(kw[hf][u][e]) + q[2 * e + 1] * bf16hi(kw[hf][u][e]);
+        s[hf][u] = lanes_sum<D>(d);
       }
-    bool full = j0 + 16 * NH <= kall;
-#pragma unroll
-    for (int hf = 0; hf < NH; ++hf) full = full && ok[hf];
-    uint32_t hides = 0;          // bit (r, hf, u): the row does not see this lane's key
-    if (!full) {
-#pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int hf = 0; hf < NH; ++hf)
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int j = j0 + 16 * hf + u * RPL + grp;
-            const bool sees = j < nlim[r] && (ok[hf] || j >= len);
-            seen[r] = sees ? 1.f : seen[r];
-            s[r][hf][u] = sees ? s[r][hf][u] : -INFINITY;
-            hides |= (sees ? 0u : 1u) << ((r * NH + hf) * U + u);
-          }
     }
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      if (full) seen[r] = 1.f;
-      float mx = m[r];
-#pragma unroll
-      for (int hf = 0; hf < NH; ++hf)
-#pragma unroll
-        for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[r][hf][u]);
-      const float ref = max_ref(mx), alpha = __builtin_amdgcn_exp2f(m[r] - ref);   // m = -inf at first: 0
-      m[r] = mx;
-      l[r] *= alpha;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[r][e] *= alpha;
+    if (full) {
+      seen = 1.f;
+    } else {
+      // what is not there weighs nothing; its values were read as 0
 #pragma unroll
       for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          s[r][hf][u] = __builtin_amdgcn_exp2f(s[r][hf][u] - ref);
-          l[r] += s[r][hf][u];
+          const int j = j0 + 16 * hf + u * RPL + grp;
+          const bool sees = j < k1 && (ok[hf] || j >= len);
+          seen = sees ? 1.f : seen;
+          s[hf][u] = sees ? s[hf][u] : -INFINITY;
         }
     }
+    float mx = m;
+#pragma unroll
+    for (int hf = 0; hf < NH; ++hf)
+#pragma unroll
+      for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[hf][u]);
+    const float ref = max_ref(mx), alpha = __builtin_amdgcn_exp2f(m - ref);   // m = -inf at first: 0
+    m = mx;
+    l *= alpha;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= alpha;
 #pragma unroll
     for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float x[8];
+        const float p = __builtin_amdgcn_exp2f(s[hf][u] - ref);
+        l += p;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[2 * e] = bf16lo(vw[hf][u][e]), x[2 * e + 1] = bf16hi(vw[hf][u][e]);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          // a value that the row does not see may be infinite
-          if (!full && (hides >> ((r * NH + hf) * U + u) & 1)) continue;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[r][e] += s[r][hf][u] * x[e];
+        for (int e = 0; e < 4; ++e) {
+          o[2 * e] += p * bf16lo(vw[hf][u][e]);
+          o[2 * e + 1] += p * bf16hi(vw[hf][u][e]);
         }
       }
     if (j0 + kStep < k1) {
@@ -332,60 +439,54 @@ __global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
     }
   }
   // the wave's groups, then the waves
+  float M = m;
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    float M = m[r];
+  for (int x = CH; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
+  const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+  l *= a;
 #pragma unroll
-    for (int x = CH; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
-    const float a = m[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[r] - M);
-    l[r] *= a;
+  for (int x = CH; x < 64; x <<= 1) {
+    l += __shfl_xor(l, x);
+    seen = fmaxf(seen, __shfl_xor(seen, x));
+  }
 #pragma unroll
-    for (int x = CH; x < 64; x <<= 1) {
-      l[r] += __shfl_xor(l[r], x);
-      seen[r] = fmaxf(seen[r], __shfl_xor(seen[r], x));
-    }
+  for (int e = 0; e < 8; ++e) {
+    o[e] *= a;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      o[r][e] *= a;
-#pragma unroll
-      for (int x = CH; x < 64; x <<= 1) o[r][e] += __shfl_xor(o[r][e], x);
-    }
-    if (lane < CH) {
-      if (lane == 0) s_m[w][r] = M, s_l[w][r] = l[r], s_seen[w][r] = seen[r];
-      s_o[w][r][2 * lane] = f32x4{o[r][0], o[r][1], o[r][2], o[r][3]};
-      s_o[w][r][2 * lane + 1] = f32x4{o[r][4], o[r][5], o[r][6], o[r][7]};
-    }
+    for (int x = CH; x < 64; x <<= 1) o[e] += __shfl_xor(o[e], x);
+  }
+  if (lane < CH) {
+    if (lane == 0) s_m[w] = M, s_l[w] = l, s_seen[w] = seen;
+    s_o[w][2 * lane] = f32x4{o[0], o[1], o[2], o[3]};
+    s_o[w][2 * lane + 1] = f32x4{o[4], o[5], o[6], o[7]};
   }
   __syncthreads();
-  if (tid < NR * (D / 4)) {
-    const int r = tid / (D / 4), c = tid % (D / 4);
-    if (r < R) {
-      float M = s_m[0][r], L = 0.f, any = 0.f;
+  if (tid < D / 4) {
+    float L = 0.f, any = 0.f;
+    M = s_m[0];
 #pragma unroll
-      for (int g = 1; g < NWAVE; ++g) M = fmaxf(M, s_m[g][r]);
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int g = 1; g < NWAVE; ++g) M = fmaxf(M, s_m[g]);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int g = 0; g < NWAVE; ++g) {
-        const float wgt = s_m[g][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[g][r] - M);
-        L += wgt * s_l[g][r];
-        any = fmaxf(any, s_seen[g][r]);
-        acc += wgt * s_o[g][r][c];
-      }
-      if (P.nsplit == 1) {
-        const float inv = row_inv(any != 0.f, L);
-        *reinterpret_cast<bf16x4*>(P.out + b * P.o_sb + (r / P.G) * P.o_ss + (h * P.G + r % P.G) * P.o_sh + 4 * c) =
-            cvt4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-      } else {
-        float* dst = P.part + (((int64_t)bh * R + r) * P.nsplit + split) * kPart<D>;
-        if (c == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{M, L, any, 0.f};
-        *reinterpret_cast<f32x4*>(dst + 4 + 4 * c) = acc;
-      }
+    for (int g = 0; g < NWAVE; ++g) {
+      const float wgt = s_m[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[g] - M);
+      L += wgt * s_l[g];
+      any = fmaxf(any, s_seen[g]);
+      acc += wgt * s_o[g][tid];
+    }
+    if (float* part = sc.template partial<D>(P)) {
+      if (tid == 0) *reinterpret_cast<f32x4*>(part) = f32x4{M, L, any, 0.f};
+      *reinterpret_cast<f32x4*>(part + 4 + 4 * tid) = acc;
+    } else {
+      const float inv = row_inv(any != 0.f, L);
+      *reinterpret_cast<bf16x4*>(P.out + b * P.o_sb + h * P.o_sh + 4 * tid) =
+          cvt4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     }
   }
-  append_share<D, NTH>(P, b, h, len, split, P.nsplit);
+  append_share<D>(P, b, h, len, sc.piece, sc.pieces);
 }
 
-// ---- more of them -------------------------------------------------------------------------------
+// ---- up to 16 rows -------------------------------------------------------------------------------
 template <int D>
 struct Geo {
   static constexpr int NS = D / 32;              // steps of the contraction over d
@@ -402,40 +503,37 @@ struct Geo {
   static_assert(AREA >= 16 * OS * 4, "16 rows of o fit");
 };
 
-// blockIdx.x: row blocks of one (b, h, split) eight indices apart, on one XCD.
-template <int D, int RT>
-__global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
+// R <= 16. Each wave walks 32 keys at a time by itself: S^T = K Q^T by 16 keys, then O^T += V^T P^T, K and V through LDS
+// of its own, so that both are read from memory in whole rows (K straight into the matrix cores, 64 bytes of 16 rows a
+// load, took 105 us where this takes 92). Bound by memory: 48 x 2 key-value heads of eight query heads on 6900-12700
+// rows, 479 MB, 85 us with the combine, 5.6 TB/s. Two workgroups a CU (72 KB of LDS, 212 registers).
+template <int D>
+__global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
   using G = Geo<D>;
-  constexpr int NS = G::NS, ND = G::ND, CH = G::CH, HL = ND / 2;   // HL: V loads of 16 keys
+  constexpr int NS = G::NS, ND = G::ND, CH = G::CH, HL = ND / 2;   // HL: loads of 16 rows
   __shared__ __attribute__((aligned(16))) char smem[NWAVE][G::AREA];
   __shared__ float s_m[NWAVE][16], s_l[NWAVE][16], s_seen[NWAVE][16];
   __shared__ int s_bad;
-  const int rb = (blockIdx.x >> 3) % P.nrb;
-  const int unit = (int)((blockIdx.x >> 3) / P.nrb) * 8 + (blockIdx.x & 7);
-  if (unit >= P.B * P.Hkv * P.nsplit) return;
-  const int split = unit % P.nsplit, bh = unit / P.nsplit;
-  const int h = bh % P.Hkv, b = bh / P.Hkv;
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int R = P.S * P.G, r0 = rb * 16 * RT, r1 = min(R, r0 + 16 * RT);
-  const int len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
+  constexpr int kStep = kKeys * NWAVE;       // keys of a workgroup's step, a tile
+  Sched<16, kStep> sc;
+  if (!sc.begin(P)) return;
+  sc.settle();
+  const int b = sc.b, h = sc.h, len = sc.len, R = P.S * P.G;
   const int lk = min(P.cap, len + P.s_new);
-  // the splits share a sequence's own keys, in whole steps
-  const int per = ((lk + P.nsplit - 1) / P.nsplit + kKeys - 1) / kKeys * kKeys;
-  const int k0 = split * per;
-  const int k1 = min(k0 + per, keys_seen(P, len, (r1 - 1) / P.G));   // the last row sees the most
-  const int kall = keys_seen(P, len, r0 / P.G);                      // every row sees the keys below
+  const int k0 = sc.first * kStep;
+  const int k1 = min(k0 + sc.count * kStep, keys_seen(P, len, P.S - 1));   // the last row sees the most
+  const int kall = keys_seen(P, len, 0);                             // every row sees the keys below
   if (tid == 0) s_bad = 0;
 
   uniform_i32* const tab = uniform(P.table + b * P.table_sb);
   const int psm = (1 << P.ps_log2) - 1;
-  const bf16* const kn = P.s_new ? P.k + b * P.k_sb + h * P.k_sh + 8 * (lane % CH) : nullptr;
-  const bf16* const vn = P.s_new ? P.v + b * P.v_sb + h * P.v_sh + 8 * (lane % CH) : nullptr;
+  const bf16 *const kn = P.k + b * P.k_sb + h * P.k_sh, *const vn = P.v + b * P.v_sb + h * P.v_sh;
   char* const area = smem[w];
 
   u32x4 kw[ND], vw[ND];
   bool ok[2];              // the 16 keys have a page, or are new rows
-  const u32x4 zero = {0u, 0u, 0u, 0u};
   const uint32_t off = (uint32_t)(lane / CH * D + 8 * (lane % CH)) * 2;
   auto load = [&](int j0) {
 #pragma unroll
@@ -444,130 +542,112 @@ __global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
       const int page = j < len ? tab[j >> P.ps_log2] : -1;
       const bool held = (unsigned)page < (unsigned)P.P;
       const int64_t at = ((((int64_t)(held ? page : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
-      const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
       ok[hf] = held;
       if (held && j + 16 <= len) {
+        const __amdgpu_buffer_rsrc_t kr = page_rows<D>(P.kp + at), vr = page_rows<D>(P.vp + at);
 #pragma unroll
         for (int u = 0; u < HL; ++u) {
-          kw[hf * HL + u] = kvc::load_once(reinterpret_cast<const bf16*>(kb + off + u * (G::RPL * D * 2)));
-          vw[hf * HL + u] = kvc::load_once(reinterpret_cast<const bf16*>(vb + off + u * (G::RPL * D * 2)));
+          kw[hf * HL + u] = page_chunk<true>(kr, off + u * (G::RPL * D * 2));
+          vw[hf * HL + u] = page_chunk<true>(vr, off + u * (G::RPL * D * 2));
         }
       } else {
         // the last cached rows, the new ones, none: row by row
+        const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
 #pragma unroll
         for (int u = 0; u < HL; ++u) {
           const int jr = j + u * G::RPL + lane / CH;
-          kw[hf * HL + u] = vw[hf * HL + u] = zero;
-          if (jr < len ? held : jr < lk) {
-            kw[hf * HL + u] = *reinterpret_cast<const u32x4*>(
-                jr < len ? kb + off + u * (G::RPL * D * 2) : reinterpret_cast<const char*>(kn + (jr - len) * P.k_ss));
-            vw[hf * HL + u] = *reinterpret_cast<const u32x4*>(
-                jr < len ? vb + off + u * (G::RPL * D * 2) : reinterpret_cast<const char*>(vn + (jr - len) * P.v_ss));
-          }
+          const bool old = jr < len, there = old ? held : jr < lk;
+          kw[hf * HL + u] = row_chunk(P, there, old, kb + off + u * (G::RPL * D * 2), kn, (jr - len) * P.k_ss + 8 * (lane % CH));
+          vw[hf * HL + u] = row_chunk(P, there, old, vb + off + u * (G::RPL * D * 2), vn, (jr - len) * P.v_ss + 8 * (lane % CH));
         }
       }
     }
   };
 
-  float m_run[RT], l_run[RT], seen[RT];
-  f32x4 oacc[RT][ND];
-  int nlim[RT];            // this lane's row sees keys below, of this split
+  float m_run = -INFINITY, l_run = 0.f, seen = 0.f;
+  f32x4 oacc[ND];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    m_run[t] = -INFINITY, l_run[t] = 0.f, seen[t] = 0.f;
-    nlim[t] = min(k1, keys_seen(P, len, min(r0 + 16 * t + l16, R - 1) / P.G));
-#pragma unroll
-    for (int d = 0; d < ND; ++d) oacc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < ND; ++d) oacc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int row = min(l16, R - 1), ri = row / P.G;         // this lane's row (past the last: that one, not stored)
+  const int nlim = min(k1, keys_seen(P, len, ri));
   u16x2 vmag = {0, 0};
 
   int j0 = k0 + kKeys * w;
   if (j0 < k1) {
     load(j0);
-    // Q^T: lane holds row l16, columns 32 s + 8 g4 + 0..7 (rows past the last: that one, not stored)
-    bf16x8 qf[RT][NS];
+    // Q^T: lane holds its row, columns 32 s + 8 g4 + 0..7
+    bf16x8 qf[NS];
+    const bf16* qp = P.q + b * P.q_sb + ri * P.q_ss + (h * P.G + row - ri * P.G) * P.q_sh + 8 * g4;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int r = min(r0 + 16 * t + l16, R - 1);
-      const bf16* qp = P.q + b * P.q_sb + (r / P.G) * P.q_ss + (h * P.G + r % P.G) * P.q_sh + 8 * g4;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) qf[t][s] = *reinterpret_cast<const bf16x8*>(qp + 32 * s);
-    }
+    for (int n = 0; n < NS; ++n) qf[n] = *reinterpret_cast<const bf16x8*>(qp + 32 * n);
     char* const karea = area + kKeys * G::VS;
     const char *const vt = area + (4 * g4 + (l16 >> 2)) * G::VS + 8 * (l16 & 3), *const kt = karea + l16 * G::KS + 16 * g4;
-    const int row = lane / CH, c16 = 16 * (lane % CH);
-    for (; j0 < k1; j0 += kKeys * NWAVE) {
+    const int lrow = lane / CH, c16 = 16 * (lane % CH);
+    for (; j0 < k1; j0 += kStep) {
 #pragma unroll
-      for (int u = 0; u < ND; ++u) *reinterpret_cast<u32x4*>(karea + (u * G::RPL + row) * G::KS + c16) = kw[u];
+      for (int u = 0; u < ND; ++u) *reinterpret_cast<u32x4*>(karea + (u * G::RPL + lrow) * G::KS + c16) = kw[u];
 #pragma unroll
       for (int u = 0; u < ND; ++u) {
         vmag = max_mag(vmag, vw[u]);
-        *reinterpret_cast<u32x4*>(area + (u * G::RPL + row) * G::VS + c16) = vw[u];
+        *reinterpret_cast<u32x4*>(area + (u * G::RPL + lrow) * G::VS + c16) = vw[u];
       }
       // a page that is missing hides cached keys only
       const bool ok0 = ok[0], ok1 = ok[1];
-      if (j0 + kKeys * NWAVE < k1) load(j0 + kKeys * NWAVE);
+      if (j0 + kStep < k1) load(j0 + kStep);
       // K: lane holds key l16 of 16, columns 32 n + 8 g4 + 0..7
-      f32x4 s[RT][2];
+      f32x4 s[2];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+      for (int hf = 0; hf < 2; ++hf) {
+        s[hf] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + 16 * hf * G::KS + 64 * n);
-#pragma unroll
-          for (int t = 0; t < RT; ++t) s[t][hf] = mfma16x16x32(kf, qf[t][n], n ? s[t][hf] : f32x4{0.f, 0.f, 0.f, 0.f});
-        }
-      bf16x8 pt[RT][3];
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
+        for (int n = 0; n < NS; ++n)
+          s[hf] = mfma16x16x32(*reinterpret_cast<const bf16x8*>(kt + 16 * hf * G::KS + 64 * n), qf[n], s[hf]);
+        s[hf] *= P.scale_log2;   // before the mask: the scale may have any sign
+      }
+      if (j0 + kKeys > min(kall, k1) || !ok0 || !ok1) {
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[t][hf][r] *= P.scale_log2;   // before the mask: the scale may have any sign
-        if (j0 + kKeys > min(kall, k1) || !ok0 || !ok1) {
+          for (int r = 0; r < 4; ++r) {
+            const int j = j0 + 16 * hf + 4 * g4 + r;
+            const bool sees = j < nlim && ((hf ? ok1 : ok0) || j >= len);
+            seen = sees ? 1.f : seen;
+            s[hf][r] = sees ? s[hf][r] : -INFINITY;
+          }
+      } else {
+        seen = 1.f;
+      }
+      float mx = s[0][0];
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
+      mx = rows_max(mx);
+      if (__builtin_amdgcn_ballot_w64(mx > m_run) != 0) {
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int j = j0 + 16 * hf + 4 * g4 + r;
-              const bool sees = j < nlim[t] && ((hf ? ok1 : ok0) || j >= len);
-              seen[t] = sees ? 1.f : seen[t];
-              s[t][hf][r] = sees ? s[t][hf][r] : -INFINITY;
-            }
-        } else {
-          seen[t] = 1.f;
-        }
-        float mx = s[t][0][0];
+        for (int d = 0; d < ND; ++d) oacc[d] *= alpha;
+      }
+      const float m_use = max_ref(m_run);
+      float e[8];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[t][e >> 2][e & 3]);
-        mx = rows_max(mx);
-        if (__builtin_amdgcn_ballot_w64(mx > m_run[t]) != 0) {
-          const float m_new = fmaxf(m_run[t], mx);
-          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[t] - m_new);
-          m_run[t] = m_new;
-          l_run[t] *= alpha;
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - m_use);
+        l_run += e[i];
+      }
+      // the probabilities go into P V as three bf16 terms, which add up to their fp32 bits
+      bf16x8 pt[3];
 #pragma unroll
-          for (int d = 0; d < ND; ++d) oacc[t][d] *= alpha;
-        }
-        const float m_use = max_ref(m_run[t]);
-        float e[8];
+      for (int n = 0; n < 3; ++n) {
+        u32x4 x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(s[t][i >> 2][i & 3] - m_use);
-          l_run[t] += e[i];
-        }
-        // the probabilities go into P V as three bf16 terms, which add up to their fp32 bits
+        for (int i = 0; i < 4; ++i)
+          x[i] = pack_hi(__builtin_bit_cast(uint32_t, e[2 * i]), __builtin_bit_cast(uint32_t, e[2 * i + 1]));
+        pt[n] = __builtin_bit_cast(bf16x8, x);
 #pragma unroll
-        for (int n = 0; n < 3; ++n) {
-          u32x4 x;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x[i] = pack_hi(__builtin_bit_cast(uint32_t, e[2 * i]), __builtin_bit_cast(uint32_t, e[2 * i + 1]));
-          pt[t][n] = __builtin_bit_cast(bf16x8, x);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)   // exact
-            e[i] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, e[i]) & 0xffff0000u);
-        }
+        for (int i = 0; i < 8; ++i)   // exact
+          e[i] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, e[i]) & 0xffff0000u);
       }
       // V^T: lane holds column 16 d + l16 of keys 4 g4 + 0..3 and 16 + 4 g4 + 0..3, as s has them
 #pragma unroll
@@ -575,48 +655,43 @@ __global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
         const u32x2 x0 = lds_read_tr(vt, 32 * d), x1 = lds_read_tr(vt, 16 * G::VS + 32 * d);
         const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{x0[0], x0[1], x1[0], x1[1]});
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-          for (int n = 0; n < 3; ++n) oacc[t][d] = mfma16x16x32(vf, pt[t][n], oacc[t][d]);
+        for (int n = 0; n < 3; ++n) oacc[d] = mfma16x16x32(vf, pt[n], oacc[d]);
       }
     }
   }
 
   __syncthreads();   // s_bad is cleared
-  bool bad = vmag[0] >= 0x7f80 || vmag[1] >= 0x7f80;
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    l_run[t] = rows_sum(l_run[t]);
-    // a score past the range upwards leaves NaN; one past it downwards (raw below -3.4e38) only counts
-    // where every key that the row sees here scores about as low
-    bad |= seen[t] != 0.f && (l_run[t] != l_run[t] || m_run[t] < 200.f - 3e38f * fabsf(P.scale_log2));
-    seen[t] = rows_max(seen[t]);
-  }
-  if (bad) s_bad = 1;
-  // the waves' results meet, 16 rows at a time
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    if (t) __syncthreads();
+  l_run = rows_sum(l_run);
+  // a score past the range upwards leaves NaN; one past it downwards (raw below -3.4e38) only counts
+  // where every key that the row sees here scores about as low
+  if (vmag[0] >= 0x7f80 || vmag[1] >= 0x7f80 ||
+      (seen != 0.f && (l_run != l_run || m_run < 200.f - 3e38f * fabsf(P.scale_log2))))
+    s_bad = 1;
+  seen = rows_max(seen);
+  // the waves' results meet
+  float* const part = sc.template partial<D>(P);
+  {
     float* o = reinterpret_cast<float*>(area) + l16 * G::OS + 4 * g4;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(o + 16 * d) = oacc[t][d];
-    if (g4 == 0) s_m[w][l16] = m_run[t], s_l[w][l16] = l_run[t], s_seen[w][l16] = seen[t];
-    __syncthreads();
-    if (s_bad) break;
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(o + 16 * d) = oacc[d];
+    if (g4 == 0) s_m[w][l16] = m_run, s_l[w][l16] = l_run, s_seen[w][l16] = seen;
+  }
+  __syncthreads();
+  if (s_bad) {
+    walk_rows<D>(P, b, h, 0, R, k0, k1, len, part);
+  } else if (const int r = tid >> 4; r < R) {
     constexpr int E = D / 16;
-    const int row = tid >> 4, r = r0 + 16 * t + row;
-    if (r >= r1) continue;
-    float M = s_m[0][row], L = 0.f, any = 0.f, x[E];
+    float M = s_m[0][r], L = 0.f, any = 0.f, x[E];
 #pragma unroll
-    for (int g = 1; g < NWAVE; ++g) M = fmaxf(M, s_m[g][row]);
+    for (int g = 1; g < NWAVE; ++g) M = fmaxf(M, s_m[g][r]);
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = 0.f;
 #pragma unroll
     for (int g = 0; g < NWAVE; ++g) {
-      const float wgt = s_m[g][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[g][row] - M);
-      L += wgt * s_l[g][row];
-      any = fmaxf(any, s_seen[g][row]);
-      const float* src = reinterpret_cast<const float*>(smem[g]) + row * G::OS + E * l16;
+      const float wgt = s_m[g][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[g][r] - M);
+      L += wgt * s_l[g][r];
+      any = fmaxf(any, s_seen[g][r]);
+      const float* src = reinterpret_cast<const float*>(smem[g]) + r * G::OS + E * l16;
 #pragma unroll
       for (int e = 0; e < E; e += 4) {
         const f32x4 y = *reinterpret_cast<const f32x4*>(src + e);
@@ -624,21 +699,20 @@ __global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
         for (int c = 0; c < 4; ++c) x[e + c] += wgt * y[c];
       }
     }
-    if (P.nsplit == 1) {
+    if (!part) {
       const float inv = row_inv(any != 0.f, L);
       bf16* dst = P.out + b * P.o_sb + (r / P.G) * P.o_ss + (h * P.G + r % P.G) * P.o_sh + E * l16;
 #pragma unroll
       for (int e = 0; e < E; e += 4)
         *reinterpret_cast<bf16x4*>(dst + e) = cvt4(x[e] * inv, x[e + 1] * inv, x[e + 2] * inv, x[e + 3] * inv);
     } else {
-      float* dst = P.part + ((((int64_t)b * P.Hkv + h) * R + r) * P.nsplit + split) * kPart<D>;
+      float* dst = part + r * kPart<D>;
       if (l16 == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{M, L, any, 0.f};
 #pragma unroll
       for (int e = 0; e < E; e += 4) *reinterpret_cast<f32x4*>(dst + 4 + E * l16 + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
     }
   }
-  if (s_bad) walk_rows<D>(P, b, h, split, r0, r1, k0, k1, len);
-  append_share<D>(P, b, h, len, rb * P.nsplit + split, P.nrb * P.nsplit);
+  append_share<D>(P, b, h, len, sc.piece, sc.pieces);
 }
 
 // ---- many rows -----------------------------------------------------------------------------------
@@ -647,8 +721,8 @@ __global__ __launch_bounds__(NT, RT == 1 ? 3 : 2) void stream_kernel(Params P) {
 // row as the lane column, V^T from transposing reads.
 template <int D, int QW>
 struct TileGeo {
-  static constexpr int KW = 4 / QW;
-  static constexpr int TK = 32 * KW;                     // keys a tile
+  static constexpr int KW = 4 / QW, NK = QW == 4 ? 2 : 1;  // waves along the keys; times 32 keys a wave has of a tile
+  static constexpr int TK = 32 * KW * NK;                // keys a tile
   static constexpr int CH = D / 8, RPP = NT / CH;        // 16-byte chunks of a row; rows that all threads load at once
   static constexpr int NP = TK / RPP;
   static constexpr int NDT = D / 32;
@@ -664,23 +738,19 @@ struct TileGeo {
 template <int D, int QW>
 __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
   using G = TileGeo<D, QW>;
-  constexpr int KW = G::KW, TK = G::TK, NP = G::NP, NDT = G::NDT, NS = D / 16, CH = G::CH, RSD = G::RSD;
+  constexpr int KW = G::KW, NK = G::NK, TK = G::TK, NP = G::NP, NDT = G::NDT, NS = D / 16, CH = G::CH, RSD = G::RSD;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int s_bad, s_hole;   // a value row or score is not finite; a tile had rows without a page
-  const int rb = (blockIdx.x >> 3) % P.nrb;
-  const int unit = (int)((blockIdx.x >> 3) / P.nrb) * 8 + (blockIdx.x & 7);
-  if (unit >= P.B * P.Hkv * P.nsplit) return;
-  const int split = unit % P.nsplit, bh = unit / P.nsplit;
-  const int h = bh % P.Hkv, b = bh / P.Hkv;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qw = w % QW, kw = w / QW;
-  const int R = P.S * P.G, r0 = rb * 32 * QW, r1 = min(R, r0 + 32 * QW);
-  const int len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
-  const int lk = min(P.cap, len + P.s_new);
-  const int per = ((lk + P.nsplit - 1) / P.nsplit + TK - 1) / TK * TK;
-  const int k0 = split * per;
-  const int k1 = min(k0 + per, keys_seen(P, len, (r1 - 1) / P.G));
+  Sched<32 * QW, TK> sc;
+  if (!sc.begin(P)) return;
+  sc.settle();
+  const int b = sc.b, h = sc.h, len = sc.len;
+  const int R = P.S * P.G, r0 = sc.rb * 32 * QW, r1 = min(R, r0 + 32 * QW);
+  const int k0 = sc.first * TK;
+  const int k1 = min(k0 + sc.count * TK, keys_seen(P, len, (r1 - 1) / P.G));
   const int kall = keys_seen(P, len, r0 / P.G);                  // every row of the block sees the keys below
   const int row = min(r0 + 32 * qw + l32, R - 1);                // this lane's (past the last: that one, not stored)
   const int ri = row / P.G, rh = h * P.G + row % P.G;
@@ -693,11 +763,9 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
   // staging: thread = chunk sch of rows srow + RPP n; V rows in permuted order
   const int srow = tid / CH, sch = tid % CH, vrow = perm_row(srow);
   const int g16 = __builtin_amdgcn_readfirstlane(srow & ~15);    // this wave's 16 keys of a pass
-  const bf16* const kn = P.s_new ? P.k + b * P.k_sb + h * P.k_sh + 8 * sch : nullptr;
-  const bf16* const vn = P.s_new ? P.v + b * P.v_sb + h * P.v_sh + 8 * sch : nullptr;
+  const bf16 *const kn = P.k + b * P.k_sb + h * P.k_sh, *const vn = P.v + b * P.v_sb + h * P.v_sh;
   const uint32_t koff = (uint32_t)((srow & 15) * D + 8 * sch) * 2, voff = (uint32_t)((vrow & 15) * D + 8 * sch) * 2;
   u32x4 ks[NP], vs[NP];
-  const u32x4 zero = {0u, 0u, 0u, 0u};
   int page[NP];                 // of this wave's keys of the tile to load next
   auto look = [&](int t0) {
 #pragma unroll
@@ -712,19 +780,16 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
       const int j = t0 + G::RPP * n + g16;
       const bool held = (unsigned)page[n] < (unsigned)P.P;
       const int64_t at = ((((int64_t)(held ? page[n] : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
-      const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
       if (held && j + 16 <= len) {
-        ks[n] = *reinterpret_cast<const u32x4*>(kb + koff);
-        vs[n] = *reinterpret_cast<const u32x4*>(vb + voff);
+        ks[n] = page_chunk<false>(page_rows<D>(P.kp + at), koff);
+        vs[n] = page_chunk<false>(page_rows<D>(P.vp + at), voff);
       } else {
         // the last cached rows, the new ones, none: row by row
         if (j < min(len, k1) && !held) s_hole = 1;
+        const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
         const int jk = j + (srow & 15), jv = j + (vrow & 15);
-        ks[n] = vs[n] = zero;
-        if (jk < len ? held : jk < k1)
-          ks[n] = *reinterpret_cast<const u32x4*>(jk < len ? kb + koff : reinterpret_cast<const char*>(kn + (jk - len) * P.k_ss));
-        if (jv < len ? held : jv < k1)
-          vs[n] = *reinterpret_cast<const u32x4*>(jv < len ? vb + voff : reinterpret_cast<const char*>(vn + (jv - len) * P.v_ss));
+        ks[n] = row_chunk(P, jk < len ? held : jk < k1, jk < len, kb + koff, kn, (jk - len) * P.k_ss + 8 * sch);
+        vs[n] = row_chunk(P, jv < len ? held : jv < k1, jv < len, vb + voff, vn, (jv - len) * P.v_ss + 8 * sch);
       }
     }
   };
@@ -771,47 +836,54 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
         load(k0 + (t + 1) * TK);
         look(k0 + (t + 2) * TK);
       }
-      const int kk = k0 + t * TK + 32 * kw;   // first key of this wave's 32
+      const int kk = k0 + t * TK + 32 * NK * kw;   // first key of this wave's
       if (kk < kend_w) {
-        const char* kt = smem + buf * G::BUF + (32 * kw + l32) * RSD + hh * 16;
-        const char* vt = smem + buf * G::BUF + G::TILE + 32 * kw * RSD + xt_lane_off<RSD>(lane);
-        f32x16 sacc;
+        const char* kt = smem + buf * G::BUF + (32 * NK * kw + l32) * RSD + hh * 16;
+        const char* vt = smem + buf * G::BUF + G::TILE + 32 * NK * kw * RSD + xt_lane_off<RSD>(lane);
+        f32x16 sacc[NK];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sacc[r] = 0.f;
-        bf16x8 ka[NS];
-        ka[0] = *reinterpret_cast<const bf16x8*>(kt);
-        ka[1] = *reinterpret_cast<const bf16x8*>(kt + 32);
+        for (int x = 0; x < NK; ++x) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {   // operands two steps ahead
-          if (s + 2 < NS) ka[s + 2] = *reinterpret_cast<const bf16x8*>(kt + 32 * (s + 2));
-          sched_fence();
-          sacc = mfma32x32x16(ka[s], qf[s], sacc);
-          sched_fence();
+          for (int r = 0; r < 16; ++r) sacc[x][r] = 0.f;
+          bf16x8 ka[NS];
+          ka[0] = *reinterpret_cast<const bf16x8*>(kt + 32 * x * RSD);
+          ka[1] = *reinterpret_cast<const bf16x8*>(kt + 32 * x * RSD + 32);
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {   // operands two steps ahead
+            if (s + 2 < NS) ka[s + 2] = *reinterpret_cast<const bf16x8*>(kt + 32 * x * RSD + 32 * (s + 2));
+            sched_fence();
+            sacc[x] = mfma32x32x16(ka[s], qf[s], sacc[x]);
+            sched_fence();
+          }
         }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sacc[r] *= c;   // before the mask: the scale may have any sign
         const bool hole = s_hole != 0;
-        if (kk + 32 > min(kall, k1) || hole) {
-          // key kk + 8 (r / 4) + 4 hh + r % 4 is seen iff it is below kq, and cached ones have a page
-          bool ok[2];
+        float mx = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const int j = kk + 16 * g;
-            ok[g] = !hole || j >= len || (unsigned)tab[j >> P.ps_log2] < (unsigned)P.P;
+        for (int x = 0; x < NK; ++x) {
+          const int kx = kk + 32 * x;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sacc[x][r] *= c;   // before the mask: the scale may have any sign
+          if (kx + 32 > min(kall, k1) || hole) {
+            // key kx + 8 (r / 4) + 4 hh + r % 4 is seen iff it is below kq, and cached ones have a page
+            bool ok[2];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const int j = kx + 16 * g;
+              ok[g] = !hole || j >= len || (unsigned)tab[j >> P.ps_log2] < (unsigned)P.P;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int j = kx + 8 * (r >> 2) + 4 * hh + (r & 3);
+              const bool sees = j < kq && (ok[r >> 3] || j >= len);
+              seen = sees ? 1.f : seen;
+              sacc[x][r] = sees ? sacc[x][r] : -INFINITY;
+            }
+          } else {
+            seen = 1.f;
           }
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = kk + 8 * (r >> 2) + 4 * hh + (r & 3);
-            const bool sees = j < kq && (ok[r >> 3] || j >= len);
-            seen = sees ? 1.f : seen;
-            sacc[r] = sees ? sacc[r] : -INFINITY;
-          }
-        } else {
-          seen = 1.f;
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[x][r]);
         }
-        float mx = sacc[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, sacc[r]);
         mx = halves_max(mx);
         if (__builtin_amdgcn_ballot_w64(mx > m_run) != 0) {
           const float m_new = fmaxf(m_run, mx);
@@ -824,37 +896,41 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
             for (int r = 0; r < 16; ++r) oacc[dt][r] *= alpha;
         }
         const float m_use = max_ref(m_run);
-        u32x4 xt[2 * NDT];
-        xt[0] = lds_read_xt<RSD>(vt, 0, 0);
-        xt[1] = lds_read_xt<RSD>(vt, 0, 1);
-        // 16 keys at a time: P's three bf16 terms, which add up to its fp32 bits, times V
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float e[8], ps = 0.f;
-          bf16x8 pt[3];
+        for (int x = 0; x < NK; ++x) {
+          const char* vx = vt + 32 * x * RSD;
+          u32x4 xt[2 * NDT];
+          xt[0] = lds_read_xt<RSD>(vx, 0, 0);
+          xt[1] = lds_read_xt<RSD>(vx, 0, 1);
+          // 16 keys at a time: P's three bf16 terms, which add up to its fp32 bits, times V
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(sacc[8 * half + i] - m_use);
-            ps += e[i];
-          }
-          l_run += ps;
+          for (int half = 0; half < 2; ++half) {
+            float e[8], ps = 0.f;
+            bf16x8 pt[3];
 #pragma unroll
-          for (int n = 0; n < 3; ++n) {
-            u32x4 x;
+            for (int i = 0; i < 8; ++i) {
+              e[i] = __builtin_amdgcn_exp2f(sacc[x][8 * half + i] - m_use);
+              ps += e[i];
+            }
+            l_run += ps;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              x[i] = pack_hi(__builtin_bit_cast(uint32_t, e[2 * i]), __builtin_bit_cast(uint32_t, e[2 * i + 1]));
-            pt[n] = __builtin_bit_cast(bf16x8, x);
+            for (int n = 0; n < 3; ++n) {
+              u32x4 y;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)   // exact
-              e[i] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, e[i]) & 0xffff0000u);
-          }
+              for (int i = 0; i < 4; ++i)
+                y[i] = pack_hi(__builtin_bit_cast(uint32_t, e[2 * i]), __builtin_bit_cast(uint32_t, e[2 * i + 1]));
+              pt[n] = __builtin_bit_cast(bf16x8, y);
 #pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) {
-            const int x = NDT * half + dt;
-            if (x + 2 < 2 * NDT) xt[x + 2] = lds_read_xt<RSD>(vt, (x + 2) / NDT, (x + 2) % NDT);
+              for (int i = 0; i < 8; ++i)   // exact
+                e[i] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, e[i]) & 0xffff0000u);
+            }
 #pragma unroll
-            for (int n = 0; n < 3; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[x]), pt[n], oacc[dt]);
+            for (int dt = 0; dt < NDT; ++dt) {
+              const int z = NDT * half + dt;
+              if (z + 2 < 2 * NDT) xt[z + 2] = lds_read_xt<RSD>(vx, (z + 2) / NDT, (z + 2) % NDT);
+#pragma unroll
+              for (int n = 0; n < 3; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[z]), pt[n], oacc[dt]);
+            }
           }
         }
       }
@@ -918,10 +994,11 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
     }
   }
   __syncthreads();
+  float* const part = sc.template partial<D>(P);
   if (s_bad) {
-    walk_rows<D>(P, b, h, split, r0, r1, k0, k1, len);
+    walk_rows<D>(P, b, h, r0, r1, k0, k1, len, part);
   } else if (kw == 0 && active) {
-    if (P.nsplit == 1) {
+    if (!part) {
       // whole rows through LDS
       constexpr int ORS = 2 * D + 16;
       const float inv = row_inv(seen != 0.f, l_run);
@@ -941,7 +1018,7 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
           *reinterpret_cast<u32x4*>(P.out + b * P.o_sb + (r / P.G) * P.o_ss + (h * P.G + r % P.G) * P.o_sh + 8 * (lane % CH)) = v;
       }
     } else if (r0 + 32 * qw + l32 < R) {
-      float* dst = P.part + (((int64_t)bh * R + row) * P.nsplit + split) * kPart<D>;
+      float* dst = part + (row - r0) * kPart<D>;
       if (hh == 0) *reinterpret_cast<f32x4*>(dst) = f32x4{m_run, l_run, seen, 0.f};
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
@@ -951,36 +1028,51 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
               f32x4{oacc[dt][4 * m], oacc[dt][4 * m + 1], oacc[dt][4 * m + 2], oacc[dt][4 * m + 3]};
     }
   }
-  append_share<D>(P, b, h, len, rb * P.nsplit + split, P.nrb * P.nsplit);
+  append_share<D>(P, b, h, len, sc.rb * sc.pieces + sc.piece, P.nrb * sc.pieces);
 }
 
-// One wave per (b, h, r): lane s weighs split s, then D / 4 lanes a split add their four columns.
-template <int D>
+// One wave per (b, h, r) of a unit of several pieces: lane i weighs the i-th, and D / 4 lanes a piece add their four
+// columns, 64 pieces at a time. Bound by its three loads one after another: what the sequence's units were cut into, the
+// pieces' maxima and sums, their results.
+template <int D, int RB>
 __global__ __launch_bounds__(256) void combine_kernel(Params P) {
   constexpr int L4 = D / 4, NG = 64 / L4;
   const int R = P.S * P.G;
-  const int64_t u = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 6;
   const int lane = threadIdx.x & 63, col = lane % L4, grp = lane / L4;
-  if (u >= (int64_t)P.B * P.Hkv * R) return;
-  const float* src = P.part + u * P.nsplit * kPart<D>;
-  const int n = P.nsplit;   // at most 64
-  f32x4 head = {-INFINITY, 0.f, 0.f, 0.f};
-  if (lane < n) head = *reinterpret_cast<const f32x4*>(src + lane * kPart<D>);
-  const float M = wave_max(head[0]);
-  const float wgt = head[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(head[0] - M);
-  float L = wgt * head[1];
-  const bool seen = __builtin_amdgcn_ballot_w64(head[2] != 0.f) != 0;
+  const int u = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (u >= P.B * P.Hkv * R) return;
+  const int bh = u / R, r = u - bh * R, b = bh / P.Hkv, h = bh - b * P.Hkv, rb = r / RB;
+  uniform_i32* const pre = uniform(P.pre);
+  const int base = pre[b], n = (pre[b + 1] - base) / (P.Hkv * P.nrb);
+  if (n == 1) return;
+  const float* src = P.part + ((int64_t)(base + (h * P.nrb + rb) * n) * RB + (r - rb * RB)) * kPart<D>;
+  constexpr int64_t kNext = (int64_t)RB * kPart<D>;
+  float M = -INFINITY, L = 0.f;
+  bool seen = false;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = grp; s0 < n + grp; s0 += 8 * NG) {
-    // eight loads in flight; past the last split its partial again, not added (it may be inf)
-    f32x4 o[8];
+  for (int p0 = 0; p0 < n; p0 += 64) {
+    const int m = min(64, n - p0);
+    f32x4 head = {-INFINITY, 0.f, 0.f, 0.f};
+    if (lane < m) head = *reinterpret_cast<const f32x4*>(src + (p0 + lane) * kNext);
+    const float before = M;
+    M = fmaxf(M, wave_max(head[0]));
+    const float ref = max_ref(M), alpha = __builtin_amdgcn_exp2f(before - ref);   // 0 at first
+    const float wgt = __builtin_amdgcn_exp2f(head[0] - ref);
+    L = L * alpha + wgt * head[1];
+    acc *= alpha;
+    seen = seen || __builtin_amdgcn_ballot_w64(head[2] != 0.f) != 0;
+    for (int s0 = 0; s0 < m; s0 += 8 * NG) {
+      // eight loads in flight; past the last piece it again, not added (it may be inf)
+      f32x4 o[8];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) o[x] = *reinterpret_cast<const f32x4*>(src + min(s0 + NG * x, n - 1) * kPart<D> + 4 + 4 * col);
+      for (int x = 0; x < 8; ++x)
+        o[x] = *reinterpret_cast<const f32x4*>(src + (p0 + min(s0 + grp + NG * x, m - 1)) * kNext + 4 + 4 * col);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const int at = s0 + NG * x;
-      const f32x4 y = acc + __shfl(wgt, at & 63) * o[x];
-      acc = at < n ? y : acc;
+      for (int x = 0; x < 8; ++x) {
+        const int at = s0 + grp + NG * x;
+        const f32x4 y = acc + __shfl(wgt, at & 63) * o[x];
+        acc = at < m ? y : acc;
+      }
     }
   }
 #pragma unroll
@@ -990,7 +1082,6 @@ __global__ __launch_bounds__(256) void combine_kernel(Params P) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], m);
   const float inv = row_inv(seen, L);
-  const int r = (int)(u % R), bh = (int)(u / R), h = bh % P.Hkv, b = bh / P.Hkv;
   if (grp == 0)
     *reinterpret_cast<bf16x4*>(P.out + b * P.o_sb + (r / P.G) * P.o_ss + (h * P.G + r % P.G) * P.o_sh + 4 * col) =
         cvt4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);

@@ -25,16 +25,6 @@ __device__ __forceinline__ void arrive() {
   __syncthreads();
 }
 
-// Sum of x over the lanes up to this one
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);   // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);   // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);   // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // row_bcast:31 into rows 2 and 3
-  return x;
-}
 // Sum of x over the threads before this one, and over all (NTH threads). s: 16 ints
 __device__ __forceinline__ int scan(int x, int* s, int* total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, y = wave_scan(x);

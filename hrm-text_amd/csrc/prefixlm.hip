@@ -1878,43 +1878,49 @@ static int table_check(const prefixlm_page_pool& p) {
 }
 static int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
-// R rows share a key-value head's keys: how they are cut into blocks, and the keys into splits.
-static int pg_rows(int64_t R) { return R <= 4 ? 4 : R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }   // of a block
-static int64_t pg_nrb(int64_t R) { return (R + pg_rows(R) - 1) / pg_rows(R); }
-static int64_t pg_nsplit(int64_t B, int64_t Hkv, int64_t R, int64_t cap) {
-  const int64_t units = B * Hkv * pg_nrb(R), most = (cap + 4 * pkv::kKeys - 1) / (4 * pkv::kKeys);
-  return std::max<int64_t>(1, std::min({((R > 4 ? 512 : 768) + units - 1) / units, most, (int64_t)pkv::kMaxSplits}));
+// R rows share a key-value head's keys: the rows of a block, whose keys are a unit's, the keys of a tile, the
+// workgroups that the units share (0: one for each unit), and the workspace of their pieces.
+static int pg_rows(int64_t B, int64_t Hkv, int64_t R) {
+  if (R <= 64) return R == 1 ? 1 : R <= 16 ? 16 : 64;
+  const int64_t heads = B * Hkv;
+  return heads * ((R + 127) / 128) < 512 && heads * ((R + 63) / 64) >= 512 ? 64 : 128;
+}
+static int pg_tile(int rows, int D) { return rows == 1 ? (D == 128 ? 64 : 128) : rows == 16 ? 4 * pkv::kKeys : 64; }
+static int pg_nwg(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
+  const int rows = pg_rows(B, Hkv, R), tile = pg_tile(rows, D), most = rows == 1 ? 768 : 512;
+  const int64_t units = B * Hkv * ((R + rows - 1) / rows), tiles = units * ((cap + tile - 1) / tile);
+  if (B > pkv::kMaxShared || 2 * units > most || tiles <= units) return 0;
+  if (cap <= (rows == 1 ? 384 : 256) || (units >= 128 && cap <= 512) || (units >= 256 && rows == 1 && cap <= 2048)) return 0;
+  return (int)std::min<int64_t>(most, tiles);
+}
+static size_t pg_workspace(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
+  const int n = pg_nwg(B, Hkv, R, D, cap);
+  return n == 0 ? 0 : align_up(sizeof(int32_t) * (B + 1)) + align_up(sizeof(float) * (size_t)n * pg_rows(B, Hkv, R) * (D + 4));
 }
 
 template <int D>
-static void pg_launch(const pkv::Params& P, int64_t nblk, hipStream_t stream) {
+static void pg_launch(const pkv::Params& P, unsigned nblk, hipStream_t stream) {
   const int64_t R = (int64_t)P.S * P.G;
-  const dim3 g((unsigned)nblk), n(pkv::NT);
-  switch (pg_rows(R)) {
-    case 4:
-      if (R == 1)
-        hipLaunchKernelGGL((pkv::decode_kernel<D, 1, pkv::NT>), g, n, 0, stream, P);
-      else if (R == 2)
-        hipLaunchKernelGGL((pkv::decode_kernel<D, 2, pkv::NT>), g, n, 0, stream, P);
-      else
-        hipLaunchKernelGGL((pkv::decode_kernel<D, 4, pkv::NT>), g, n, 0, stream, P);
+  const dim3 g(nblk), n(pkv::NT), c((unsigned)((P.B * P.Hkv * R + 3) / 4));
+  switch (pg_rows(P.B, P.Hkv, R)) {
+    case 1:
+      hipLaunchKernelGGL((pkv::decode_kernel<D>), g, n, 0, stream, P);
+      if (P.nwg) hipLaunchKernelGGL((pkv::combine_kernel<D, 1>), c, n, 0, stream, P);
       break;
     case 16:
-      hipLaunchKernelGGL((pkv::stream_kernel<D, 1>), g, n, 0, stream, P);
-      break;
-    case 32:
-      hipLaunchKernelGGL((pkv::stream_kernel<D, 2>), g, n, 0, stream, P);
+      hipLaunchKernelGGL((pkv::stream_kernel<D>), g, n, 0, stream, P);
+      if (P.nwg) hipLaunchKernelGGL((pkv::combine_kernel<D, 16>), c, n, 0, stream, P);
       break;
     case 64:
       hipLaunchKernelGGL((pkv::tile_kernel<D, 2>), g, n, (pkv::TileGeo<D, 2>::LDS_BYTES), stream, P);
+      if (P.nwg) hipLaunchKernelGGL((pkv::combine_kernel<D, 64>), c, n, 0, stream, P);
       break;
     default:
       hipLaunchKernelGGL((pkv::tile_kernel<D, 4>), g, n, (pkv::TileGeo<D, 4>::LDS_BYTES), stream, P);
+      if (P.nwg) hipLaunchKernelGGL((pkv::combine_kernel<D, 128>), c, n, 0, stream, P);
   }
-  if (P.nsplit > 1)
-    hipLaunchKernelGGL((pkv::combine_kernel<D>), dim3((unsigned)((P.B * P.Hkv * R + 3) / 4)), dim3(256), 0, stream, P);
 }
-static_assert(pkv::TileGeo<128, 4>::LDS_BYTES <= 65536 && pkv::TileGeo<64, 2>::LDS_BYTES <= 65536, "within the default limit");
+static_assert(pkv::TileGeo<64, 4>::LDS_BYTES <= 65536 && pkv::TileGeo<64, 2>::LDS_BYTES <= 65536, "within the default limit");
 // The one tile whose LDS is above the default limit, allowed once per device
 static int pg_allow_lds() {
   static std::mutex mu;
@@ -1927,6 +1933,9 @@ static int pg_allow_lds() {
   if (done[dev]) return PREFIXLM_OK;
   e = hipFuncSetAttribute(reinterpret_cast<const void*>(&pkv::tile_kernel<128, 2>), hipFuncAttributeMaxDynamicSharedMemorySize,
                           (pkv::TileGeo<128, 2>::LDS_BYTES));
+  if (e == hipSuccess)
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&pkv::tile_kernel<128, 4>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (pkv::TileGeo<128, 4>::LDS_BYTES));
   if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
   done[dev] = true;
   return PREFIXLM_OK;
@@ -1940,8 +1949,7 @@ size_t prefixlm_paged_workspace_size(int32_t batch, int32_t seqlen_q, int32_t nu
       page_size < 1 || columns < 1)
     return 0;
   const int64_t R = (int64_t)seqlen_q * (num_heads / num_kv_heads);
-  const int64_t n = pg_nsplit(batch, num_kv_heads, R, (int64_t)columns * page_size);
-  return n == 1 ? 0 : align_up(sizeof(float) * (size_t)batch * num_kv_heads * R * n * (head_dim + 4));
+  return pg_workspace(batch, num_kv_heads, R, head_dim, (int64_t)columns * page_size);
 }
 
 int prefixlm_paged_fwd(const prefixlm_paged_args* a, void* stream_) {
@@ -2000,20 +2008,23 @@ int prefixlm_paged_fwd(const prefixlm_paged_args* a, void* stream_) {
   P.scale_log2 = a->softmax_scale * kLog2e;
   const int64_t R = (int64_t)S * P.G;
   if (R > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "seqlen_q=%d x %d heads of a group is too large", S, P.G);
-  P.nsplit = (int)pg_nsplit(P.B, P.Hkv, R, cap);
-  P.nrb = (int)pg_nrb(R);
-  const int64_t units = (int64_t)P.B * P.Hkv * P.nsplit;
-  if (units > 0x7fffffff || P.nrb > 0x7fffffff / ((units + 7) / 8 * 8) || !launchable((units + 7) / 8 * 8 * P.nrb, pkv::NT) ||
-      !launchable(((int64_t)P.B * P.Hkv * R + 3) / 4, 256))
+  const int rows = pg_rows(P.B, P.Hkv, R);
+  P.nrb = (int)((R + rows - 1) / rows);
+  P.nwg = pg_nwg(P.B, P.Hkv, R, pool.head_dim, cap);
+  P.pre = static_cast<int32_t*>(a->workspace);
+  P.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + align_up(sizeof(int32_t) * ((size_t)P.B + 1)));
+  const int64_t units = (int64_t)P.B * P.Hkv;
+  if (units > 0x7ffffff0 || P.nrb > 0x7fffffff / ((units + 7) / 8 * 8) || !launchable((units + 7) / 8 * 8 * P.nrb, pkv::NT) ||
+      !launchable((units * R + 3) / 4, 256))
     return fail(PREFIXLM_ERR_INVALID, "grid too large");
-  const int64_t nblk = pg_rows(R) > 4 ? (units + 7) / 8 * 8 * P.nrb : units;
+  const int64_t nblk = P.nwg ? P.nwg : (units + 7) / 8 * 8 * P.nrb;
   rc = pg_allow_lds();
   if (rc) return rc;
   (void)hipGetLastError();
   if (pool.head_dim == 128)
-    pg_launch<128>(P, nblk, stream);
+    pg_launch<128>(P, (unsigned)nblk, stream);
   else
-    pg_launch<64>(P, nblk, stream);
+    pg_launch<64>(P, (unsigned)nblk, stream);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "paged kv-cache launch: %s", hipGetErrorString(e));
   return PREFIXLM_OK;
