@@ -222,11 +222,11 @@ __device__ __forceinline__ u32x4 row_chunk(const Params& P, bool there, bool old
 }
 
 // This workgroup's share of the new rows of (b, h), part `part` of `parts`, into their pages
-template <int D>
+template <int D, int NTH = NT>
 __device__ __forceinline__ void append_share(const Params& P, int b, int h, int len, int part, int parts) {
   constexpr int CH = D / 8;   // 16-byte chunks of a row
   const int c = 8 * (threadIdx.x % CH), is_v = (threadIdx.x / CH) & 1;
-  for (int i = part + parts * (threadIdx.x / (2 * CH)); i < P.s_new; i += parts * (NT / (2 * CH))) {
+  for (int i = part + parts * (threadIdx.x / (2 * CH)); i < P.s_new; i += parts * (NTH / (2 * CH))) {
     const int j = len + i;
     if (j >= P.cap) break;
     const int page = P.table[b * P.table_sb + (j >> P.ps_log2)];
@@ -315,9 +315,9 @@ __device__ __forceinline__ float lanes_sum(float x) {
 // where there is much to read (64 x 16 heads on 2150-3993 rows, 1.6 GB: 257 us, 6.2 TB/s; 3 x 12 on 16000-29000 65 us,
 // 5.6), by the chain of length, page, keys, joining where there is little (16 heads on 900 rows 9.8 us with the
 // combine). The matrix cores (stream) are as fast on the former and 0.6 to 1.2 us slower on the latter.
-template <int D>
-__global__ __launch_bounds__(NT) void decode_kernel(Params P) {
-  constexpr int CH = D / 8, RPL = 64 / CH, NH = D == 128 ? 1 : 2, U = 16 / RPL;
+template <int D, int NTH>
+__global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
+  constexpr int NWAVE = NTH / 64, CH = D / 8, RPL = 64 / CH, NH = D == 128 ? 1 : 2, U = 16 / RPL;
   constexpr int kStep = 16 * NH * NWAVE;     // keys of a workgroup's step, a tile
   __shared__ float s_m[NWAVE], s_l[NWAVE], s_seen[NWAVE];
   __shared__ f32x4 s_o[NWAVE][D / 4];
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(NT) void decode_kernel(Params P) {
           cvt4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     }
   }
-  append_share<D>(P, b, h, len, sc.piece, sc.pieces);
+  append_share<D, NTH>(P, b, h, len, sc.piece, sc.pieces);
 }
 
 // ---- up to 16 rows -------------------------------------------------------------------------------

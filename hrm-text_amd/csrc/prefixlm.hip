@@ -1878,19 +1878,29 @@ static int table_check(const prefixlm_page_pool& p) {
 }
 static int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
-// R rows share a key-value head's keys: the rows of a block, whose keys are a unit's, the keys of a tile, the
-// workgroups that the units share (0: one for each unit), and the workspace of their pieces.
+// R rows share a key-value head's keys. The rows of a block, which picks the kernel: one token of ungrouped heads alone;
+// up to 16 (64 x 4 key-value heads of four on 2150-3993 rows 75 us, 80 without the matrix cores); blocks of 64 from 17
+// on, most of which may be empty (24 x 4 heads, 20 rows, on 1720-3194 34 us, 40 with 32 rows of 16 in the kernel for
+// 16), where 128 fill the chip or 64 do not either, 128 (16 x 16 heads, 512 rows, on 6000-7000 945 us, 1050 by 64; 4 x 16
+// x 509 on 1433-2662 147 with two pieces a unit, 124 by 64 without pieces).
 static int pg_rows(int64_t B, int64_t Hkv, int64_t R) {
   if (R <= 64) return R == 1 ? 1 : R <= 16 ? 16 : 64;
   const int64_t heads = B * Hkv;
   return heads * ((R + 127) / 128) < 512 && heads * ((R + 63) / 64) >= 512 ? 64 : 128;
 }
+// Keys of a tile
 static int pg_tile(int rows, int D) { return rows == 1 ? (D == 128 ? 64 : 128) : rows == 16 ? 4 * pkv::kKeys : 64; }
+// The workgroups that the units share, 0: one for each unit. Two a CU, three of the smaller ones for one row (16 heads x
+// 12 on 16000-29000 rows 65 us with 768, 63 with 512, 66 with 1024), unless units are as good as enough, or their
+// keys take less time than the combine's launch. One row, one workgroup of 512 threads a unit against 768 that
+// share: 16 units of 512 rows 7.5 and 9.5 us, of 1024 11.6 and 9.9; 64 of 1024 13.7 and 14.6, of 1536 18.5 and 16.2;
+// 128 of 1024 15.1 and 18.5; 256 of 2048 35.6 and 39. More rows: 16 units of 256 8.8 and 11.0, of 512 13.0 and 11.4; 128 of
+// 512 14.6 and 15.3.
 static int pg_nwg(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
   const int rows = pg_rows(B, Hkv, R), tile = pg_tile(rows, D), most = rows == 1 ? 768 : 512;
   const int64_t units = B * Hkv * ((R + rows - 1) / rows), tiles = units * ((cap + tile - 1) / tile);
   if (B > pkv::kMaxShared || 2 * units > most || tiles <= units) return 0;
-  if (cap <= (rows == 1 ? 384 : 256) || (units >= 128 && cap <= 512) || (units >= 256 && rows == 1 && cap <= 2048)) return 0;
+  if (rows == 1 ? cap <= 768 + 5 * units : cap <= 256 || (units >= 128 && cap <= 512)) return 0;
   return (int)std::min<int64_t>(most, tiles);
 }
 static size_t pg_workspace(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
@@ -1904,7 +1914,10 @@ static void pg_launch(const pkv::Params& P, unsigned nblk, hipStream_t stream) {
   const dim3 g(nblk), n(pkv::NT), c((unsigned)((P.B * P.Hkv * R + 3) / 4));
   switch (pg_rows(P.B, P.Hkv, R)) {
     case 1:
-      hipLaunchKernelGGL((pkv::decode_kernel<D>), g, n, 0, stream, P);
+      if (P.nwg)
+        hipLaunchKernelGGL((pkv::decode_kernel<D, pkv::NT>), g, n, 0, stream, P);
+      else
+        hipLaunchKernelGGL((pkv::decode_kernel<D, 512>), g, dim3(512), 0, stream, P);
       if (P.nwg) hipLaunchKernelGGL((pkv::combine_kernel<D, 1>), c, n, 0, stream, P);
       break;
     case 16:
@@ -2014,7 +2027,7 @@ int prefixlm_paged_fwd(const prefixlm_paged_args* a, void* stream_) {
   P.pre = static_cast<int32_t*>(a->workspace);
   P.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + align_up(sizeof(int32_t) * ((size_t)P.B + 1)));
   const int64_t units = (int64_t)P.B * P.Hkv;
-  if (units > 0x7ffffff0 || P.nrb > 0x7fffffff / ((units + 7) / 8 * 8) || !launchable((units + 7) / 8 * 8 * P.nrb, pkv::NT) ||
+  if (units > 0x7ffffff0 || P.nrb > 0x7fffffff / ((units + 7) / 8 * 8) || !launchable((units + 7) / 8 * 8 * P.nrb, 512) ||
       !launchable((units * R + 3) / 4, 256))
     return fail(PREFIXLM_ERR_INVALID, "grid too large");
   const int64_t nblk = P.nwg ? P.nwg : (units + 7) / 8 * 8 * P.nrb;

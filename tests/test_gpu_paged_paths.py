@@ -54,7 +54,7 @@ def _shares(B, S, Hq, Hkv, D, ps, M):
 
 
 # rows that share keys, key-value heads, sequences, capacity, whether the units are cut into pieces
-SIZES = [(1, 1, 2, 2, 384, False), (1, 1, 2, 2, 400, True), (1, 1, 16, 8, 512, False), (1, 1, 20, 13, 4096, True),
+SIZES = [(1, 1, 2, 2, 784, False), (1, 1, 2, 2, 800, True), (1, 1, 16, 8, 512, False), (1, 1, 20, 13, 4096, True),
          (1, 1, 96, 4, 640, False), (1, 1, 100, 4, 640, False), (2, 1, 2, 2, 256, False), (2, 1, 2, 2, 272, True),
          (1, 16, 16, 8, 512, False), (1, 7, 32, 8, 640, True), (3, 5, 65, 4, 640, False), (5, 4, 3, 2, 256, False),
          (17, 1, 2, 2, 640, True), (32, 2, 33, 8, 384, False), (64, 1, 2, 1, 1280, True), (65, 1, 2, 2, 256, False),
