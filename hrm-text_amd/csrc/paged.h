@@ -94,7 +94,10 @@ __device__ __forceinline__ float rows_sum(float x) {
 // P.nwg the units of a sequence of t tiles are cut into n(t) = ceil(t / c) pieces each, c the smallest length, of
 // those that a few bisections try, at which all pieces together are at most P.nwg: the pieces are then of nearly
 // the same length, whatever the sequences' are, and all in flight at once. Each wave finds c by itself, lane i
-// holding sequences i, i + 64, ...
+// holding sequences i, i + 64, ... It costs 1 us of a call and saves what the longest sequence took more than the
+// others with as many pieces for each (48 x 2 heads on 6900-12700 rows 92 us with eight, now 85; 3 x 12 on 16000-29000 72
+// with 16, now 65). Dealing the tiles out evenly, wherever units begin and end, was as fast for one row and slower for
+// several (24 x 4 heads of 20 rows 48 us where pieces took 40): a workgroup then begins and ends two units.
 template <int RB, int TS>
 struct Sched {
   int b, h, rb, len, first, count, piece, pieces, wg;
@@ -715,7 +718,7 @@ __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
   append_share<D>(P, b, h, len, sc.piece, sc.pieces);
 }
 
-// ---- many rows -----------------------------------------------------------------------------------
+// ---- more rows ------------------------------------------------------------------------------------
 // Workgroup = 32 QW rows of (b, h, split): QW waves along the rows and KW = 4 / QW along the keys, as the
 // contiguous cache's extend kernel: a staged tile of 32 KW keys serves all of them, S^T = K Q^T with the
 // row as the lane column, V^T from transposing reads.
@@ -1032,8 +1035,8 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
 }
 
 // One wave per (b, h, r) of a unit of several pieces: lane i weighs the i-th, and D / 4 lanes a piece add their four
-// columns, 64 pieces at a time. Bound by its three loads one after another: what the sequence's units were cut into, the
-// pieces' maxima and sums, their results.
+// columns, 64 pieces at a time. Bound by its loads one after another, what the sequence's units were cut into, then the
+// pieces: 3.3 us with the launch for 16 rows of 14 pieces, 4.7 for 768 of five.
 template <int D, int RB>
 __global__ __launch_bounds__(256) void combine_kernel(Params P) {
   constexpr int L4 = D / 4, NG = 64 / L4;

@@ -1885,6 +1885,7 @@ static int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 // x 509 on 1433-2662 147 with two pieces a unit, 124 by 64 without pieces).
 static int pg_rows(int64_t B, int64_t Hkv, int64_t R) {
   if (R <= 64) return R == 1 ? 1 : R <= 16 ? 16 : 64;
+  if (B >= 512 || Hkv >= 512) return 128;
   const int64_t heads = B * Hkv;
   return heads * ((R + 127) / 128) < 512 && heads * ((R + 63) / 64) >= 512 ? 64 : 128;
 }
@@ -1897,9 +1898,10 @@ static int pg_tile(int rows, int D) { return rows == 1 ? (D == 128 ? 64 : 128) :
 // 128 of 1024 15.1 and 18.5; 256 of 2048 35.6 and 39. More rows: 16 units of 256 8.8 and 11.0, of 512 13.0 and 11.4; 128 of
 // 512 14.6 and 15.3.
 static int pg_nwg(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
+  if (B > pkv::kMaxShared || Hkv > 512) return 0;
   const int rows = pg_rows(B, Hkv, R), tile = pg_tile(rows, D), most = rows == 1 ? 768 : 512;
   const int64_t units = B * Hkv * ((R + rows - 1) / rows), tiles = units * ((cap + tile - 1) / tile);
-  if (B > pkv::kMaxShared || 2 * units > most || tiles <= units) return 0;
+  if (2 * units > most || tiles <= units) return 0;
   if (rows == 1 ? cap <= 768 + 5 * units : cap <= 256 || (units >= 128 && cap <= 512)) return 0;
   return (int)std::min<int64_t>(most, tiles);
 }
