@@ -1205,8 +1205,8 @@ PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t cap = c.table.size(1) * c.k.size(3);
   if (B != c.table.size(0) || D != c.k.size(4) || Hq % Hkv || S > INT32_MAX || Hq > INT32_MAX || cap > INT32_MAX) return none();
   if (has_new && (k.sizes() != at::IntArrayRef({B, S, Hkv, D}) || v.sizes() != k.sizes())) return none();
-  if (!apart({c.k, c.v, c.refs, c.table}, {q, k, v})) return none();
   if (!lens.parse(a[7], q, B) || (!lens.t.defined() && (lens.c < 0 || lens.c > cap))) return none();
+  if (!apart({c.k, c.v, c.refs, c.table}, {q, k, v, lens.t})) return none();
   if (a[8] == Py_None)
     scale = 1.0 / std::sqrt((double)D);
   else if (!get_double(a[8], &scale))
@@ -1271,7 +1271,7 @@ PyObject* py_pages_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Pages c;
   RowCounts lens, more;
   if (!ready(n, 6) || c10::InferenceMode::is_enabled() || !c.parse(a) || c.pool.batch > 8192 || !lens.parse(a[4], c.k, c.pool.batch) ||
-      !more.parse(a[5], c.k, c.pool.batch) || !apart({c.k, c.v, c.refs, c.table}, {}))
+      !more.parse(a[5], c.k, c.pool.batch) || !apart({c.k, c.v, c.refs, c.table}, {lens.t, more.t}))
     return none();
   Tensor out;
   {
@@ -1294,7 +1294,7 @@ PyObject* py_pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Pages c;
   Tensor parents;
   if (!ready(n, 3) || c10::InferenceMode::is_enabled() || !c.parse_counts(a, 16) || c.pool.batch > 8192 || !get_tensor(a[2], &parents) ||
-      !meta(parents, c.refs) || parents.numel() != c.pool.batch || !apart({c.refs, c.table}, {}))
+      !meta(parents, c.refs) || parents.numel() != c.pool.batch || !apart({c.refs, c.table}, {parents}))
     return none();
   {
     pybind11::gil_scoped_release no_gil;
@@ -1313,7 +1313,7 @@ PyObject* py_pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Scalar ps;
   RowCounts keep;
   if (!ready(n, 4) || c10::InferenceMode::is_enabled() || !PyLong_CheckExact(a[2]) || !get_scalar(a[2], &ps) || ps.v < 16 || ps.v > 1024 ||
-      !c.parse_counts(a, ps.v) || !keep.parse(a[3], c.refs, c.pool.batch) || !apart({c.refs, c.table}, {}))
+      !c.parse_counts(a, ps.v) || !keep.parse(a[3], c.refs, c.pool.batch) || !apart({c.refs, c.table}, {keep.t}))
     return none();
   {
     pybind11::gil_scoped_release no_gil;
@@ -1358,7 +1358,7 @@ PyObject* py_pages_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return none();
   }
   if (!get_tensor(a[8], &src) || !get_tensor(a[9], &dst) || !meta(src, c.k) || !meta(dst, c.k) || src.dim() != 1 ||
-      src.sizes() != dst.sizes() || src.numel() == 0)
+      src.sizes() != dst.sizes() || src.numel() == 0 || !apart({c.k, c.v}, {src, dst}))
     return none();
   {
     pybind11::gil_scoped_release no_gil;

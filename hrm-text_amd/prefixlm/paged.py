@@ -151,8 +151,8 @@ def paged_kvcache_attn(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], k_pa
             _check4(x, name)
             if tuple(x.shape) != (B, S, Hkv, D) or x.device != dev:
                 raise ValueError(f"{name} must be [{B}, {S}, {Hkv}, {D}] on {dev} (got {tuple(x.shape)} on {x.device})")
-    _apart((k_pages, v_pages, refs, page_table), (q,) if k is None else (q, k, v))
     lens, _ = _rows(cache_seqlens, B, dev, "cache_seqlens")
+    _apart((k_pages, v_pages, refs, page_table), [x for x in (q, k, v, lens) if x is not None])
     if lens is None and not 0 <= cache_seqlen <= cap:
         raise ValueError(f"cache_seqlens = {cache_seqlen} is outside [0, {cap}]")
     lib = _capi.load()
@@ -219,9 +219,9 @@ def _reserve(k_pages: Tensor, v_pages: Tensor, refs: Tensor, page_table: Tensor,
     _check_pages(k_pages, v_pages)
     dev, N = k_pages.device, page_table.shape[0]
     _check_table(refs, page_table, k_pages.shape[1], dev, MAX_SEQUENCES)
-    _apart((k_pages, v_pages, refs, page_table))
     lens, _ = _rows(cache_seqlens, N, dev, "cache_seqlens")
     new, _ = _rows(new_rows, N, dev, "new_rows")
+    _apart((k_pages, v_pages, refs, page_table), [x for x in (lens, new) if x is not None])
     short = torch.empty(N, dtype=torch.int32, device=dev)
     _call("prefixlm_pages_reserve", dev, _pool(k_pages, v_pages, refs, page_table), True, rows=_ptr(lens), row_const=cache_seqlen,
           new_rows=_ptr(new), new_row_const=new_row, result=_ptr(short))
@@ -240,7 +240,8 @@ def paged_kvcache_reserve(cache: PagedKVCache, cache_seqlens: Union[int, Tensor,
     sequences and columns; of a page whose holders all ask for it in this call the first keeps it. Where a
     shared page is left, its rows below ``cache_seqlens`` are copied, in every layer. Returns int32 [batch]:
     how many columns are left without a page of their own, 0 as long as pages last; new rows in these are not stored
-    by ``flash_attn_with_paged_kvcache``. At most 8192 sequences."""
+    by ``flash_attn_with_paged_kvcache``. Rows below ``cache_seqlens`` that no page held, such as these, hold what their
+    page held before once they are given one. At most 8192 sequences."""
     if cache_seqlens is None:
         cache_seqlens = 0
     native = _native_calls()
@@ -259,8 +260,8 @@ def _fork(refs: Tensor, page_table: Tensor, parents: Tensor) -> None:
     if dev.type != "cuda":
         raise ValueError(f"the cache must be on a GPU (got {dev})")
     _check_table(refs, page_table, None, dev, MAX_SEQUENCES)
-    _apart((refs, page_table))
     src, _ = _rows(parents, page_table.shape[0], dev, "parents")
+    _apart((refs, page_table), (src,))
     _call("prefixlm_pages_fork", dev, _pool(None, None, refs, page_table, (1, refs.shape[0], 1, 16, 64)), src=_ptr(src))
 
 
@@ -287,8 +288,8 @@ def _free(refs: Tensor, page_table: Tensor, page_size: int, keep_rows: Optional[
     if dev.type != "cuda":
         raise ValueError(f"the cache must be on a GPU (got {dev})")
     _check_table(refs, page_table, None, dev)
-    _apart((refs, page_table))
     keep, _ = _rows(keep_rows, page_table.shape[0], dev, "keep_rows")
+    _apart((refs, page_table), () if keep is None else (keep,))
     _call("prefixlm_pages_free", dev, _pool(None, None, refs, page_table, (1, refs.shape[0], 1, page_size, 64)), rows=_ptr(keep),
           row_const=keep_row)
 
@@ -351,9 +352,9 @@ def _copy(k_pages: Tensor, v_pages: Tensor, k_source: Optional[Tensor], v_source
         raise ValueError(f"src {tuple(src.shape)} and dst {tuple(dst.shape)} must be lists of the same length")
     n = src.numel()
     src, dst = _rows(src, n, dev, "src")[0], _rows(dst, n, dev, "dst")[0]
-    _apart(pools)
     if not n:
         return
+    _apart(pools, (src, dst))
     word = torch.empty((1, 1), dtype=torch.int32, device=dev)   # neither table nor refs are read
     pool = _pool(k_pages, v_pages, word, word)
     source = _pool(k_source, v_source, word, word) if k_source is not None else None
