@@ -35,6 +35,7 @@ constexpr int NT = 256;
 constexpr int NWAVE = NT / 64;
 constexpr int kKeys = 32;          // keys of a wave's step
 constexpr int kMaxShared = 256;    // sequences of a call whose units are cut
+constexpr float kAbove = 8.f;      // log2 of how far a weight may pass the largest one so far (tile)
 // floats per partial: max (log2 units), sum, whether a key was seen, unused, o[D]
 template <int D>
 constexpr int kPart = D + 4;
@@ -71,6 +72,9 @@ __device__ __forceinline__ int keys_seen(const Params& P, int len, int i) {
   const int lk = min(P.cap, len + P.s_new);
   return P.causal ? min(lk, len + P.s_new - P.S + i + 1) : lk;
 }
+// Weights are taken 2^spread below the largest score's, so that the n of a row add up to at most 1/2 and what they weigh
+// stays within fp32's range wherever the values do
+__device__ __forceinline__ float spread(int n) { return (float)(33 - __builtin_clz(max(n, 1))); }
 // 1 / (sum of the weights): a row that sees no key is 0, one whose scores are all -inf NaN
 __device__ __forceinline__ float row_inv(bool seen, float sum) { return seen ? 1.f / sum : 0.f; }
 
@@ -111,14 +115,30 @@ struct Sched {
     piece = first = 0;
     pieces = 1;
     if (P.nwg == 0) {
-      // row blocks of one (b, h) eight indices apart, on one XCD
-      rb = (int)((blockIdx.x >> 3) % P.nrb);
-      const int u = (int)((blockIdx.x >> 3) / P.nrb) * 8 + (blockIdx.x & 7);
+      // Row blocks of one (b, h) eight indices apart, on one XCD. The longest sequences first (16 x 16 x 512 rows on
+      // 1000-7000 612 us in their own order, 506 so), and of an XCD's 64 workgroups that start at once, two a CU, the later
+      // 32 the other way round, so that a long one shares its CU with a short one (4 x 16 x 509 on 1433-2662 2 us of 105)
+      int j = (int)(blockIdx.x >> 3);
+      const int most = min((int)(gridDim.x >> 3), 64);
+      if (RB >= 64 && j >= 32 && j < most) j = 31 + most - j;
+      rb = P.nrb - 1 - j % P.nrb;
+      const int u = j / P.nrb * 8 + (int)(blockIdx.x & 7);
       if (u >= P.B * P.Hkv) return false;
       wg = 0;
       h = u % P.Hkv;
       b = u / P.Hkv;
-      len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
+      if (RB >= 64 && P.seqlens && P.B > 1 && P.B <= 64) {
+        const int mine = lane < P.B ? cache_len(P, lane) : -1;
+        int at = 0;
+        for (int i = 0; i < P.B; ++i) {
+          const int other = __builtin_amdgcn_readlane(mine, i);
+          at += other > mine || (other == mine && i < lane);
+        }
+        b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < P.B && at == b));
+        len = __builtin_amdgcn_readlane(mine, b);
+      } else {
+        len = __builtin_amdgcn_readfirstlane(cache_len(P, b));
+      }
       count = tiles(P, len, rb);
       return true;
     }
@@ -245,9 +265,9 @@ __device__ __forceinline__ void append_share(const Params& P, int b, int h, int 
 // Rows [r0, r1) over keys [k0, k1) without the matrix cores: 16 lanes a row, key by key. For pieces
 // whose values hold an infinity or NaN (0 * inf in P V would reach rows that must not see the key), and
 // for scores that pass fp32's range before the softmax scale, or whose largest is about -3e38: here the
-// scale comes first.
+// scale comes first. down: what the unit's other pieces take the weights below.
 template <int D>
-__device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int r0, int r1, int k0, int k1, int len, float* part) {
+__device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int r0, int r1, int k0, int k1, int len, float down, float* part) {
   constexpr int E = D / 16;
   const int g16 = threadIdx.x & 15;
   auto get = [&](const bf16* p, float* f) {
@@ -282,7 +302,7 @@ __device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int r0,
       for (int e = 0; e < E; ++e) s += q[e] * x[e];
       s = row16_sum(s);
       const float mx = fmaxf(m, s), ref = max_ref(mx);
-      const float alpha = __builtin_amdgcn_exp2f(m - ref), p = __builtin_amdgcn_exp2f(s - ref);
+      const float alpha = __builtin_amdgcn_exp2f(m - ref), p = __builtin_amdgcn_exp2f(s - (ref + down));
       m = mx;
       l = l * alpha + p;
       get(vr, x);
@@ -378,6 +398,7 @@ __global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
     load(j0);
     look(j0 + kStep);
   }
+  const float down = spread(lk);
   float q[8], o[8], m = -INFINITY, l = 0.f, seen = 0.f;
   {
     const u32x4 x = *reinterpret_cast<const u32x4*>(P.q + b * P.q_sb + h * P.q_sh + c8);
@@ -428,7 +449,7 @@ __global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
     for (int hf = 0; hf < NH; ++hf)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float p = __builtin_amdgcn_exp2f(s[hf][u] - ref);
+        const float p = __builtin_amdgcn_exp2f(s[hf][u] - (ref + down));
         l += p;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -567,6 +588,7 @@ __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
     }
   };
 
+  const float down = spread(lk);
   float m_run = -INFINITY, l_run = 0.f, seen = 0.f;
   f32x4 oacc[ND];
 #pragma unroll
@@ -632,7 +654,7 @@ __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) oacc[d] *= alpha;
       }
-      const float m_use = max_ref(m_run);
+      const float m_use = max_ref(m_run) + down;
       float e[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -681,7 +703,7 @@ __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
   }
   __syncthreads();
   if (s_bad) {
-    walk_rows<D>(P, b, h, 0, R, k0, k1, len, part);
+    walk_rows<D>(P, b, h, 0, R, k0, k1, len, down, part);
   } else if (const int r = tid >> 4; r < R) {
     constexpr int E = D / 16;
     float M = s_m[0][r], L = 0.f, any = 0.f, x[E];
@@ -719,9 +741,18 @@ __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
 }
 
 // ---- more rows ------------------------------------------------------------------------------------
-// Workgroup = 32 QW rows of (b, h, split): QW waves along the rows and KW = 4 / QW along the keys, as the
-// contiguous cache's extend kernel: a staged tile of 32 KW keys serves all of them, S^T = K Q^T with the
-// row as the lane column, V^T from transposing reads.
+// Workgroup = 32 QW rows of (b, h) over a unit's or a piece's keys: QW waves along the rows and KW = 4 / QW along the
+// keys; a staged tile of 64 keys serves all of them. S^T = K Q^T with the row as the lane column, V^T from transposing
+// reads. What it is made of, as 4 x 16 heads x 509 rows on 1433-2662 went from 124 us to 84 (420 TFLOP/s; 16 x 16 x 512
+// on 6000-7000 from 890 to 703, 640 TFLOP/s):
+//  - the weights go into P V as two bf16 terms, each rounded to nearest: off by 2^-16 of a weight, a 256th of out's own
+//    rounding, where three would hold all 24 bits for a third more matrix products;
+//  - what a row's weights are relative to (m_run) is raised only once one passes it by 2^kAbove: any reference does;
+//  - the scale is applied with that reference in one fma: to |scale|, a negative one having turned q's signs;
+//  - tiles in one page or of new rows alone are loaded off one base, with the bounds that the buffer checks.
+// Bound by the waves' own chains (two a SIMD): of an iteration's 4200 cycles for two tiles the matrix cores take 1540, the
+// vector instructions 1900, loads and stores alone 2600. Loads that reach further ahead (one word of each line, two to five
+// tiles before) made it 6 to 8% slower.
 template <int D, int QW>
 struct TileGeo {
   static constexpr int KW = 4 / QW, NK = QW == 4 ? 2 : 1;  // waves along the keys; times 32 keys a wave has of a tile
@@ -738,7 +769,7 @@ struct TileGeo {
   static_assert((4 - QW) * MERGE <= LDS_BYTES && QW * OUT <= LDS_BYTES, "epilogue areas fit");
 };
 
-template <int D, int QW>
+template <int D, int QW, bool WIDE>
 __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
   using G = TileGeo<D, QW>;
   constexpr int KW = G::KW, NK = G::NK, TK = G::TK, NP = G::NP, NDT = G::NDT, NS = D / 16, CH = G::CH, RSD = G::RSD;
@@ -768,9 +799,17 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
   const int g16 = __builtin_amdgcn_readfirstlane(srow & ~15);    // this wave's 16 keys of a pass
   const bf16 *const kn = P.k + b * P.k_sb + h * P.k_sh, *const vn = P.v + b * P.v_sb + h * P.v_sh;
   const uint32_t koff = (uint32_t)((srow & 15) * D + 8 * sch) * 2, voff = (uint32_t)((vrow & 15) * D + 8 * sch) * 2;
+  // and of new rows, which 31 bits reach over a tile unless they are very far apart
+  const bool near = P.k_ss < (1 << 23) && P.v_ss < (1 << 23);
+  static_assert(TK == 64, "WIDE: a tile lies in one page");
+  const uint32_t kfar = (uint32_t)((srow & 15) * (int)P.k_ss + 8 * sch) * 2, vfar = (uint32_t)((vrow & 15) * (int)P.v_ss + 8 * sch) * 2;
   u32x4 ks[NP], vs[NP];
   int page[NP];                 // of this wave's keys of the tile to load next
   auto look = [&](int t0) {
+    if (WIDE) {
+      page[0] = t0 < len ? tab[t0 >> P.ps_log2] : -1;
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
       const int j = t0 + G::RPP * n + g16;
@@ -778,16 +817,40 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
     }
   };
   auto load = [&](int t0) {
+    if (WIDE && t0 + TK <= len && (unsigned)page[0] < (unsigned)P.P) {
+      const int64_t at = ((((int64_t)page[0] * P.Hkv + h) << P.ps_log2) + (t0 & psm)) * D;
+      const __amdgpu_buffer_rsrc_t kr = make_rsrc(P.kp + at, TK * D * 2), vr = make_rsrc(P.vp + at, TK * D * 2);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        const int s = (G::RPP * n + g16) * D * 2;
+        ks[n] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)koff, s, 0);
+        vs[n] = __builtin_amdgcn_raw_buffer_load_b128(vr, (int)voff, s, 0);
+      }
+      return;
+    }
+    if (t0 >= len && near) {
+      // new rows; 0 past the last
+      const int rows = min(TK, k1 - t0);
+      const __amdgpu_buffer_rsrc_t kr = make_rsrc(kn + (t0 - len) * P.k_ss, rows > 0 ? (uint32_t)((rows - 1) * (int)P.k_ss + D) * 2 : 0);
+      const __amdgpu_buffer_rsrc_t vr = make_rsrc(vn + (t0 - len) * P.v_ss, rows > 0 ? (uint32_t)((rows - 1) * (int)P.v_ss + D) * 2 : 0);
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        ks[n] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(kfar + (G::RPP * n + g16) * (int)P.k_ss * 2), 0, 0);
+        vs[n] = __builtin_amdgcn_raw_buffer_load_b128(vr, (int)(vfar + (G::RPP * n + g16) * (int)P.v_ss * 2), 0, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
       const int j = t0 + G::RPP * n + g16;
-      const bool held = (unsigned)page[n] < (unsigned)P.P;
-      const int64_t at = ((((int64_t)(held ? page[n] : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
+      const int pg = page[WIDE ? 0 : n];
+      const bool held = j < len && (unsigned)pg < (unsigned)P.P;
+      const int64_t at = ((((int64_t)(held ? pg : 0) * P.Hkv + h) << P.ps_log2) + (j & psm)) * D;
       if (held && j + 16 <= len) {
         ks[n] = page_chunk<false>(page_rows<D>(P.kp + at), koff);
         vs[n] = page_chunk<false>(page_rows<D>(P.vp + at), voff);
       } else {
-        // the last cached rows, the new ones, none: row by row
+        // the last cached rows and the first new ones, rows without a page: row by row
         if (j < min(len, k1) && !held) s_hole = 1;
         const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
         const int jk = j + (srow & 15), jv = j + (vrow & 15);
@@ -796,17 +859,16 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
       }
     }
   };
-  u16x2 vmag = {0, 0};
   auto store = [&](int buf) {
     char* base = smem + buf * G::BUF + srow * RSD + sch * 16;
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
       *reinterpret_cast<u32x4*>(base + G::RPP * n * RSD) = ks[n];
       *reinterpret_cast<u32x4*>(base + G::TILE + G::RPP * n * RSD) = vs[n];
-      vmag = max_mag(vmag, vs[n]);
     }
   };
 
+  const float down = spread(min(P.cap, len + P.s_new)) + kAbove;
   float m_run = -INFINITY, l_run = 0.f, seen = 0.f;
   f32x16 oacc[NDT];
 #pragma unroll
@@ -826,13 +888,19 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
     {
       const bf16* qp = P.q + b * P.q_sb + ri * P.q_ss + rh * P.q_sh + 8 * hh;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(qp + 16 * s);
+      for (int s = 0; s < NS; ++s) {
+        // -q for a negative scale
+        u32x4 x = *reinterpret_cast<const u32x4*>(qp + 16 * s);
+        const uint32_t flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;
+        for (int e = 0; e < 4; ++e) x[e] ^= flip;
+        qf[s] = __builtin_bit_cast(bf16x8, x);
+      }
     }
     store(0);
 #pragma unroll
     for (int s = 0; s < NS; ++s) settle(__builtin_bit_cast(u32x4, qf[s]));
     __syncthreads();
-    const float c = P.scale_log2;
+    const float c = fabsf(P.scale_log2);
     for (int t = 0; t < nt; ++t) {
       const int buf = t & 1;
       if (t + 1 < nt) {
@@ -864,8 +932,6 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
 #pragma unroll
         for (int x = 0; x < NK; ++x) {
           const int kx = kk + 32 * x;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sacc[x][r] *= c;   // before the mask: the scale may have any sign
           if (kx + 32 > min(kall, k1) || hole) {
             // key kx + 8 (r / 4) + 4 hh + r % 4 is seen iff it is below kq, and cached ones have a page
             bool ok[2];
@@ -887,8 +953,8 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sacc[x][r]);
         }
-        mx = halves_max(mx);
-        if (__builtin_amdgcn_ballot_w64(mx > m_run) != 0) {
+        mx = c * halves_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m_run + kAbove) != 0) {
           const float m_new = fmaxf(m_run, mx);
           const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
           m_run = m_new;
@@ -898,41 +964,34 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) oacc[dt][r] *= alpha;
         }
-        const float m_use = max_ref(m_run);
+        const float m_use = max_ref(m_run) + down;
 #pragma unroll
         for (int x = 0; x < NK; ++x) {
           const char* vx = vt + 32 * x * RSD;
           u32x4 xt[2 * NDT];
           xt[0] = lds_read_xt<RSD>(vx, 0, 0);
           xt[1] = lds_read_xt<RSD>(vx, 0, 1);
-          // 16 keys at a time: P's three bf16 terms, which add up to its fp32 bits, times V
+          // 16 keys at a time: P's two bf16 terms times V
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float e[8], ps = 0.f;
-            bf16x8 pt[3];
+            bf16x8 pt[2];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              e[i] = __builtin_amdgcn_exp2f(sacc[x][8 * half + i] - m_use);
+              e[i] = __builtin_amdgcn_exp2f(c * sacc[x][8 * half + i] - m_use);
               ps += e[i];
             }
             l_run += ps;
+            pt[0] = cvt8(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]);
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
-              u32x4 y;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                y[i] = pack_hi(__builtin_bit_cast(uint32_t, e[2 * i]), __builtin_bit_cast(uint32_t, e[2 * i + 1]));
-              pt[n] = __builtin_bit_cast(bf16x8, y);
-#pragma unroll
-              for (int i = 0; i < 8; ++i)   // exact
-                e[i] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, e[i]) & 0xffff0000u);
-            }
+            for (int i = 0; i < 8; ++i) e[i] -= (float)pt[0][i];   // exact
+            pt[1] = cvt8(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]);
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) {
               const int z = NDT * half + dt;
               if (z + 2 < 2 * NDT) xt[z + 2] = lds_read_xt<RSD>(vx, (z + 2) / NDT, (z + 2) % NDT);
 #pragma unroll
-              for (int n = 0; n < 3; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[z]), pt[n], oacc[dt]);
+              for (int n = 0; n < 2; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[z]), pt[n], oacc[dt]);
             }
           }
         }
@@ -944,7 +1003,12 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
   l_run = halves_sum(l_run);
   // a score past the range upwards leaves NaN; one past it downwards (raw below -3.4e38) only counts
   // where every key that the row sees here scores about as low
-  if (vmag[0] >= 0x7f80 || vmag[1] >= 0x7f80 || (seen != 0.f && (l_run != l_run || m_run < 200.f - 3e38f * fabsf(P.scale_log2))))
+  bool bad = false;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bad = bad || !(fabsf(oacc[dt][r]) < INFINITY);
+  if (bad || (seen != 0.f && (l_run != l_run || m_run < 200.f - 3e38f * fabsf(P.scale_log2))))
     s_bad = 1;
   seen = halves_max(seen);
   // the KW waves of 32 rows: waves kw > 0 hand theirs to wave kw = 0
@@ -999,7 +1063,7 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
   __syncthreads();
   float* const part = sc.template partial<D>(P);
   if (s_bad) {
-    walk_rows<D>(P, b, h, r0, r1, k0, k1, len, part);
+    walk_rows<D>(P, b, h, r0, r1, k0, k1, len, down, part);
   } else if (kw == 0 && active) {
     if (!part) {
       // whole rows through LDS

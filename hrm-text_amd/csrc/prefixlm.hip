@@ -1901,7 +1901,7 @@ static int pg_nwg(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
   if (B > pkv::kMaxShared || Hkv > 512) return 0;
   const int rows = pg_rows(B, Hkv, R), tile = pg_tile(rows, D), most = rows == 1 ? 768 : 512;
   const int64_t units = B * Hkv * ((R + rows - 1) / rows), tiles = units * ((cap + tile - 1) / tile);
-  if (2 * units > most || tiles <= units) return 0;
+  if (2 * units > most || tiles <= units || tiles > 0x7fffffff) return 0;   // the kernels add the tiles up in 32 bits
   if (rows == 1 ? cap <= 768 + 5 * units : cap <= 256 || (units >= 128 && cap <= 512)) return 0;
   return (int)std::min<int64_t>(most, tiles);
 }
@@ -1927,16 +1927,22 @@ static void pg_launch(const pkv::Params& P, unsigned nblk, hipStream_t stream) {
       if (P.nwg) hipLaunchKernelGGL((pkv::combine_kernel<D, 16>), c, n, 0, stream, P);
       break;
     case 64:
-      hipLaunchKernelGGL((pkv::tile_kernel<D, 2>), g, n, (pkv::TileGeo<D, 2>::LDS_BYTES), stream, P);
+      if (P.ps_log2 >= 6)
+        hipLaunchKernelGGL((pkv::tile_kernel<D, 2, true>), g, n, (pkv::TileGeo<D, 2>::LDS_BYTES), stream, P);
+      else
+        hipLaunchKernelGGL((pkv::tile_kernel<D, 2, false>), g, n, (pkv::TileGeo<D, 2>::LDS_BYTES), stream, P);
       if (P.nwg) hipLaunchKernelGGL((pkv::combine_kernel<D, 64>), c, n, 0, stream, P);
       break;
     default:
-      hipLaunchKernelGGL((pkv::tile_kernel<D, 4>), g, n, (pkv::TileGeo<D, 4>::LDS_BYTES), stream, P);
+      if (P.ps_log2 >= 6)
+        hipLaunchKernelGGL((pkv::tile_kernel<D, 4, true>), g, n, (pkv::TileGeo<D, 4>::LDS_BYTES), stream, P);
+      else
+        hipLaunchKernelGGL((pkv::tile_kernel<D, 4, false>), g, n, (pkv::TileGeo<D, 4>::LDS_BYTES), stream, P);
       if (P.nwg) hipLaunchKernelGGL((pkv::combine_kernel<D, 128>), c, n, 0, stream, P);
   }
 }
 static_assert(pkv::TileGeo<64, 4>::LDS_BYTES <= 65536 && pkv::TileGeo<64, 2>::LDS_BYTES <= 65536, "within the default limit");
-// The one tile whose LDS is above the default limit, allowed once per device
+// The tiles of 128 columns, whose LDS is above the default limit, allowed once per device
 static int pg_allow_lds() {
   static std::mutex mu;
   static bool done[64] = {};
@@ -1946,11 +1952,12 @@ static int pg_allow_lds() {
   if (dev < 0 || dev >= 64) return fail(PREFIXLM_ERR_INVALID, "device %d >= 64", dev);
   std::lock_guard<std::mutex> g(mu);
   if (done[dev]) return PREFIXLM_OK;
-  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&pkv::tile_kernel<128, 2>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                          (pkv::TileGeo<128, 2>::LDS_BYTES));
-  if (e == hipSuccess)
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&pkv::tile_kernel<128, 4>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                            (pkv::TileGeo<128, 4>::LDS_BYTES));
+  static_assert(pkv::TileGeo<128, 2>::LDS_BYTES == pkv::TileGeo<128, 4>::LDS_BYTES);
+  const void* const tiles[] = {
+      reinterpret_cast<const void*>(&pkv::tile_kernel<128, 2, false>), reinterpret_cast<const void*>(&pkv::tile_kernel<128, 2, true>),
+      reinterpret_cast<const void*>(&pkv::tile_kernel<128, 4, false>), reinterpret_cast<const void*>(&pkv::tile_kernel<128, 4, true>)};
+  for (const void* f : tiles)
+    if (e == hipSuccess) e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (pkv::TileGeo<128, 2>::LDS_BYTES));
   if (e != hipSuccess) return fail(PREFIXLM_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(e));
   done[dev] = true;
   return PREFIXLM_OK;

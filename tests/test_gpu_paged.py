@@ -3,7 +3,9 @@
 Tolerances (u = 2^-24). A score sums up to 128 products in fp32, off by at most 140 u of the sum of their
 magnitudes A, and exponentials of scores off by d change each weight by d relative, a sum of weighted
 rows by 2 d of the sum of p |v|; n keys add n u more, and the splits' joins 100 u. The probabilities enter
-P V as three bf16 terms, their 24 bits. out is rounded to bf16, 2^-8 relative. Pages are equal bit for bit.
+P V as three bf16 terms, their 24 bits, or in blocks of 64 and 128 rows as two, each rounded to nearest: what the first leaves
+is at most 2^-8 of p, what the second leaves of that 2^-8 again, 2^-16 p = 256 u of the sum of p |v|. out is rounded to
+bf16, 2^-8 relative. Pages are equal bit for bit.
 """
 import math
 
@@ -39,7 +41,7 @@ def _tol(q, cache, k, mag, want, softmax_scale=None, top=None):
     s = 1.0 / math.sqrt(D) if softmax_scale is None else abs(softmax_scale)
     A = q.double().abs().sum(-1, keepdim=True) * top * s
     n = cache[3].shape[1] * cache[0].shape[3]
-    return 2.0 ** -8 * want.abs() + (2 * 140 * U * A + (n + 100) * U) * mag + 1e-30
+    return 2.0 ** -8 * want.abs() + (2 * 140 * U * A + (n + 100 + 256) * U) * mag + 1e-30
 
 
 def _same(got, want, tag=""):

@@ -28,7 +28,7 @@ def _to(cache):
 def _tol(q, top, rows, mag, want):
     """top: the largest magnitude of a key; rows: the most that a query sees."""
     A = q.double().abs().sum(-1, keepdim=True) * top / math.sqrt(q.shape[-1])
-    return 2.0 ** -8 * want.abs() + (2 * 140 * U * A + (rows + 100) * U) * mag + 1e-30
+    return 2.0 ** -8 * want.abs() + (2 * 140 * U * A + (rows + 100 + 256) * U) * mag + 1e-30
 
 
 def _check(q, cache, k, v, lens, causal, only=None):

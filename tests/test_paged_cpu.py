@@ -212,6 +212,9 @@ def test_pools_that_differ_null_args_and_workspaces(lib):
     assert lib.prefixlm_pages_workspace_size(ctypes.byref(_pool())) == (4 * (100 + 300 + 1 + 9) + 255) // 256 * 256
     assert lib.prefixlm_paged_workspace_size(1, 1, 5, 2, 128, 16, 4) == 0
     assert lib.prefixlm_paged_workspace_size(1, 1, 16, 16, 128, 64, 64) > 0
+    # 256 sequences of 2^30 rows are 2^32 tiles of 64, which no 32 bits add up: a workgroup for each
+    assert lib.prefixlm_paged_workspace_size(256, 1, 1, 1, 128, 1024, 1 << 20) == 0
+    assert lib.prefixlm_paged_workspace_size(64, 1, 1, 1, 128, 1024, 1 << 20) > 0
 
 
 @pytest.mark.parametrize("cname,cls", [("prefixlm_page_pool", _capi.PagePool), ("prefixlm_paged_args", _capi.PagedArgs),
