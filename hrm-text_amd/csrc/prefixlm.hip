@@ -1881,13 +1881,15 @@ static int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 // R rows share a key-value head's keys. The rows of a block, which picks the kernel: one token of ungrouped heads alone;
 // up to 16 (64 x 4 key-value heads of four on 2150-3993 rows 75 us, 80 without the matrix cores); blocks of 64 from 17
 // on, most of which may be empty (24 x 4 heads, 20 rows, on 1720-3194 34 us, 40 with 32 rows of 16 in the kernel for
-// 16), where 128 fill the chip or 64 do not either, 128 (16 x 16 heads, 512 rows, on 6000-7000 945 us, 1050 by 64; 4 x 16
-// x 509 on 1433-2662 147 with two pieces a unit, 124 by 64 without pieces).
-static int pg_rows(int64_t B, int64_t Hkv, int64_t R) {
+// 16); from 65 on 128, or 64 where these start all at once, two a CU (three of 64 columns), and 128 would be one a CU: 4 x
+// 16 heads x 509 rows on 1433-2662 83 us (128: 101, 108 in pieces), of 64 columns 54; 3 x 16 78 (90); 6 x 16 x 64 columns 70
+// (82). More or fewer: 6 x 16 134 by 64, 122 by 128; 5 x 16 122 and 116; 24 x 4 x 400 145 and 126; 2 x 16 67 and 66; 16 x 16 x
+// 512 on 6000-7000 796 and 706.
+static int pg_rows(int64_t B, int64_t Hkv, int64_t R, int D) {
   if (R <= 64) return R == 1 ? 1 : R <= 16 ? 16 : 64;
   if (B >= 512 || Hkv >= 512) return 128;
-  const int64_t heads = B * Hkv;
-  return heads * ((R + 127) / 128) < 512 && heads * ((R + 63) / 64) >= 512 ? 64 : 128;
+  const int64_t blocks = B * Hkv * ((R + 63) / 64);
+  return blocks > 256 && blocks <= (D == 128 ? 512 : 768) ? 64 : 128;
 }
 // Keys of a tile
 static int pg_tile(int rows, int D) { return rows == 1 ? (D == 128 ? 64 : 128) : rows == 16 ? 4 * pkv::kKeys : 64; }
@@ -1899,7 +1901,7 @@ static int pg_tile(int rows, int D) { return rows == 1 ? (D == 128 ? 64 : 128) :
 // 512 14.6 and 15.3.
 static int pg_nwg(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
   if (B > pkv::kMaxShared || Hkv > 512) return 0;
-  const int rows = pg_rows(B, Hkv, R), tile = pg_tile(rows, D), most = rows == 1 ? 768 : 512;
+  const int rows = pg_rows(B, Hkv, R, D), tile = pg_tile(rows, D), most = rows == 1 ? 768 : 512;
   const int64_t units = B * Hkv * ((R + rows - 1) / rows), tiles = units * ((cap + tile - 1) / tile);
   if (2 * units > most || tiles <= units || tiles > 0x7fffffff) return 0;   // the kernels add the tiles up in 32 bits
   if (rows == 1 ? cap <= 768 + 5 * units : cap <= 256 || (units >= 128 && cap <= 512)) return 0;
@@ -1907,14 +1909,14 @@ static int pg_nwg(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
 }
 static size_t pg_workspace(int64_t B, int64_t Hkv, int64_t R, int D, int64_t cap) {
   const int n = pg_nwg(B, Hkv, R, D, cap);
-  return n == 0 ? 0 : align_up(sizeof(int32_t) * (B + 1)) + align_up(sizeof(float) * (size_t)n * pg_rows(B, Hkv, R) * (D + 4));
+  return n == 0 ? 0 : align_up(sizeof(int32_t) * (B + 1)) + align_up(sizeof(float) * (size_t)n * pg_rows(B, Hkv, R, D) * (D + 4));
 }
 
 template <int D>
 static void pg_launch(const pkv::Params& P, unsigned nblk, hipStream_t stream) {
   const int64_t R = (int64_t)P.S * P.G;
   const dim3 g(nblk), n(pkv::NT), c((unsigned)((P.B * P.Hkv * R + 3) / 4));
-  switch (pg_rows(P.B, P.Hkv, R)) {
+  switch (pg_rows(P.B, P.Hkv, R, D)) {
     case 1:
       if (P.nwg)
         hipLaunchKernelGGL((pkv::decode_kernel<D, pkv::NT>), g, n, 0, stream, P);
@@ -2030,7 +2032,7 @@ int prefixlm_paged_fwd(const prefixlm_paged_args* a, void* stream_) {
   P.scale_log2 = a->softmax_scale * kLog2e;
   const int64_t R = (int64_t)S * P.G;
   if (R > 0x7fffffff) return fail(PREFIXLM_ERR_INVALID, "seqlen_q=%d x %d heads of a group is too large", S, P.G);
-  const int rows = pg_rows(P.B, P.Hkv, R);
+  const int rows = pg_rows(P.B, P.Hkv, R, pool.head_dim);
   P.nrb = (int)((R + rows - 1) / rows);
   P.nwg = pg_nwg(P.B, P.Hkv, R, pool.head_dim, cap);
   P.pre = static_cast<int32_t*>(a->workspace);
