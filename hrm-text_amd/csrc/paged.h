@@ -235,13 +235,12 @@ template <bool ONCE>
 __device__ __forceinline__ u32x4 page_chunk(__amdgpu_buffer_rsrc_t rows, uint32_t off) {
   return __builtin_amdgcn_raw_buffer_load_b128(rows, (int)off, 0, ONCE ? 2 : 0);
 }
-// 16 bytes of a row of a sequence: `cached`, or `at` elements into the new rows `fresh`; 0 if it is not there, where
-// q is read instead.
-__device__ __forceinline__ u32x4 row_chunk(const Params& P, bool there, bool old, const char* cached, const bf16* fresh, int64_t at) {
+// 16 bytes of a row of a sequence: `cached`, or `at` elements into the new rows `fresh`; of zeros if it is not there, so
+// that nothing waits for what is read
+__device__ const u32x4 kNoRow = {0, 0, 0, 0};
+__device__ __forceinline__ u32x4 row_chunk(bool there, bool old, const char* cached, const bf16* fresh, int64_t at) {
   const char* p = old ? cached : reinterpret_cast<const char*>(fresh + at);
-  const u32x4 x = *reinterpret_cast<const u32x4*>(there ? p : reinterpret_cast<const char*>(P.q));
-  const uint32_t keep = there ? ~0u : 0u;
-  return u32x4{x[0] & keep, x[1] & keep, x[2] & keep, x[3] & keep};
+  return *reinterpret_cast<const u32x4*>(there ? p : reinterpret_cast<const char*>(&kNoRow));
 }
 
 // This workgroup's share of the new rows of (b, h), part `part` of `parts`, into their pages
@@ -386,8 +385,8 @@ __global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
         for (int u = 0; u < U; ++u) {
           const int jr = j + u * RPL + grp;
           const bool old = jr < len, there = old ? ok[hf] : jr < lk;
-          kw[hf][u] = row_chunk(P, there, old, kb + off + u * (RPL * D * 2), kn, (jr - len) * P.k_ss + c8);
-          vw[hf][u] = row_chunk(P, there, old, vb + off + u * (RPL * D * 2), vn, (jr - len) * P.v_ss + c8);
+          kw[hf][u] = row_chunk(there, old, kb + off + u * (RPL * D * 2), kn, (jr - len) * P.k_ss + c8);
+          vw[hf][u] = row_chunk(there, old, vb + off + u * (RPL * D * 2), vn, (jr - len) * P.v_ss + c8);
         }
       }
     }
@@ -581,8 +580,8 @@ __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
         for (int u = 0; u < HL; ++u) {
           const int jr = j + u * G::RPL + lane / CH;
           const bool old = jr < len, there = old ? held : jr < lk;
-          kw[hf * HL + u] = row_chunk(P, there, old, kb + off + u * (G::RPL * D * 2), kn, (jr - len) * P.k_ss + 8 * (lane % CH));
-          vw[hf * HL + u] = row_chunk(P, there, old, vb + off + u * (G::RPL * D * 2), vn, (jr - len) * P.v_ss + 8 * (lane % CH));
+          kw[hf * HL + u] = row_chunk(there, old, kb + off + u * (G::RPL * D * 2), kn, (jr - len) * P.k_ss + 8 * (lane % CH));
+          vw[hf * HL + u] = row_chunk(there, old, vb + off + u * (G::RPL * D * 2), vn, (jr - len) * P.v_ss + 8 * (lane % CH));
         }
       }
     }
@@ -854,8 +853,8 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
         if (j < min(len, k1) && !held) s_hole = 1;
         const char *kb = reinterpret_cast<const char*>(P.kp + at), *vb = reinterpret_cast<const char*>(P.vp + at);
         const int jk = j + (srow & 15), jv = j + (vrow & 15);
-        ks[n] = row_chunk(P, jk < len ? held : jk < k1, jk < len, kb + koff, kn, (jk - len) * P.k_ss + 8 * sch);
-        vs[n] = row_chunk(P, jv < len ? held : jv < k1, jv < len, vb + voff, vn, (jv - len) * P.v_ss + 8 * sch);
+        ks[n] = row_chunk(jk < len ? held : jk < k1, jk < len, kb + koff, kn, (jk - len) * P.k_ss + 8 * sch);
+        vs[n] = row_chunk(jv < len ? held : jv < k1, jv < len, vb + voff, vn, (jv - len) * P.v_ss + 8 * sch);
       }
     }
   };
