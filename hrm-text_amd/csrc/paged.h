@@ -529,7 +529,7 @@ struct Geo {
 // R <= 16. Each wave walks 32 keys at a time by itself: S^T = K Q^T by 16 keys, then O^T += V^T P^T, K and V through LDS
 // of its own, so that both are read from memory in whole rows (K straight into the matrix cores, 64 bytes of 16 rows a
 // load, took 105 us where this takes 92). Bound by memory: 48 x 2 key-value heads of eight query heads on 6900-12700
-// rows, 479 MB, 85 us with the combine, 5.6 TB/s. Two workgroups a CU (72 KB of LDS, 212 registers).
+// rows, 479 MB, 81 us, 5.9 TB/s, and 5 the combine. Two workgroups a CU (72 KB of LDS, 212 registers).
 template <int D>
 __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
   using G = Geo<D>;
