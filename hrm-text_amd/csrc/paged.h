@@ -742,15 +742,16 @@ __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
 // ---- more rows ------------------------------------------------------------------------------------
 // Workgroup = 32 QW rows of (b, h) over a unit's or a piece's keys: QW waves along the rows and KW = 4 / QW along the
 // keys; a staged tile of 64 keys serves all of them. S^T = K Q^T with the row as the lane column, V^T from transposing
-// reads. What it is made of, as 4 x 16 heads x 509 rows on 1433-2662 went from 124 us to 84 (420 TFLOP/s; 16 x 16 x 512
-// on 6000-7000 from 890 to 703, 640 TFLOP/s):
-//  - the weights go into P V as two bf16 terms, each rounded to nearest: off by 2^-16 of a weight, a 256th of out's own
-//    rounding, where three would hold all 24 bits for a third more matrix products;
+// reads. 4 x 16 heads x 509 rows on 1582-2028 take 84 us (400 TFLOP/s; first 124), 16 x 16 x 512 on 6053-6782 812 (553
+// TFLOP/s; first 890):
+//  - the weights go into P V as three bf16 terms, the upper 8 bits of what the terms before leave, which hold the fp32
+//    value as in the other kernels. Two, each rounded to nearest, took 75 and 706 us, but left up to 90 2^-24 of sums that
+//    cancel and three times as many results off their nearest bf16 as a softmax in fp32 leaves;
 //  - what a row's weights are relative to (m_run) is raised only once one passes it by 2^kAbove: any reference does;
 //  - the scale is applied with that reference in one fma: to |scale|, a negative one having turned q's signs;
 //  - tiles in one page or of new rows alone are loaded off one base, with the bounds that the buffer checks.
-// Bound by the waves' own chains (two a SIMD): of an iteration's 4200 cycles for two tiles the matrix cores take 1540, the
-// vector instructions 1900, loads and stores alone 2600. Loads that reach further ahead (one word of each line, two to five
+// Bound by the waves' own chains (two a SIMD): of an iteration's 4700 cycles for two tiles the matrix cores take 2050, the
+// vector instructions 2200, loads and stores alone 2600. Loads that reach further ahead (one word of each line, two to five
 // tiles before) made it 6 to 8% slower.
 template <int D, int QW>
 struct TileGeo {
@@ -970,27 +971,34 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
           u32x4 xt[2 * NDT];
           xt[0] = lds_read_xt<RSD>(vx, 0, 0);
           xt[1] = lds_read_xt<RSD>(vx, 0, 1);
-          // 16 keys at a time: P's two bf16 terms times V
+          // 16 keys at a time: the weights' three bf16 terms, which add up to their fp32 bits, times V
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             float e[8], ps = 0.f;
-            bf16x8 pt[2];
+            bf16x8 pt[3];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               e[i] = __builtin_amdgcn_exp2f(c * sacc[x][8 * half + i] - m_use);
               ps += e[i];
             }
             l_run += ps;
-            pt[0] = cvt8(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] -= (float)pt[0][i];   // exact
-            pt[1] = cvt8(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]);
+            for (int n = 0; n < 3; ++n) {
+              u32x4 hi;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                hi[i] = pack_hi(__builtin_bit_cast(uint32_t, e[2 * i]), __builtin_bit_cast(uint32_t, e[2 * i + 1]));
+              pt[n] = __builtin_bit_cast(bf16x8, hi);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)   // exact
+                e[i] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, e[i]) & 0xffff0000u);
+            }
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) {
               const int z = NDT * half + dt;
               if (z + 2 < 2 * NDT) xt[z + 2] = lds_read_xt<RSD>(vx, (z + 2) / NDT, (z + 2) % NDT);
 #pragma unroll
-              for (int n = 0; n < 2; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[z]), pt[n], oacc[dt]);
+              for (int n = 0; n < 3; ++n) oacc[dt] = mfma32x32x16(__builtin_bit_cast(bf16x8, xt[z]), pt[n], oacc[dt]);
             }
           }
         }
