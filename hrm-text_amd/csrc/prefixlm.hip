@@ -2037,11 +2037,11 @@ int prefixlm_paged_fwd(const prefixlm_paged_args* a, void* stream_) {
   P.nwg = pg_nwg(P.B, P.Hkv, R, pool.head_dim, cap);
   P.pre = static_cast<int32_t*>(a->workspace);
   P.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + align_up(sizeof(int32_t) * ((size_t)P.B + 1)));
-  const int64_t units = (int64_t)P.B * P.Hkv;
-  if (units > 0x7ffffff0 || P.nrb > 0x7fffffff / ((units + 7) / 8 * 8) || !launchable((units + 7) / 8 * 8 * P.nrb, 512) ||
-      !launchable((units * R + 3) / 4, 256))
+  // pieces and their join are few; without them the first launch is the only one
+  const int64_t units = (int64_t)P.B * P.Hkv, eighths = (units + 7) / 8 * 8;
+  if (!P.nwg && (units > 0x7ffffff0 || P.nrb > 0x7fffffff / eighths || !launchable(eighths * P.nrb, rows == 1 ? 512 : pkv::NT)))
     return fail(PREFIXLM_ERR_INVALID, "grid too large");
-  const int64_t nblk = P.nwg ? P.nwg : (units + 7) / 8 * 8 * P.nrb;
+  const int64_t nblk = P.nwg ? P.nwg : eighths * P.nrb;
   rc = pg_allow_lds();
   if (rc) return rc;
   (void)hipGetLastError();
