@@ -2162,11 +2162,14 @@ int prefixlm_pages_fork(const prefixlm_pages_args* a, void* stream_) {
   P.parents = a->src;
   P.table_sb = p.table_stride;
   P.N = p.batch; P.M = p.columns; P.P = p.num_pages;
-  // 64 KB of LDS
+  // 64 KB of LDS; as many columns a workgroup as a launch of a very wide table takes
   P.TC = std::min(p.batch <= 1024 ? 16 : p.batch <= 2048 ? 8 : p.batch <= 4096 ? 4 : 2, p.columns);
+  auto nblk = [&] { return ((int64_t)p.columns + P.TC - 1) / P.TC; };
+  while (!launchable(nblk(), pages::NTH) && 2 * P.TC * p.batch <= 16384) P.TC *= 2;
+  if (!launchable(nblk(), pages::NTH)) return fail(PREFIXLM_ERR_INVALID, "a table of %d x %d is too large", p.batch, p.columns);
   (void)hipGetLastError();
-  hipLaunchKernelGGL(pages::fork_kernel, dim3((unsigned)((p.columns + P.TC - 1) / P.TC)), dim3(pages::NTH),
-                     sizeof(int32_t) * P.N * P.TC, reinterpret_cast<hipStream_t>(stream_), P);
+  hipLaunchKernelGGL(pages::fork_kernel, dim3((unsigned)nblk()), dim3(pages::NTH), sizeof(int32_t) * P.N * P.TC,
+                     reinterpret_cast<hipStream_t>(stream_), P);
   return pages_end("page fork");
 }
 

@@ -1,4 +1,5 @@
-"""GPU: attention over pages with more rows than a launch of a wave for each could take, where no such launch is made.
+"""GPU: attention over pages with more rows than a launch of a wave for each could take, where no such launch is made, and
+forks of the widest table.
 
 Tolerance: as in tests/test_gpu_paged_holes.py."""
 import math
@@ -6,7 +7,7 @@ import math
 import pytest
 import torch
 
-from prefixlm import PagedKVCache, flash_attn_with_paged_kvcache
+from prefixlm import PagedKVCache, flash_attn_with_paged_kvcache, paged_kvcache_fork
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -37,3 +38,20 @@ def test_more_rows_than_a_wave_each():
     out = flash_attn_with_paged_kvcache(q, cache, cache_seqlens=n)
     for a in out[0].split(1 << 19):
         assert torch.equal(a, out[0, :2].repeat(a.shape[0] // 2, 1, 1))
+
+
+@pytest.mark.parametrize("columns", [1 << 26, (1 << 26) - 7])
+def test_fork_of_2_to_30_rows(columns):
+    g = torch.Generator().manual_seed(2)
+    table = torch.full((2, columns), -1, dtype=torch.int32, device=DEV)
+    at = torch.cat((torch.randint(0, columns, (1000,), generator=g), torch.tensor([0, 1 << 25, columns - 17, columns - 1]))).to(DEV)
+    table[1, at] = torch.arange(at.numel(), dtype=torch.int32, device=DEV)
+    table[0, columns - 2] = at.numel()
+    P = at.numel() + 1
+    refs = torch.bincount(table.clamp_min(-1).add(1).view(-1), minlength=P + 1)[1:].int()
+    pages = [torch.zeros(1, P, 1, 16, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    cache = PagedKVCache(*pages, refs.clone(), table.clone())
+    paged_kvcache_fork(cache, torch.tensor([1, 1], dtype=torch.int32, device=DEV))
+    assert torch.equal(cache.page_table[0], table[1]) and torch.equal(cache.page_table[1], table[1])
+    refs = torch.bincount(table[1].add(1), minlength=P + 1)[1:].int()
+    assert torch.equal(cache.refs, 2 * refs)

@@ -28,3 +28,9 @@ def test_attention_past_a_launch(lib, B, Hkv, G, S):
     a = _capi.PagedArgs(pool=_pool(batch=B, num_kv_heads=Hkv), q=FAKE, out=FAKE, cache_seqlen=3, seqlen_q=S, num_heads=G * Hkv,
                         softmax_scale=0.1, workspace=FAKE, workspace_bytes=1 << 62)
     assert lib.prefixlm_paged_fwd(ctypes.byref(a), None) == 1 and "too large" in _capi.last_error()
+
+
+@pytest.mark.parametrize("N,columns", [(600, 1 << 26), (1024, 1 << 26), (8192, 1 << 24)])
+def test_fork_past_a_launch(lib, N, columns):
+    a = _capi.PagesArgs(pool=_pool(batch=N, columns=columns), src=FAKE)
+    assert lib.prefixlm_pages_fork(ctypes.byref(a), None) == 1 and "too large" in _capi.last_error()
