@@ -181,10 +181,12 @@ def flash_attn_with_paged_kvcache(q: Tensor, cache: PagedKVCache, k: Optional[Te
     """Attention of q [B, S, Hq, D] bf16 over one layer of a cache in pages, one table row for each of q's
     batch; Hq is a multiple of the cache's heads Hkv, and query head h reads key-value head
     ``h // (Hq // Hkv)``. k, v [B, S, Hkv, D] (or None: the cache only) are new rows behind the first
-    ``cache_seqlens`` rows (an int, or int32 [B] on the GPU, where values outside [0, columns * page_size] count
+    ``cache_seqlens`` rows (an int in [0, columns * page_size], or int32 [B] on the GPU, where values outside count
     as the nearest of the two; None = 0). They are attended as given, and stored where the sequence holds the
-    page alone (``paged_kvcache_reserve`` sees to it); rows past the table's end are dropped. Cached rows
-    without a page are not seen. ``causal``: query i sees keys j <= rows - S + i, as in
+    page alone (``paged_kvcache_reserve`` sees to it); rows past the table's end are dropped. All S rows count in
+    every sequence: where sequences have fewer and are padded behind, pass ``causal``, with which no row sees those
+    behind it; without it the padding is seen as keys, so only sequences with the same number of new rows go into one
+    call. Cached rows without a page are not seen. ``causal``: query i sees keys j <= rows - S + i, as in
     ``flash_attn_with_kvcache``. A query that sees no key gives a row of 0. Forward only: the call has
     no gradient."""
     if cache_seqlens is None:

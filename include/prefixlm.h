@@ -437,7 +437,8 @@ typedef struct prefixlm_page_pool {
 /* Attention of q [B, S, num_heads, head_dim] over a layer's pages (B = pool.batch; num_heads a multiple of
  * num_kv_heads: query head h reads key-value head h / (num_heads / num_kv_heads)). k, v [B, S,
  * num_kv_heads, head_dim] (or both NULL) are rows cache_seqlens[b] .. + S - 1 of their sequences: attended as given,
- * and stored in pages that refs counts once; those at columns * page_size and beyond are dropped. Cached rows
+ * and stored in pages that refs counts once; those at columns * page_size and beyond are dropped. All S rows count in
+ * every sequence, as keys too: rows padded behind a sequence's own are hidden by is_causal alone. Cached rows
  * without a page are not seen. Lengths outside [0, columns * page_size] count as the nearest of the two.
  * is_causal: query i sees keys j <= rows - S + i. A query that sees no key gives 0. Unit stride over
  * head_dim; other strides multiples of 8; pointers 16-byte aligned. */
