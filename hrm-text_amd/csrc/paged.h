@@ -19,8 +19,10 @@
 //   tile    : more rows: 64 or 128 a workgroup, which share tiles of the keys in LDS;
 //   combine : joins the pieces of a unit.
 //
-// A unit is a block of rows of one (sequence, key-value head); its keys are tiles. Where units are few, each is cut
-// into pieces, as many as its sequence's tiles are worth, so that sequences of any lengths end together (Sched).
+// A unit is a block of rows of one (sequence, key-value head); its keys are tiles. Where units are few (up to 384 for one
+// row, 256 for more, of up to 256 sequences), each is cut into pieces, as many as its sequence's tiles are worth, so that
+// sequences of any lengths end together (Sched). Where they are many, each is one workgroup, whatever its length: a batch
+// of short sequences and a very long one then ends with the long one's units alone.
 #pragma once
 #include "common.h"
 #include "kvcache.h"
@@ -99,9 +101,9 @@ __device__ __forceinline__ float rows_sum(float x) {
 // those that a few bisections try, at which all pieces together are at most P.nwg: the pieces are then of nearly
 // the same length, whatever the sequences' are, and all in flight at once. Each wave finds c by itself, lane i
 // holding sequences i, i + 64, ... It costs 1 us of a call and saves what the longest sequence took more than the
-// others with as many pieces for each (48 x 2 heads on 6900-12700 rows 92 us with eight, now 85; 3 x 12 on 16000-29000 72
-// with 16, now 65). Dealing the tiles out evenly, wherever units begin and end, was as fast for one row and slower for
-// several (24 x 4 heads of 20 rows 48 us where pieces took 40): a workgroup then begins and ends two units.
+// others with as many pieces for each (48 x 2 heads of eight on 7284-12554 rows 92 us with eight, now 84). Dealing the
+// tiles out evenly, wherever units begin and end, was as fast for one row and slower for several (24 x 4 heads of 20 rows 48
+// us where pieces took 40): a workgroup then begins and ends two units.
 template <int RB, int TS>
 struct Sched {
   int b, h, rb, len, first, count, piece, pieces, wg;
@@ -116,8 +118,8 @@ struct Sched {
     pieces = 1;
     if (P.nwg == 0) {
       // Row blocks of one (b, h) eight indices apart, on one XCD. The longest sequences first (16 x 16 x 512 rows on
-      // 1000-7000 612 us in their own order, 506 so), and of an XCD's 64 workgroups that start at once, two a CU, the later
-      // 32 the other way round, so that a long one shares its CU with a short one (4 x 16 x 509 on 1433-2662 2 us of 105)
+      // 1109-6998 645 us in their own order, 534 so), and of an XCD's 64 workgroups that start at once, two a CU, the later
+      // 32 the other way round, so that a long one shares its CU with a short one (4 x 16 x 509 on 1454-2353 93 us, 89 so)
       int j = (int)(blockIdx.x >> 3);
       const int most = min((int)(gridDim.x >> 3), 64);
       if (RB >= 64 && j >= 32 && j < most) j = 31 + most - j;
@@ -264,7 +266,8 @@ __device__ __forceinline__ void append_share(const Params& P, int b, int h, int 
 // Rows [r0, r1) over keys [k0, k1) without the matrix cores: 16 lanes a row, key by key. For pieces
 // whose values hold an infinity or NaN (0 * inf in P V would reach rows that must not see the key), and
 // for scores that pass fp32's range before the softmax scale, or whose largest is about -3e38: here the
-// scale comes first. down: what the unit's other pieces take the weights below.
+// scale comes first. A scale of 0, which hides whether they did, brings every row here: right, and slow.
+// down: what the unit's other pieces take the weights below.
 template <int D>
 __device__ __forceinline__ void walk_rows(const Params& P, int b, int h, int r0, int r1, int k0, int k1, int len, float down, float* part) {
   constexpr int E = D / 16;
@@ -334,9 +337,9 @@ __device__ __forceinline__ float lanes_sum(float x) {
 }
 
 // R = 1. Each wave walks 16 NH keys at a time by itself; D / 8 lanes hold a key row, 16 bytes each. Bound by memory
-// where there is much to read (64 x 16 heads on 2150-3993 rows, 1.6 GB: 257 us, 6.2 TB/s; 3 x 12 on 16000-29000 65 us,
-// 5.6), by the chain of length, page, keys, joining where there is little (16 heads on 900 rows 9.8 us with the
-// combine). The matrix cores (stream) are as fast on the former and 0.6 to 1.2 us slower on the latter.
+// where there is much to read (64 x 16 heads on 2163-3972 rows, 1.58 GB: 250 us, 6.3 TB/s; 3 x 12 on 20735-25651, 428 MB,
+// 69 us, 6.2), by the chain of length, page, keys, joining where there is little (16 heads on 783 rows 6.0 us, and 3.8
+// the combine). The matrix cores (stream) are as fast on the former and 0.6 to 1.2 us slower on the latter.
 template <int D, int NTH>
 __global__ __launch_bounds__(NTH) void decode_kernel(Params P) {
   constexpr int NWAVE = NTH / 64, CH = D / 8, RPL = 64 / CH, NH = D == 128 ? 1 : 2, U = 16 / RPL;
@@ -528,7 +531,7 @@ struct Geo {
 
 // R <= 16. Each wave walks 32 keys at a time by itself: S^T = K Q^T by 16 keys, then O^T += V^T P^T, K and V through LDS
 // of its own, so that both are read from memory in whole rows (K straight into the matrix cores, 64 bytes of 16 rows a
-// load, took 105 us where this takes 92). Bound by memory: 48 x 2 key-value heads of eight query heads on 6900-12700
+// load, took 105 us where this took 92 then). Bound by memory: 48 x 2 key-value heads of eight query heads on 7284-12554
 // rows, 479 MB, 81 us, 5.9 TB/s, and 5 the combine. Two workgroups a CU (72 KB of LDS, 212 registers).
 template <int D>
 __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
@@ -742,11 +745,11 @@ __global__ __launch_bounds__(NT, 2) void stream_kernel(Params P) {
 // ---- more rows ------------------------------------------------------------------------------------
 // Workgroup = 32 QW rows of (b, h) over a unit's or a piece's keys: QW waves along the rows and KW = 4 / QW along the
 // keys; a staged tile of 64 keys serves all of them. S^T = K Q^T with the row as the lane column, V^T from transposing
-// reads. 4 x 16 heads x 509 rows on 1582-2028 take 84 us (400 TFLOP/s; first 124), 16 x 16 x 512 on 6053-6782 812 (553
-// TFLOP/s; first 890):
+// reads. 4 x 16 heads x 509 rows on 1454-2353 take 89 us (402 TFLOP/s; first 124), on 1582-2028 84, 16 x 16 x 512 on
+// 6053-6782 808 (557 TFLOP/s; first 890):
 //  - the weights go into P V as three bf16 terms, the upper 8 bits of what the terms before leave, which hold the fp32
-//    value as in the other kernels. Two, each rounded to nearest, took 75 and 706 us, but left up to 90 2^-24 of sums that
-//    cancel and three times as many results off their nearest bf16 as a softmax in fp32 leaves;
+//    value as in the other kernels. Two, each rounded to nearest, took 75 and 706 us of the latter two, but left up to 90
+//    2^-24 of sums that cancel and three times as many results off their nearest bf16 as a softmax in fp32 leaves;
 //  - what a row's weights are relative to (m_run) is raised only once one passes it by 2^kAbove: any reference does;
 //  - the scale is applied with that reference in one fma: to |scale|, a negative one having turned q's signs;
 //  - tiles in one page or of new rows alone are loaded off one base, with the bounds that the buffer checks.
@@ -1107,7 +1110,7 @@ __global__ __launch_bounds__(NT, 2) void tile_kernel(Params P) {
 
 // One wave per (b, h, r) of a unit of several pieces: lane i weighs the i-th, and D / 4 lanes a piece add their four
 // columns, 64 pieces at a time. Bound by its loads one after another, what the sequence's units were cut into, then the
-// pieces: 3.3 us with the launch for 16 rows of 14 pieces, 4.7 for 768 of five.
+// pieces: 3.8 us with the launch for 16 rows of 13 pieces, 4.6 for 768 of five.
 template <int D, int RB>
 __global__ __launch_bounds__(256) void combine_kernel(Params P) {
   constexpr int L4 = D / 4, NG = 64 / L4;

@@ -251,7 +251,7 @@ struct ForkParams {
   int N, M, P, TC;          // TC: columns a workgroup
 };
 // A workgroup has TC columns of every sequence: all entries are read before one is written. Latency: 64 sequences of 37
-// columns 3.1 us. Counts change by integer atomics, whose order changes nothing.
+// columns 3.2 us. Counts change by integer atomics, whose order changes nothing.
 __global__ __launch_bounds__(NTH) void fork_kernel(ForkParams P) {
   extern __shared__ int32_t s_new[];   // [N, TC]
   const int c0 = blockIdx.x * P.TC, total = P.N * P.TC;
@@ -280,7 +280,7 @@ struct FreeParams {
   int64_t table_sb;
   int N, M, P, ps_log2, keep_const;
 };
-// thread = one entry: 64 x 32 in 2.6 us
+// thread = one entry: 64 x 32 in 4.4 us, of which the launch is most
 __global__ __launch_bounds__(256) void free_kernel(FreeParams P) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (int64_t)P.N * P.M) return;
@@ -304,7 +304,7 @@ struct CompactParams {
 };
 // One workgroup. U pages are in use: the i-th of them from U on moves to the i-th free one below U. Pools of up to
 // 16384 pages stay in registers between the two looks at their counts; the free ones meet the others in LDS. Bound by
-// its loads, two scans and stores: 1500 pages 6.1 us, 400 5.5.
+// its loads, two scans and stores: 1500 pages 6.0 us, 400 5.5.
 __global__ __launch_bounds__(NTH) void compact_kernel(CompactParams P) {
   __shared__ int s_scan[NTH / 64];
   __shared__ uint16_t s_hole[kLook / 2];

@@ -1879,12 +1879,13 @@ static int table_check(const prefixlm_page_pool& p) {
 static int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
 
 // R rows share a key-value head's keys. The rows of a block, which picks the kernel: one token of ungrouped heads alone;
-// up to 16 (64 x 4 key-value heads of four on 2150-3993 rows 75 us, 80 without the matrix cores); blocks of 64 from 17
-// on, most of which may be empty (24 x 4 heads, 20 rows, on 1720-3194 34 us, 40 with 32 rows of 16 in the kernel for
-// 16); from 65 on 128, or 64 where these start all at once, two a CU (three of 64 columns), and 128 would be one a CU: 4 x
-// 16 heads x 509 rows on 1433-2662 83 us (128: 101, 108 in pieces), of 64 columns 54; 3 x 16 78 (90); 6 x 16 x 64 columns 70
-// (82). More or fewer: 6 x 16 134 by 64, 122 by 128; 5 x 16 122 and 116; 24 x 4 x 400 145 and 126; 2 x 16 67 and 66; 16 x 16 x
-// 512 on 6000-7000 796 and 706.
+// up to 16 (64 x 4 key-value heads of four on 2163-3972 rows 75 us, 80 without the matrix cores); blocks of 64 from 17
+// on, most of which may be empty (24 x 4 heads, 20 rows, on 1729-3063 32 us; with 32 rows of 16 in the kernel for 16 it
+// took 40 for 34 then); from 65 on 128, or 64 where these start all at once on 256 CUs, two a CU (three of 64 columns), and
+// 128 would be one a CU: 4 x 16 heads x 509 rows on 1582-2028 84 us (128: 106), of 64 columns 52 (76); 3 x 16 74 (88); 6 x 16
+// x 64 columns 71 (85). More or fewer: 6 x 16 130 by 64, 129 by 128; 5 x 16 123 and 116; 24 x 4 x 400 on 1437-2614 140 and
+// 124; 2 x 16 64 and 61; 16 x 16 x 512 on 6053-6782 923 and 807. Only the call's sizes are known here: on few cached rows the
+// blocks of 128, which are then cut, cost more than they save (16 heads x 900 rows on 119 41 us, 39 by 64).
 static int pg_rows(int64_t B, int64_t Hkv, int64_t R, int D) {
   if (R <= 64) return R == 1 ? 1 : R <= 16 ? 16 : 64;
   if (B >= 512 || Hkv >= 512) return 128;
@@ -1893,9 +1894,9 @@ static int pg_rows(int64_t B, int64_t Hkv, int64_t R, int D) {
 }
 // Keys of a tile
 static int pg_tile(int rows, int D) { return rows == 1 ? (D == 128 ? 64 : 128) : rows == 16 ? 4 * pkv::kKeys : 64; }
-// The workgroups that the units share, 0: one for each unit. Two a CU, three of the smaller ones for one row (16 heads x
-// 12 on 16000-29000 rows 65 us with 768, 63 with 512, 66 with 1024), unless units are as good as enough, or their
-// keys take less time than the combine's launch. One row, one workgroup of 512 threads a unit against 768 that
+// The workgroups that the units share, 0: one for each unit. Two a CU, three of the smaller ones for one row (3 x 12 heads
+// on 20735-25651 rows 74 us with 768, 71 with 512, 73 with 1024), unless units are as good as enough, or their
+// keys, as many as the table has room for, take less time than the combine's launch. One row, one workgroup of 512 threads a unit against 768 that
 // share: 16 units of 512 rows 7.5 and 9.5 us, of 1024 11.6 and 9.9; 64 of 1024 13.7 and 14.6, of 1536 18.5 and 16.2;
 // 128 of 1024 15.1 and 18.5; 256 of 2048 35.6 and 39. More rows: 16 units of 256 8.8 and 11.0, of 512 13.0 and 11.4; 128 of
 // 512 14.6 and 15.3.
