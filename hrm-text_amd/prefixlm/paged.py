@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from typing import NamedTuple, Optional, Union
 
 import torch
@@ -111,17 +112,26 @@ def _pool(k_pages: Optional[Tensor], v_pages: Optional[Tensor], refs: Tensor, pa
                           L, P, H, ps, D, N, M)
 
 
+def _whole(x, name: str) -> int:
+    try:
+        return operator.index(x)
+    except TypeError:
+        raise ValueError(f"{name} must be a whole number or a tensor (got {x!r})") from None
+
+
 def _rows(x: Union[int, Tensor, None], n: int, dev, name: str):
     """(int32 [n] on dev, or None; the constant in its place)."""
-    if x is None:
-        return None, 0
     if not isinstance(x, Tensor):
-        return None, max(-1, min(int(x), 2**31 - 1))
+        return None, max(-1, min(_whole(x, name), 2**31 - 1))
     if x.dtype not in (torch.int32, torch.int64) or x.numel() != n or x.device != dev:
         raise ValueError(f"{name} must be an int or int32 [{n}] on {dev} (got {x.dtype} {tuple(x.shape)} on {x.device})")
     if x.dtype == torch.int64:   # outside int32 is outside every cache
         x = x.clamp(-2**31, 2**31 - 1).to(torch.int32)
     return x.reshape(-1).contiguous(), 0
+
+
+def _given(x: Optional[Tensor], n: int, dev, name: str) -> Optional[Tensor]:
+    return None if x is None else _rows(x, n, dev, name)[0]
 
 
 # ---- attention ------------------------------------------------------------------------------
@@ -151,7 +161,7 @@ def paged_kvcache_attn(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], k_pa
             _check4(x, name)
             if tuple(x.shape) != (B, S, Hkv, D) or x.device != dev:
                 raise ValueError(f"{name} must be [{B}, {S}, {Hkv}, {D}] on {dev} (got {tuple(x.shape)} on {x.device})")
-    lens, _ = _rows(cache_seqlens, B, dev, "cache_seqlens")
+    lens = _given(cache_seqlens, B, dev, "cache_seqlens")
     _apart((k_pages, v_pages, refs, page_table), [x for x in (q, k, v, lens) if x is not None])
     if lens is None and not 0 <= cache_seqlen <= cap:
         raise ValueError(f"cache_seqlens = {cache_seqlen} is outside [0, {cap}]")
@@ -198,7 +208,7 @@ def flash_attn_with_paged_kvcache(q: Tensor, cache: PagedKVCache, k: Optional[Te
             return out
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(q.shape[-1])
-    lens, n = (cache_seqlens, 0) if isinstance(cache_seqlens, Tensor) else (None, int(cache_seqlens))
+    lens, n = (cache_seqlens, 0) if isinstance(cache_seqlens, Tensor) else (None, _whole(cache_seqlens, "cache_seqlens"))
     return paged_kvcache_attn(q, k, v, *cache, lens, n, int(layer), bool(causal), float(softmax_scale))
 
 
@@ -221,8 +231,7 @@ def _reserve(k_pages: Tensor, v_pages: Tensor, refs: Tensor, page_table: Tensor,
     _check_pages(k_pages, v_pages)
     dev, N = k_pages.device, page_table.shape[0]
     _check_table(refs, page_table, k_pages.shape[1], dev, MAX_SEQUENCES)
-    lens, _ = _rows(cache_seqlens, N, dev, "cache_seqlens")
-    new, _ = _rows(new_rows, N, dev, "new_rows")
+    lens, new = _given(cache_seqlens, N, dev, "cache_seqlens"), _given(new_rows, N, dev, "new_rows")
     _apart((k_pages, v_pages, refs, page_table), [x for x in (lens, new) if x is not None])
     short = torch.empty(N, dtype=torch.int32, device=dev)
     _call("prefixlm_pages_reserve", dev, _pool(k_pages, v_pages, refs, page_table), True, rows=_ptr(lens), row_const=cache_seqlen,
@@ -262,7 +271,7 @@ def _fork(refs: Tensor, page_table: Tensor, parents: Tensor) -> None:
     if dev.type != "cuda":
         raise ValueError(f"the cache must be on a GPU (got {dev})")
     _check_table(refs, page_table, None, dev, MAX_SEQUENCES)
-    src, _ = _rows(parents, page_table.shape[0], dev, "parents")
+    src = _given(parents, page_table.shape[0], dev, "parents")
     _apart((refs, page_table), (src,))
     _call("prefixlm_pages_fork", dev, _pool(None, None, refs, page_table, (1, refs.shape[0], 1, 16, 64)), src=_ptr(src))
 
@@ -290,7 +299,7 @@ def _free(refs: Tensor, page_table: Tensor, page_size: int, keep_rows: Optional[
     if dev.type != "cuda":
         raise ValueError(f"the cache must be on a GPU (got {dev})")
     _check_table(refs, page_table, None, dev)
-    keep, _ = _rows(keep_rows, page_table.shape[0], dev, "keep_rows")
+    keep = _given(keep_rows, page_table.shape[0], dev, "keep_rows")
     _apart((refs, page_table), () if keep is None else (keep,))
     _call("prefixlm_pages_free", dev, _pool(None, None, refs, page_table, (1, refs.shape[0], 1, page_size, 64)), rows=_ptr(keep),
           row_const=keep_row)
@@ -353,7 +362,7 @@ def _copy(k_pages: Tensor, v_pages: Tensor, k_source: Optional[Tensor], v_source
     if src.dim() != 1 or src.shape != dst.shape:
         raise ValueError(f"src {tuple(src.shape)} and dst {tuple(dst.shape)} must be lists of the same length")
     n = src.numel()
-    src, dst = _rows(src, n, dev, "src")[0], _rows(dst, n, dev, "dst")[0]
+    src, dst = _given(src, n, dev, "src"), _given(dst, n, dev, "dst")
     if not n:
         return
     _apart(pools, (src, dst))
